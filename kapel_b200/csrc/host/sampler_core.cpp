@@ -222,6 +222,9 @@ int filters_alive(const double* l, int n, const Settings& s, Alive& a) {
             }
         kth = heap.front();
     }
+    // An infinite logit leaves no probabilities to filter by (its own is inf - inf): the first of them stands.
+    for (int i = 0; i < n; ++i)
+        if (l[i] > std::numeric_limits<double>::max()) return s.top_p <= 0.0 ? 0 : i;
     const size_t room = kth == NEG_INF ? (size_t)finite : 2 * (size_t)s.top_k;
     a.idx.reserve(room); a.l.reserve(room);
     for (int i = 0; i < n; ++i)
