@@ -441,11 +441,12 @@ class Scheduler:
     def _choose_on_device(self, logits, producing: List[int], rows: List[int]):
         """The chosen tokens as an int32 device tensor, a token a row of `logits` (rows outside `rows`
         belong to nobody and get the largest logit), enqueued and not waited for; None where the
-        choice needs the host (filters, penalties) or the logits are not on a device."""
+        choice needs the host (penalties) or the logits are not on a device."""
         if not producing or not getattr(logits, "is_cuda", False):
             return None
         entries = [self.entries[rid] for rid in producing]
-        if not all(e.request.sampling.on_device() for e in entries):
+        plain = all(e.request.sampling.on_device() for e in entries)
+        if not plain and not all(e.request.sampling.filtered_on_device() for e in entries):
             return None
         import torch
 
@@ -454,6 +455,8 @@ class Scheduler:
         if all(e.request.sampling.is_greedy() for e in entries):
             return K.sample(logits)
         n = int(logits.shape[0])
+        if not plain:
+            return self._sample_filtered(logits, rows, entries, n) if logits.shape[1] <= K.SAMPLE_FILTERED_VOCAB else None
         temps, us = [0.0] * n, [0.0] * n
         for i, e in zip(rows, entries):
             temps[i] = max(0.0, e.request.sampling.temperature)
@@ -463,9 +466,29 @@ class Scheduler:
         self._sample_inputs = host                  # pinned memory must outlive its copy
         return K.sample(logits, dev[0], dev[1])
 
+    def _sample_filtered(self, logits, rows: List[int], entries, n: int):
+        """Rows with top_k, top_p or min_p, beside rows without: one copy of the settings, one launch, in 64 bits like the host's choice."""
+        import torch
+
+        from .. import kernels as K
+
+        table = np.zeros((5, n), np.float64)                # temperature, top_p, min_p, uniform; top_k in 32 bits
+        table[1] = 1.0
+        top_k = table[4].view(np.int32)
+        for i, e in zip(rows, entries):
+            s = e.request.sampling
+            temperature = max(0.0, s.temperature)           # a row of its own that is greedy stays greedy
+            u = e.sampler.uniform() if temperature > 0 else 0.0
+            table[:4, i] = temperature, s.top_p, s.min_p, u
+            top_k[i] = min(max(0, int(s.top_k or 0)), 2 ** 31 - 1)
+        host = torch.from_numpy(table).pin_memory()
+        dev = host.to(logits.device, non_blocking=True)
+        self._sample_inputs = host                          # pinned memory must outlive its copy
+        return K.sample_filtered(logits, dev[0], dev[4].view(torch.int32)[:n], dev[1], dev[2], dev[3])
+
     def _choose(self, logits, producing: List[int], rows: Optional[List[int]] = None) -> List[int]:
-        """One token per producing request: on the device when only the logits decide (greedy
-        without penalties, or a plain temperature; engine.rs:584-597), else on the host in
+        """One token per producing request: on the device when the logits and the request's settings
+        decide (no penalties; engine.rs:584-597), else on the host in
         64-bit with the request's own sampler (engine.rs:599-616). `rows` names each request's
         row of `logits` (by default row i is request i's)."""
         if not producing:

@@ -179,6 +179,14 @@ def _need(t: torch.Tensor, what: str, dtype=None, shape=None) -> torch.Tensor:
     return t
 
 
+def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Launches go to the current device's stream: every tensor has to be there."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: a tensor on {t.device} while device {here} is the current one")
+
+
 def _f(x: float) -> ctypes.c_float:
     return ctypes.c_float(float(x))
 
@@ -2033,12 +2041,36 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor] = None, uni
     return out
 
 
+SAMPLE_FILTERED_VOCAB = 1 << 19         # the largest vocabulary `sample_filtered` takes
+
+
+def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
+                    uniform: torch.Tensor) -> torch.Tensor:
+    """One token a row of float32 logits [rows, vocab], by the host sampler's rules (`sampling.Sampler`) and in 64 bits as there: the
+    first largest where the row's temperature is 0 or less; else logits / temperature, top_k (0 or less: none; what ties with the
+    k-th stays), top_p (1 or more: none; the lower index first among equals), min_p (0 or less: none), and the first index
+    whose running total exceeds `uniform` times what is left. `temperature`, `top_p`, `min_p` and `uniform` are float64 [rows], `top_k`
+    int32 [rows], all on the logits' device, which has to be the current one. Nothing left (a top_p of 0 or less, a min_p above 1) gives
+    token 0; logits with a NaN or an infinity among them their first largest."""
+    _need(logits, "sample_filtered logits", torch.float32)
+    if logits.dim() != 2:
+        raise KernelError(f"sample_filtered: logits {tuple(logits.shape)} are not [rows, vocab]")
+    rows, vocab = logits.shape
+    for t, what in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (uniform, "uniform")):
+        _need(t, f"sample_filtered {what}", torch.float64, (rows,))
+    _need(top_k, "sample_filtered top_k", torch.int32, (rows,))
+    _on_current_device("sample_filtered", logits, temperature, top_k, top_p, min_p, uniform)
+    out = _fresh((rows,), torch.int32, logits.device)
+    _check(library().kb_sample_filtered(_ptr(out), _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform),
+                                        int(rows), int(vocab), _stream()))
+    return out
+
 # ------------------------------------------------------------------------------------------
 # Timing by kernel name, in the manner of Kapel's `Timed<B>` wrapper backend
 # (crates/kapel-cli/examples/profile.rs:17-56): every entry point above is bracketed by CUDA
 # events and its device time added up under its name and its largest argument's shape.
 _TIMED = ("embed", "rope_table", "rope_append", "glu", "cast", "gather_rows", "rmsnorm", "add_rmsnorm", "gemm",
-          "paged_attention_rows", "paged_attention_mma", "sample", "proj_norm_append", "head_gate", "mlstm_scan", "moe_route",
+          "paged_attention_rows", "paged_attention_mma", "sample", "sample_filtered", "proj_norm_append", "head_gate", "mlstm_scan", "moe_route",
           "moe_sort", "moe_grouped", "moe_combine", "gemm_glu_fused", "paged_attention_decode_fused", "layernorm", "concat2",
           "head_norm_rope_append", "latent_append", "head_linear", "delta_scan", "latent_attention_mma", "proj_rope_append",
           "pool_blocks", "pooled_attention", "act", "token_shift", "conv_append", "gdelta_scan", "gate_scan", "weighted_sum2",

@@ -7,8 +7,9 @@ then a draw from what is left. The generator is xoshiro256** seeded by four Spli
 uniform number in [0, 1) (sampling.rs:241-260). Arithmetic on the host is 64-bit, as there.
 
 A request whose choice needs only the logits (greedy without penalties, or a plain
-temperature) can be served where the logits are, by `kernels.sample`; the uniform number still
-comes from this generator, so the same seed gives the same tokens.
+temperature) can be served where the logits are, by `kernels.sample`, one with filters by
+`kernels.sample_filtered`; the uniform number still comes from this generator, so the same seed
+gives the same tokens. Penalties, which look at the tokens so far, stay here.
 
 The arithmetic runs in the host library (`csrc/host/sampler_core.cpp`): a choice over 256,000
 logits with top_k takes about a millisecond there, where sorting them with numpy took ten to
@@ -75,6 +76,11 @@ class Sampling:
     def on_device(self) -> bool:
         """Only the logits, a temperature and a uniform number decide."""
         return not self.has_penalties() and (self.is_greedy() or not self.has_filters())
+
+
+    def filtered_on_device(self) -> bool:
+        """The logits, the filters' settings and a uniform number decide: `kernels.sample_filtered` follows the host's rules."""
+        return not self.has_penalties()
 
 
 class Rng:
