@@ -1,0 +1,252 @@
+// Attention of single tokens over shared and own pages (see attention_shared.cuh for the cut), for any element type and head size up
+// to 256; and the kernel that joins the pieces.
+//
+// A block of 256 threads walks its units of 32 positions. Eight threads have one (row, head) pair of the 32 that a tile takes: each
+// computes every eighth position's score out of keys and queries in shared memory, and keeps every eighth group of four components of the
+// sum in registers. All arithmetic is 32-bit. Where some row of the tile does not see all of a unit (its window begins there, its
+// positions end there) what a row does not see is left out of its sum, not multiplied by zero: it may be anything.
+#include "attention_shared.cuh"
+
+namespace kb {
+
+constexpr int SR_PAIRS = 32, SR_KEYS = 32, SR_THREADS = 256, SR_DIM = 256;
+
+template <typename T> struct SharedRowsSmem {
+    float q[SR_PAIRS][SR_DIM + 4];
+    float k[SR_KEYS][SR_DIM + 4];
+    float v[SR_KEYS][SR_DIM];
+    long long line[SR_KEYS];               // a position's line of this kv head in the tables, -1 for none
+    SharedCut cut;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedParams p) {
+    extern __shared__ __align__(16) unsigned char sr_raw[];
+    SharedRowsSmem<T>& s = *reinterpret_cast<SharedRowsSmem<T>*>(sr_raw);
+    const int tid = threadIdx.x, pair = tid >> 3, sub = tid & 7, lane = tid & 31;
+    const int group = p.hq / p.hkv, rows_a_tile = SR_PAIRS / group;
+    const T* q = static_cast<const T*>(p.q);
+    const T* kt = static_cast<const T*>(p.k_table);
+    const T* vt = static_cast<const T*>(p.v_table);
+    shared_make_cut(p, s.cut, rows_a_tile, SR_KEYS);
+    if (blockIdx.x == 0) shared_leave_cut(p, s.cut);
+    const long long units = (long long)s.cut.units * p.hkv;
+    const int workers = shared_workers(units);
+    if ((int)blockIdx.x >= workers) return;
+    const int begin = shared_begin(blockIdx.x, units, workers), end = shared_begin(blockIdx.x + 1, units, workers);
+    const int d4 = (p.d + 3) / 4;
+    for (int u = begin; u < end;) {
+        const SharedPart w = shared_part(p, s.cut, u, end, SR_KEYS, SR_PAIRS);
+        u += w.n_units;
+        const int pairs = w.n * group;
+        const int row = w.row0 + pair / group;
+        const bool own = pair < pairs;
+        __syncthreads();                                 // the part before is done with the queries
+        for (int i = tid; i < pairs * d4 * 4; i += SR_THREADS) {
+            const int r = i / (d4 * 4), c = i % (d4 * 4);
+            s.q[r][c] = c < p.d ? Elem<T>::load(q + ((size_t)(w.row0 + r / group) * p.hq + w.kvh * group + r % group) * p.d + c) : 0.f;
+        }
+        const int count = own ? min(p.row_count[row], w.hi) : 0;
+        const int first = own ? max(shared_first(p, p.row_count[row]), w.lo) : 0;
+        float m = -INFINITY, l = 0.f;
+        float4 acc[SR_DIM / 32];
+#pragma unroll
+        for (int j = 0; j < SR_DIM / 32; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int t = 0; t < w.n_units; ++t) {
+            const int j0 = (w.lo / SR_KEYS + w.first_unit + t) * SR_KEYS;
+            __syncthreads();                             // the unit before is done with keys and values
+            if (tid < SR_KEYS) {
+                const int j = j0 + tid;
+                long long line = -1;
+                if (j >= w.lo && j < w.hi) {
+                    const int page = p.block_table[(size_t)w.looks * p.table_width + j / p.page_size];
+                    if (page >= 0 && page < p.n_pages) line = ((long long)page * p.hkv + w.kvh) * p.page_size + j % p.page_size;
+                }
+                s.line[tid] = line;
+            }
+            __syncthreads();
+            for (int i = tid; i < SR_KEYS * d4 * 4; i += SR_THREADS) {
+                const int r = i / (d4 * 4), c = i % (d4 * 4);
+                s.k[r][c] = c < p.d && s.line[r] >= 0 ? Elem<T>::load(kt + s.line[r] * p.d + c) : 0.f;
+            }
+            for (int i = tid; i < SR_KEYS * p.dv; i += SR_THREADS) {
+                const int r = i / p.dv, c = i % p.dv;
+                s.v[r][c] = s.line[r] >= 0 ? Elem<T>::load(vt + s.line[r] * p.dv + c) : 0.f;
+            }
+            __syncthreads();
+            float x[SR_KEYS / 8];
+            float top = -INFINITY;
+            bool all = true;
+#pragma unroll
+            for (int i = 0; i < SR_KEYS / 8; ++i) {
+                const int j = sub + 8 * i;
+                float dot = 0.f;
+                if (own)
+                    for (int c = 0; c < d4; ++c) {
+                        const float4 a = *reinterpret_cast<const float4*>(&s.q[pair][4 * c]), b = *reinterpret_cast<const float4*>(&s.k[j][4 * c]);
+                        dot = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, dot))));
+                    }
+                dot *= p.scale;
+                if (p.cap > 0.f) dot = p.cap * tanhf(dot / p.cap);
+                const bool sees = j0 + j >= first && j0 + j < count && s.line[j] >= 0;
+                all = all && sees;
+                x[i] = sees ? dot : -INFINITY;
+                top = fmaxf(top, x[i]);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float next = fmaxf(m, top);
+            const float fade = next == -INFINITY ? 1.f : expf(m - next);       // e^-inf = 0 where nothing was seen before
+            m = next;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < SR_KEYS / 8; ++i) {
+                x[i] = x[i] == -INFINITY ? 0.f : expf(x[i] - m);
+                sum += x[i];
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l = l * fade + sum;
+#pragma unroll
+            for (int j = 0; j < SR_DIM / 32; ++j) { acc[j].x *= fade; acc[j].y *= fade; acc[j].z *= fade; acc[j].w *= fade; }
+            const bool whole = __all_sync(0xffffffffu, all || !own);
+#pragma unroll
+            for (int i = 0; i < SR_KEYS / 8; ++i)
+#pragma unroll
+                for (int b = 0; b < 8; ++b) {
+                    const float e = __shfl_sync(0xffffffffu, x[i], (lane & 24) + b);
+                    const int j = 8 * i + b;
+                    if (!own || (!whole && e == 0.f)) continue;
+#pragma unroll
+                    for (int c = 0; c < SR_DIM / 32; ++c) {
+                        const int at = 32 * c + 4 * sub;
+                        if (at >= p.dv) break;
+                        const float4 v = *reinterpret_cast<const float4*>(&s.v[j][at]);
+                        acc[c].x = fmaf(e, v.x, acc[c].x);
+                        acc[c].y = fmaf(e, v.y, acc[c].y);
+                        acc[c].z = fmaf(e, v.z, acc[c].z);
+                        acc[c].w = fmaf(e, v.w, acc[c].w);
+                    }
+                }
+        }
+        if (own) {
+            float* piece = p.pieces + (w.place + pair) * (p.dv + 2);
+#pragma unroll
+            for (int c = 0; c < SR_DIM / 32; ++c) {
+                const int at = 32 * c + 4 * sub;
+                if (at < p.dv) piece[at] = acc[c].x;
+                if (at + 1 < p.dv) piece[at + 1] = acc[c].y;
+                if (at + 2 < p.dv) piece[at + 2] = acc[c].z;
+                if (at + 3 < p.dv) piece[at + 3] = acc[c].w;
+            }
+            if (sub == 0) { piece[p.dv] = m; piece[p.dv + 1] = l; }
+        }
+    }
+}
+
+// Joins a (row, head) pair's pieces: its tile's, block by block, then its own. A block a pair.
+constexpr int SJ_THREADS = 128;
+template <typename T>
+__global__ void __launch_bounds__(SJ_THREADS) shared_combine_kernel(const SharedParams p, int tile_pairs) {
+    const int r = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    const int group = p.hq / p.hkv, kvh = head / group;
+    const int* cut = p.cut;
+    const int tiles = cut[0], blocks = cut[2], tile_rows_total = cut[3];
+    const int units = cut[1] * p.hkv;
+    const int* upto = cut + SH_CUT_HEAD + 4 * SH_ROWS;
+    const int t = cut[SH_CUT_HEAD + r];
+    long long place[2];
+    int first[2] = {0, 0}, last[2] = {-1, -1};           // blocks that have a piece, of the tile and of the row itself
+    for (int k = 0; k < 2; ++k) {
+        const int item = k == 0 ? t : tiles + r;
+        place[k] = 0;
+        if (item < 0) continue;
+        const int n = upto[item + 1] - upto[item];
+        if (n == 0) continue;
+        const long long u = (long long)upto[item] * p.hkv + (long long)kvh * n;
+        first[k] = shared_block_of(u, units, blocks);
+        last[k] = shared_block_of(u + n - 1, units, blocks);
+        if (k == 0) {
+            const int* tile = cut + SH_CUT_HEAD + SH_ROWS + 3 * t;
+            place[k] = ((long long)tile[2] * p.hkv + (long long)kvh * tile[1] + (r - tile[0])) * group + head % group;
+        } else {
+            place[k] = ((long long)(tile_rows_total + r) * p.hkv + kvh) * group + head % group;
+        }
+    }
+    const int width = p.dv + 2;
+    float m = p.sinks ? p.sinks[head] : -INFINITY;
+    for (int k = 0; k < 2; ++k)
+        for (int b = first[k]; b <= last[k]; ++b) m = fmaxf(m, p.pieces[(place[k] + (long long)b * tile_pairs) * width + p.dv]);
+    float total = p.sinks && m != -INFINITY ? expf(p.sinks[head] - m) : 0.f;
+    constexpr int MOST = SR_DIM / SJ_THREADS;
+    float sum[MOST];
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) sum[j] = 0.f;
+    for (int k = 0; k < 2; ++k)
+        for (int b = first[k]; b <= last[k]; ++b) {
+            const float* piece = p.pieces + (place[k] + (long long)b * tile_pairs) * width;
+            const float pm = piece[p.dv];
+            if (pm == -INFINITY) continue;               // a range of which the row sees nothing
+            const float fade = expf(pm - m);
+            total = fmaf(fade, piece[p.dv + 1], total);
+#pragma unroll
+            for (int j = 0; j < MOST; ++j)
+                if (tid + j * SJ_THREADS < p.dv) sum[j] = fmaf(fade, piece[tid + j * SJ_THREADS], sum[j]);
+        }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    T* out = static_cast<T*>(p.out) + ((size_t)r * p.hq + head) * p.dv;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j)
+        if (tid + j * SJ_THREADS < p.dv) Elem<T>::store(out + tid + j * SJ_THREADS, sum[j] * inv);
+}
+
+template <typename T> static int launch_shared_rows(const SharedParams& p, int blocks, cudaStream_t s) {
+    const int smem = (int)sizeof(SharedRowsSmem<T>);
+    const cudaError_t e = cudaFuncSetAttribute(shared_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    shared_rows_kernel<T><<<blocks, SR_THREADS, smem, s>>>(p);
+    if (int err = check_launch("shared_attention")) return err;
+    shared_combine_kernel<T><<<dim3(p.rows, p.hq), SJ_THREADS, 0, s>>>(p, SR_PAIRS);
+    return check_launch("shared_attention");
+}
+
+}  // namespace kb
+
+using namespace kb;
+
+static int shared_blocks() { return multiprocessors(); }
+
+// Floats of scratch memory: the pieces, then the cut.
+extern "C" long long kb_shared_attention_scratch_floats(int rows, int hq, int dv) {
+    if (rows <= 0 || rows > SH_ROWS || hq <= 0 || dv <= 0) return 0;
+    return shared_places(rows, hq, shared_blocks(), SR_PAIRS) * (dv + 2) + SH_CUT_INTS;
+}
+
+// 1 where the kernels take these sizes.
+extern "C" int kb_shared_attention_takes(int dtype, int hq, int hkv, int d, int dv, int page_size) {
+    return (dtype == KB_DT_F32 || dtype == KB_DT_BF16) && hkv > 0 && hq > 0 && hq % hkv == 0 && hq / hkv <= SR_PAIRS && d > 0 && d <= SR_DIM && dv > 0 &&
+           dv <= SR_DIM && page_size > 0;
+}
+
+extern "C" int kb_shared_attention(void* out, const void* q, const void* k_table, const void* v_table, int dtype, const int* block_table,
+                                   const int* row_count, const int* share_id, const int* share_len, int rows, int hq, int hkv, int d, int dv,
+                                   int page_size, int table_width, int n_pages, int window, float scale, float cap, const float* sinks,
+                                   float* scratch, long long scratch_floats, void* stream) {
+    KB_REQUIRE(rows >= 0 && rows <= SH_ROWS, "shared_attention: %d rows (0..%d)", rows, SH_ROWS);
+    KB_REQUIRE(kb_shared_attention_takes(dtype, hq, hkv, d, dv, page_size),
+               "shared_attention: dtype code %d, %d heads over %d of %d / %d, pages of %d are not taken", dtype, hq, hkv, d, dv, page_size);
+    KB_REQUIRE(table_width > 0 && n_pages > 0 && window >= 0 && cap >= 0.f, "shared_attention: table width %d, pages %d, window %d, soft cap %g", table_width,
+               n_pages, window, cap);
+    KB_REQUIRE((long long)table_width * page_size <= 0x7fffffffll / 4 && ((long long)table_width * page_size / SR_KEYS + 2) * 2 * rows * hkv <= 0x7fffffffll,
+               "shared_attention: %d block tables of %d pages of %d positions are too many for one launch", rows, table_width, page_size);
+    if (rows == 0) return 0;
+    KB_REQUIRE(scratch != nullptr && scratch_floats >= kb_shared_attention_scratch_floats(rows, hq, dv), "shared_attention: scratch memory of %lld floats",
+               scratch_floats);
+    SharedParams p = {};
+    p.q = q; p.k_table = k_table; p.v_table = v_table; p.block_table = block_table; p.row_count = row_count; p.share_id = share_id;
+    p.share_len = share_len; p.sinks = sinks; p.out = out; p.pieces = scratch; p.rows = rows; p.hq = hq; p.hkv = hkv; p.d = d; p.dv = dv;
+    p.page_size = page_size; p.table_width = table_width; p.n_pages = n_pages; p.window = window; p.scale = scale; p.cap = cap;
+    const int blocks = shared_blocks();
+    p.cut = reinterpret_cast<int*>(scratch + shared_places(rows, hq, blocks, SR_PAIRS) * (dv + 2));
+    return dtype == KB_DT_F32 ? launch_shared_rows<float>(p, blocks, (cudaStream_t)stream) : launch_shared_rows<__nv_bfloat16>(p, blocks, (cudaStream_t)stream);
+}

@@ -65,7 +65,7 @@ def library():
                 for name in ("kb_gemm_bf16_scratch_floats", "kb_paged_attention_scratch_floats", "kb_attention_mma_scratch_floats", "kb_sample_scratch_floats",
                              "kb_mlstm_state_floats", "kb_delta_state_floats", "kb_delta_scratch_floats", "kb_delta_chunk_floats", "kb_gemm_f32_scratch_floats", "kb_pooled_attention_scratch_floats",
                              "kb_pooled_attention_mma_scratch_floats", "kb_pooled_attention_mma_kept_floats", "kb_decay_scan_scratch_floats",
-                             "kb_retention_scratch_floats"):
+                             "kb_retention_scratch_floats", "kb_shared_attention_scratch_floats"):
                     getattr(lib, name).restype = ctypes.c_longlong
                 lib.kb_launch_count.restype = ctypes.c_ulonglong
                 lib.kb_dependent_launch_count.restype = ctypes.c_ulonglong
@@ -240,6 +240,19 @@ def fill_rows(table: torch.Tensor, rows: torch.Tensor, value: float = 0.0) -> No
     width = table.numel() // table.shape[0]
     _check(library().kb_fill_rows_f32(_ptr(table), _ptr(rows), int(rows.numel()), ctypes.c_longlong(width), int(table.shape[0]),
                                       _f(value), _stream()))
+
+
+def copy_rows(table: torch.Tensor, source: torch.Tensor, target: torch.Tensor) -> None:
+    """table[target[i]] = table[source[i]] for a table [n, ...] and int32 row numbers on the device; no row is in both lists."""
+    _need(table, "copy_rows table")
+    _dt(table, "copy_rows table")
+    _need(source, "copy_rows source", torch.int32)
+    _need(target, "copy_rows target", torch.int32, (source.numel(),))
+    _on_current_device("copy_rows", table, source, target)
+    if table.dim() < 1 or table.numel() == 0 or source.numel() == 0:
+        return
+    _check(library().kb_copy_rows(_ptr(table), _ptr(source), _ptr(target), int(source.numel()), int(table.shape[0]),
+                                  ctypes.c_longlong(table.numel() // table.shape[0] * table.element_size()), _stream()))
 
 
 class SplitSum:
@@ -1022,6 +1035,52 @@ def paged_attention_mma(q, k_table, v_table, block_table, row_count, tiles, page
                                     _f(softcap or 0.0), int(decode), int(bool(relative) and bool(decode)), int(keep_first or 0),
                                     _ptr(scratch), int(block or 0), _ptr(sinks), _stream())
     )
+    return out
+
+
+SHARED_PREFIX_ROWS = 512                # the most requests one call of `shared_prefix_attention` takes
+
+
+def shared_prefix_takes(dtype, hq: int, hkv: int, d: int, dv: int, page_size: int) -> bool:
+    """Whether `shared_prefix_attention` takes these sizes."""
+    return dtype in _CODES and bool(library().kb_shared_attention_takes(_CODES[dtype], int(hq), int(hkv), int(d), int(dv), int(page_size)))
+
+
+def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_id, share_len, page_size: int, window: Optional[int],
+                            scale: float, softcap: Optional[float], sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a decode step's single tokens [rows, hq, d] (row r is request r, its pages in row r of `block_table`, its own
+    position the last of the `row_count[r]` it has seen) where requests share the pages of a prompt: rows that follow one another with the
+    same `share_id` and `share_len` (int32 [rows]) have the same pages for their first share_len positions, and what they share is read
+    once for all of them, out of the block table of the one that sees furthest back. share_len is taken down to whole pages and to the row's
+    count; 0 shares nothing. Up to SHARED_PREFIX_ROWS rows. Window, soft cap and `sinks` as for `paged_attention_mma`; a row that
+    sees nothing gives zeros. With a window, shared values that only some rows of a group still see have to be finite in bfloat16."""
+    _need(q, "shared attention q")
+    if q.dim() != 3:
+        raise KernelError(f"shared attention: q {tuple(q.shape)} is not [rows, heads, head size]")
+    rows, hq, d = q.shape
+    dt = _dt(q, "shared attention q")
+    _need(k_table, "shared attention k table", q.dtype)
+    _need(v_table, "shared attention v table", q.dtype)
+    if k_table.dim() != 4 or k_table.shape[2] != page_size or k_table.shape[3] != d or v_table.dim() != 4 or v_table.shape[:3] != k_table.shape[:3]:
+        raise KernelError(f"shared attention: tables {tuple(k_table.shape)} / {tuple(v_table.shape)} are not [pages, kv_heads, {page_size}, {d}]")
+    n_pages, hkv, dv = k_table.shape[0], k_table.shape[1], v_table.shape[3]
+    _need(block_table, "shared attention block table", torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] < rows:
+        raise KernelError(f"shared attention: a block table of {tuple(block_table.shape)} for {rows} requests")
+    for t, what in ((row_count, "row_count"), (share_id, "share_id"), (share_len, "share_len")):
+        _need(t, f"shared attention {what}", torch.int32, (rows,))
+    if sinks is not None:
+        _need(sinks, "shared attention sinks", torch.float32, (hq,))
+    _on_current_device("shared attention", q, k_table, v_table, block_table, row_count, share_id, share_len, sinks)
+    if window is not None and window < 0:
+        raise KernelError(f"shared attention: a window of {window}")
+    out = _fresh((rows, hq, dv), q.dtype, q.device)
+    lib = library()
+    need = int(lib.kb_shared_attention_scratch_floats(rows, hq, dv))
+    scratch = _fresh((need,), torch.float32, q.device) if need else None
+    _check(lib.kb_shared_attention(_ptr(out), _ptr(q), _ptr(k_table), _ptr(v_table), dt, _ptr(block_table), _ptr(row_count), _ptr(share_id),
+                                   _ptr(share_len), rows, hq, hkv, d, dv, int(page_size), int(block_table.shape[1]), int(n_pages),
+                                   int(window or 0), _f(scale), _f(softcap or 0.0), _ptr(sinks), _ptr(scratch), ctypes.c_longlong(need), _stream()))
     return out
 
 
@@ -2070,7 +2129,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
 # (crates/kapel-cli/examples/profile.rs:17-56): every entry point above is bracketed by CUDA
 # events and its device time added up under its name and its largest argument's shape.
 _TIMED = ("embed", "rope_table", "rope_append", "glu", "cast", "gather_rows", "rmsnorm", "add_rmsnorm", "gemm",
-          "paged_attention_rows", "paged_attention_mma", "sample", "sample_filtered", "proj_norm_append", "head_gate", "mlstm_scan", "moe_route",
+          "paged_attention_rows", "paged_attention_mma", "shared_prefix_attention", "sample", "sample_filtered", "proj_norm_append", "head_gate", "mlstm_scan", "moe_route",
           "moe_sort", "moe_grouped", "moe_combine", "gemm_glu_fused", "paged_attention_decode_fused", "layernorm", "concat2",
           "head_norm_rope_append", "latent_append", "head_linear", "delta_scan", "latent_attention_mma", "proj_rope_append",
           "pool_blocks", "pooled_attention", "act", "token_shift", "conv_append", "gdelta_scan", "gate_scan", "weighted_sum2",
