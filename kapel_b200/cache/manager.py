@@ -13,6 +13,11 @@ Beside the pages there are slots for per-request state of fixed size (Kapel's `s
 cache.rs:141-144,846-897): slot 0 belongs to padding rows, a request gets a slot of its own
 for its lifetime, and `Plan.fresh` says which slots a step must clear.
 
+A sequence may be forked (`fork`): the new one holds the same whole pages, which go back when the
+last holder ends, and a copy of the page that is not full yet; both write only behind what they share.
+Sequences of one fork form a family, and a step whose rows are of one family, one behind the other,
+may read what they share once for all of them (`shared_runs`).
+
 The manager is host code only. Device tables are made by an `allocate(shape, dtype)` function
 given by the engine, so every decision here can be tested without a GPU. The bookkeeping (free
 lists, page lists, the arrays of a step) runs in the host library, `csrc/host/cache_core.cpp`;
@@ -104,6 +109,7 @@ class Plan:
     taken: List[Tuple[int, Hashable, int, int]] = field(default_factory=list)  # (group, id, logical, physical)
     committed: bool = False
     native: object = None        # the manager's own: the entries as the host library takes them
+    share: object = None         # (ids, positions) by row where single tokens share pages (`CacheManager.shared_runs`), else None
     added: List[Hashable] = field(default_factory=list)   # the step function's: sequences it added for this step
 
     @property
@@ -195,6 +201,8 @@ class CacheManager:
         self._scratch = np.zeros(max(n_groups, 1), np.int32)
         self._info = np.zeros(7, np.int64)
         self._info_ptr = self._info.ctypes.data
+        self._family: Dict[Hashable, Tuple[int, int]] = {}       # sequence -> (family, positions its members share, whole pages)
+        self._families = 0
         self._names = 0                                          # counts the sequences that have come or gone
         if allocate is not None:
             self.allocate_tables(allocate, dtype)
@@ -248,9 +256,50 @@ class CacheManager:
     def remove_sequence(self, seq_id) -> None:
         """Gives back everything the sequence holds, last page first."""
         slot = self._sequences.pop(seq_id)
+        self._family.pop(seq_id, None)
         self._names += 1
         if self._lib.kc_remove(self._h, slot) != 0:
             raise AssertionError(f"sequence {seq_id!r} (slot {slot}) could not give its pages back")
+
+    def fork(self, seq_id, new_id) -> List[Tuple[int, int, int]]:
+        """Adds `new_id`, which goes on where `seq_id` is: it holds the same whole pages, and a page of its
+        own where the last one is not full. Returns [(group, page, the new sequence's page)], the pages whose lines the
+        caller copies (and the state of one slot to the other's) before either sequence goes on. Raises `CacheFull` and
+        takes nothing if a slot or a page is lacking."""
+        if new_id in self._sequences:
+            raise ValueError(f"sequence {new_id!r} is already in the cache")
+        if seq_id not in self._sequences:
+            raise KeyError(f"sequence {seq_id!r} is not in the cache")
+        copies, n = np.zeros((max(1, len(self.groups)), 3), np.int32), np.zeros(1, np.int32)
+        slot = self._lib.kc_fork(self._h, self._sequences[seq_id], _ptr(copies), _ptr(n))
+        if slot == -1:
+            raise ValueError(f"sequence {seq_id!r} holds nothing yet that could be shared")
+        if slot == -2:
+            raise CacheFull(1, 0, "slots")
+        if slot < 0:
+            raise CacheFull(1, 0, self.groups[int(copies[0, 0])].name)
+        self._sequences[new_id] = slot
+        self._names += 1
+        shared = self.length(seq_id) // self.page_size * self.page_size
+        if shared and self.groups:
+            if seq_id not in self._family:
+                self._families += 1
+                self._family[seq_id] = (self._families, shared)
+            self._family[new_id] = self._family[seq_id]
+        return [tuple(int(x) for x in t) for t in copies[: int(n[0])]]
+
+    def shared_runs(self, seq_ids: Sequence[Hashable]):
+        """(ids, positions), int32 each, for the rows of a step in which these sequences bring a token each: neighbours of one family have
+        the same id and the number of positions they share; 0 positions for a sequence without such a neighbour. None where
+        there is none at all."""
+        if len(self._family) < 2:
+            return None
+        ids, lengths = np.zeros((2, len(seq_ids)), np.int32)
+        found = [self._family.get(s) for s in seq_ids]
+        for r, f in enumerate(found):
+            if f is not None and ((r > 0 and found[r - 1] == f) or (r + 1 < len(found) and found[r + 1] == f)):
+                ids[r], lengths[r] = f
+        return (ids, lengths) if lengths.any() else None
 
     def length(self, seq_id) -> int:
         return self._lib.kc_length(self._h, self._sequences[seq_id])
@@ -374,6 +423,8 @@ class CacheManager:
                     buf[at_entry : at_entry + n], buf[at_entry + n : at_entry + 2 * n], buf[at_entry + 2 * n : at_entry + 3 * n],
                     buf[at_entry + 3 * n : at_entry + 4 * n], buf[at_fresh:].view(np.bool_)[:n], group_plans, taken)
         plan.native = (self._names, sc, n)
+        if n_rows == n:
+            plan.share = self.shared_runs([s for s, _ in entries])
         return plan
 
     def _entries_arrays(self, entries):
@@ -411,7 +462,7 @@ class CacheManager:
 
     # ------------------------------------------------------------------ checks
     def check(self) -> None:
-        """No page lost, none held twice: every held page belongs to exactly one sequence."""
+        """No page lost, none held more often than counted: every held page belongs to as many sequences as its count says."""
         msg = ctypes.create_string_buffer(512)
         if self._lib.kc_check(self._h, msg, 512):
             raise AssertionError(msg.value.decode())

@@ -2,8 +2,8 @@
 
 Kapel keeps a free list with reference counts and a typed `CacheFull{needed, free}`
 (crates/kapel-models/src/cache.rs:148-150,419-433; crates/kapel-models/src/lib.rs:70-77).
-Here pages are never shared, so a page is either free or held by exactly one owner; the pool
-checks that on every call. The bookkeeping itself is in the host library
+Here a page is free or held by one owner, or by several after `CacheManager.fork`: it goes
+back when the last of them gives it back; the pool checks that on every call. The bookkeeping itself is in the host library
 (`csrc/host/cache_core.cpp`), built with the C++ compiler alone at first use.
 """
 from __future__ import annotations

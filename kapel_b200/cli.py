@@ -8,7 +8,7 @@
 Options keep Kapel's names and meanings where it has them. This engine's own: `--tokens` (token
 ids instead of text), `--prompt-len N` (N seeded random token ids as the prompt), `--random
 CONFIG --seed-weights S` (no folder: a model of CONFIG, a config.json or a preset's name, with
-random weights made on the device), `--pages`, `--max-pass-tokens`, `--max-sequences` (Kapel's
+random weights made on the device), `--samples N` (N answers to one prompt, one a line), `--pages`, `--max-pass-tokens`, `--max-sequences` (Kapel's
 engine options, crates/kapel-infer/src/engine.rs:36-64), `--strict`, and `init`.
 """
 from __future__ import annotations
@@ -46,6 +46,7 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--min-p", type=float, default=None)
     run.add_argument("--repetition-penalty", type=float, default=None)
     run.add_argument("--seed", type=int, default=0, help="the seed of the draws (default 0)")
+    run.add_argument("--samples", type=int, default=1, metavar="N", help="N answers to the prompt, which is computed once; the i-th (from 0) draws with seed + i (default 1)")
     run.add_argument("--stop", action="append", default=[], help="end the answer at TEXT (repeatable); with --tokens, comma-separated ids")
     run.add_argument("--kv-cache", default=None, help="the type of the cache of keys and values (only the compute dtype here)")
     run.add_argument("--quantize", default=None, help="not built in this engine")
@@ -74,6 +75,9 @@ def main(argv=None) -> int:
         return 2
     if (args.model is None) == (args.random is None):
         print("error: give either MODEL or --random CONFIG", file=sys.stderr)
+        return 2
+    if args.samples < 1:
+        print("error: --samples must be positive", file=sys.stderr)
         return 2
     if args.prompt_len is not None and args.prompt_len <= 0:
         print("error: --prompt-len must be positive", file=sys.stderr)
@@ -108,6 +112,22 @@ def main(argv=None) -> int:
             prompt, stop = args.prompt, list(args.stop)
         temperature = 0.0 if args.greedy else args.temperature
         t0 = time.perf_counter()
+        if args.samples > 1:
+            answers = model.generate_samples(prompt, args.samples, max_tokens=args.max_tokens, temperature=temperature, top_k=args.top_k, top_p=args.top_p,
+                                             min_p=args.min_p, repetition_penalty=args.repetition_penalty, seed=args.seed, stop=stop,
+                                             ignore_eos=args.ignore_eos)
+            total = time.perf_counter() - t0
+            for answer in answers:
+                print(answer if args.prompt is not None else ",".join(str(t) for t in answer))
+            if args.stats:
+                n_prompt = len(prompt) if not isinstance(prompt, str) else len(model.tokenize(prompt))
+                n = sum(len(a) if args.prompt is None else len(model.tokenize(a, add_special_tokens=False)) for a in answers)
+                print(f"load {t_load:.2f} s; prompt {n_prompt} tokens; {args.samples} answers; {n} tokens; {n / total:.1f} tokens/s, the prompt's time included",
+                      file=sys.stderr)
+                st = model.last_scheduler.stats()
+                print(f"passes {st.passes} ({st.recorded_passes} recorded); preemptions {st.preemptions}; pages {st.pages}, free {st.free_pages}; "
+                      f"released by windows {st.released_pages}", file=sys.stderr)
+            return 0
         first = None
         out = []
         for piece in model.generate(prompt, max_tokens=args.max_tokens, temperature=temperature, top_k=args.top_k,

@@ -8,6 +8,10 @@
 // functions over an opaque handle, called through ctypes; no GPU code, so every decision is tested
 // without one. The Python class `CacheManager` owns the handle and the device tables.
 //
+// A sequence may be forked: the new one holds the same whole pages (a page goes back when its last
+// holder gives it back; Kapel counts references likewise, cache.rs:419-433) and a page of its own for
+// the positions of a page that is not full yet, which the caller copies.
+//
 // Orders matter and are part of the contract (a replay of the same requests takes the same pages):
 // a fresh pool hands out page 0 first; the page given back last is taken first; a sequence that ends
 // gives its pages back last page first, group by group; slot 1 is handed out first and the slot
@@ -24,7 +28,7 @@ namespace {
 struct Pool {
     int n = 0;
     std::vector<int> free_;            // taken from the back
-    std::vector<uint8_t> held;
+    std::vector<int> held;             // how many sequences hold a page
 
     explicit Pool(int pages) : n(pages), held((size_t)pages, 0) {
         free_.reserve((size_t)pages);
@@ -41,8 +45,7 @@ struct Pool {
     int give(int p) {                  // 0, -1 not of this pool, -2 given back twice
         if (p < 0 || p >= n) return -1;
         if (!held[(size_t)p]) return -2;
-        held[(size_t)p] = 0;
-        free_.push_back(p);
+        if (--held[(size_t)p] == 0) free_.push_back(p);
         return 0;
     }
     int check(std::string* why) const {
@@ -168,6 +171,43 @@ int kc_remove(void* h, int slot) {
     *s = Seq();
     c->free_slots.push_back(slot);
     return bad ? -2 : 0;
+}
+
+// A new sequence that goes on where the one in `slot` is: the same whole pages, and in every group that has a page in use at the end a page of
+// its own for it. `copies` receives (group, page, the new sequence's page) for those, up to one a group; returns the new slot, or -1: no
+// such sequence or one that holds nothing yet, -2: no slot is free, -3: a group (copies[0]) lacks a page. Nothing is taken then.
+int kc_fork(void* h, int slot, int* copies, int* n_copies) {
+    Cache* c = as_cache(h);
+    *n_copies = 0;
+    Seq* from = c->live(slot);
+    if (!from || from->length <= 0) return -1;
+    if (c->free_slots.empty()) return -2;
+    const int pages = c->pages_for(from->length);          // of a step that is planned but not committed there may be more
+    const bool partly = from->length % c->page_size != 0;
+    for (int g = 0; g < c->groups(); ++g)
+        if (partly && from->pages[(size_t)g][(size_t)pages - 1] >= 0 && c->pools[(size_t)g].free_.empty()) { copies[0] = g; return -3; }
+    const int to = kc_add(h);
+    Seq& s = c->seqs[(size_t)to];
+    from = c->live(slot);
+    s.fresh = false;
+    s.length = from->length;
+    s.released = from->released;
+    for (int g = 0; g < c->groups(); ++g) {
+        Pool& pool = c->pools[(size_t)g];
+        std::vector<int>& mine = s.pages[(size_t)g];
+        mine.assign(from->pages[(size_t)g].begin(), from->pages[(size_t)g].begin() + pages);
+        for (int i = 0; i < pages; ++i) {
+            if (mine[(size_t)i] < 0) continue;
+            if (partly && i == pages - 1) {
+                int* t = copies + 3 * (*n_copies)++;
+                t[0] = g; t[1] = mine[(size_t)i]; t[2] = pool.take();
+                mine[(size_t)i] = t[2];
+            } else {
+                ++pool.held[(size_t)mine[(size_t)i]];
+            }
+        }
+    }
+    return to;
 }
 
 int kc_length(void* h, int slot) {
@@ -374,25 +414,22 @@ int kc_check(void* h, char* msg, int cap) {
     for (int g = 0; g < c->groups(); ++g) {
         const Pool& pool = c->pools[(size_t)g];
         if (pool.check(&why)) return fail("group " + std::to_string(g) + ": " + why);
-        std::vector<int> owner((size_t)pool.n, 0);
-        long long owned = 0;
+        std::vector<int> owners((size_t)pool.n, 0);
         for (int slot = 1; slot <= c->max_sequences; ++slot) {
             const Seq& s = c->seqs[(size_t)slot];
             if (!s.live) continue;
             for (int p : s.pages[(size_t)g]) {
                 if (p < 0) continue;
                 if (p >= pool.n) return fail("group " + std::to_string(g) + ": page " + std::to_string(p) + " is not of the pool");
-                if (owner[(size_t)p]) return fail("group " + std::to_string(g) + ": page " + std::to_string(p) + " held by slots " +
-                                                  std::to_string(owner[(size_t)p]) + " and " + std::to_string(slot));
                 if (!pool.held[(size_t)p]) return fail("group " + std::to_string(g) + ": page " + std::to_string(p) + " of slot " +
                                                        std::to_string(slot) + " is on the free list");
-                owner[(size_t)p] = slot;
-                ++owned;
+                ++owners[(size_t)p];
             }
         }
-        const long long held = (long long)pool.n - (long long)pool.free_.size();
-        if (owned != held) return fail("group " + std::to_string(g) + ": " + std::to_string(held) + " pages held, " +
-                                       std::to_string(owned) + " owned: pages lost");
+        for (int p = 0; p < pool.n; ++p)
+            if (owners[(size_t)p] != pool.held[(size_t)p])
+                return fail("group " + std::to_string(g) + ": page " + std::to_string(p) + " counted as held " + std::to_string(pool.held[(size_t)p]) +
+                            " times, by " + std::to_string(owners[(size_t)p]) + " sequences: pages lost or held twice");
     }
     std::vector<uint8_t> free_slot((size_t)c->max_sequences + 1, 0);
     for (int s : c->free_slots) {

@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from ..cache import Plan
-from ..kernels import row_tile_blocks, sm_count
+from ..kernels import SHARED_PREFIX_ROWS, row_tile_blocks, sm_count
 
 
 class GroupBatch:
@@ -55,6 +55,21 @@ def decode_split(pairs: int, longest: int, sms: int, window: Optional[int] = Non
             best = (cost, split)
     split = best[1]
     return split, max(1, -(-(span if relative else longest) // split))
+
+
+# Positions that need not be read again from which a step of single tokens goes by `kernels.shared_prefix_attention`.
+SHARED_POSITIONS = 512
+
+
+def sharing_of(plan):
+    """`plan.share` where reading shared pages once pays, else None."""
+    share = getattr(plan, "share", None)
+    if share is None or plan.rows > SHARED_PREFIX_ROWS:
+        return None
+    ids, lengths = share
+    begins = np.ones(len(ids), bool)
+    begins[1:] = (ids[1:] != ids[:-1]) | (lengths[1:] == 0)
+    return share if int(lengths[~begins].sum()) >= SHARED_POSITIONS else None
 
 
 # Latent attention: a request's rows from which its keys and values are made for every head: that costs about 6 ns a position (16 heads of
@@ -200,6 +215,9 @@ class StepBatch:
         for g in plan.groups:
             parts.append(g.lines)
             parts.append(g.block_table.reshape(-1))
+        share = sharing_of(plan)
+        if share is not None:
+            parts.extend(share)
         sizes = [p.size for p in parts]
         total = sum(sizes)
         host = torch.empty((max(total, 1),), dtype=torch.int32, pin_memory=(device.type == "cuda"))
@@ -230,6 +248,8 @@ class StepBatch:
         self.groups = []
         for i, shape in enumerate(table_shapes):
             self.groups.append(GroupBatch(views[6 + 2 * i], views[7 + 2 * i].view(shape)))
+        at = 6 + 2 * len(table_shapes)
+        self.share = (views[at], views[at + 1]) if len(views) > at else None        # (ids, positions) of rows that share pages
 
     def attention_tiles(self, heads_per_kv: int, kv_heads: int, window: Optional[int] = None, head_dim: int = 256,
                         prompt_kernel: str = "mma", keep_first: int = 0):

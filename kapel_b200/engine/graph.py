@@ -19,7 +19,7 @@ from typing import Dict, List, Optional, Tuple
 import numpy as np
 import torch
 
-from .batch import GroupBatch, StepBatch, decode_split, pooled_slices, sm_count
+from .batch import GroupBatch, StepBatch, decode_split, pooled_slices, sharing_of, sm_count
 
 ROW_BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
 WIDTH_STEP = 64          # block-table widths are rounded up to a multiple of this many pages
@@ -28,12 +28,15 @@ WIDTH_STEP = 64          # block-table widths are rounded up to a multiple of th
 class StaticBatch:
     """A batch of fixed size whose inputs live in one device buffer that replays rewrite."""
 
-    def __init__(self, rows: int, width: int, n_groups: int, device, chunk: int, page_size: int):
+    share = None             # (ids, positions) of rows that share pages, on the device, in a recording that reads those once
+
+    def __init__(self, rows: int, width: int, n_groups: int, device, chunk: int, page_size: int, shared: bool = False):
+        """`shared`: the pass's rows say which of them share pages (`share`), and attention reads what they share once."""
         self.rows = self.entries = rows
         self.width = width
         self.chunk = chunk
         self.memo: Dict[object, object] = {}
-        sizes = [rows] * 6 + [rows, rows * width] * n_groups
+        sizes = [rows] * 6 + [rows, rows * width] * n_groups + [rows, rows] * int(shared)
         self.total = sum(sizes)
         # Two pinned staging buffers taken in turn: the next pass can be written while the copy of
         # the last one may still be in flight. Each has an event recorded behind its copy; the host
@@ -51,6 +54,7 @@ class StaticBatch:
             at += n
         self.ids, self.positions, self.row_entry, self.row_count, self.want_rows, self.slots = views[:6]
         self.groups = [GroupBatch(views[6 + 2 * g], views[7 + 2 * g].view(rows, width)) for g in range(n_groups)]
+        self.share = (views[-2], views[-1]) if shared else None
         self._sizes = sizes
         self.fixed_slots = max(1, -(-(width * page_size) // chunk))
         # the tensor-core attention kernel's tiles: every row a tile of one token
@@ -152,6 +156,9 @@ class StaticBatch:
             w = g.block_table.shape[1]
             table[:n, :w] = g.block_table
             at += rows * width
+        if self.share is not None:
+            for values in plan.share:
+                put(values, 0)
         return which
 
 
@@ -169,12 +176,12 @@ class DecodeGraphs:
         # and destroying a recording while another engine is capturing one invalidates the capture.
         self._engine = weakref.ref(engine)
         self.max_rows = max_rows
-        self.graphs: Dict[Tuple[int, int], Tuple[torch.cuda.CUDAGraph, StaticBatch, torch.Tensor]] = {}
+        self.graphs: Dict[tuple, Tuple[torch.cuda.CUDAGraph, StaticBatch, torch.Tensor]] = {}
         self.replays = 0
         self.replayed_kernels = 0      # kernels that ran inside replays (the library counts only launches it makes itself)
         self.pool = None
         self.passes = 0                # decode passes offered to `run`, recorded or not
-        self.unrecordable: Dict[Tuple[int, int], int] = {}     # bucket -> the pass at which its recording failed
+        self.unrecordable: Dict[tuple, int] = {}     # bucket -> the pass at which its recording failed
         self.failed_captures = 0
         self.last_capture_error: Optional[str] = None
         # Failure injection on the host, for tests: this many of the next recordings raise inside the capture.
@@ -186,11 +193,16 @@ class DecodeGraphs:
                 return b, -(-width // WIDTH_STEP) * WIDTH_STEP
         return None
 
+    def key_of(self, plan) -> Optional[tuple]:
+        """The bucket of a decode-only plan: (rows, block-table width), and a third word where it reads shared pages once."""
+        width = max(g.block_table.shape[1] for g in plan.groups) if plan.groups else 1
+        key = self.bucket(plan.rows, width)
+        return (*key, "shared") if key is not None and sharing_of(plan) is not None else key
+
     def prepare(self, plan):
         """Stages a decode-only plan whose token ids are not known yet: (plan, bucket, staging
         buffer), or None if its bucket has no recording so far."""
-        width = max(g.block_table.shape[1] for g in plan.groups) if plan.groups else 1
-        key = self.bucket(plan.rows, width)
+        key = self.key_of(plan)
         if key is None or key not in self.graphs:
             return None
         return plan, key, self.graphs[key][1].fill_host(plan)
@@ -224,7 +236,7 @@ class DecodeGraphs:
 
         graph = None
         try:
-            static = StaticBatch(key[0], key[1], len(plan.groups), eng.device, eng.chunk, eng.cache.page_size)
+            static = StaticBatch(key[0], key[1], len(plan.groups), eng.device, eng.chunk, eng.cache.page_size, shared=len(key) > 2)
             static.fill(plan, ids)
             # Once eagerly on a side stream (kernels set their attributes, the allocator warms up), then the capture.
             side = torch.cuda.Stream()
@@ -264,8 +276,7 @@ class DecodeGraphs:
         takes it or its bucket cannot be recorded (now): the caller then runs the pass eagerly. A
         recording that fails loses only itself; its bucket is tried again `RETRY_AFTER` passes later.
         The result is a view of the recording's output: use it before the next replay."""
-        width = max(g.block_table.shape[1] for g in plan.groups) if plan.groups else 1
-        key = self.bucket(plan.rows, width)
+        key = self.key_of(plan)
         self.passes += 1
         if key is None:
             return None
@@ -358,7 +369,7 @@ class PromptGraphs:
         before = tuple(int(plan.row_count[int(s)]) - 1 for s in plan.q_start)
         # which rows are wanted is data (the gather's indices) when a row count was rounded; else part of the shape
         wanted = (len(want_rows),) if rounded else tuple(int(w) for w in want_rows)
-        return q_len, before, rounded, wanted, tuple(tuple(g.block_table.shape) for g in plan.groups)
+        return q_len, before, rounded, wanted, tuple(tuple(g.block_table.shape) for g in plan.groups), sharing_of(plan) is not None
 
     def run(self, plan, ids, want_rows) -> Optional[torch.Tensor]:
         """Logits of the pass through a recording of its shape, or None: the caller runs it eagerly.

@@ -21,15 +21,21 @@ prompt longer than the limit is refused when it is added, and a request whose ne
 have to be fed beyond the limit ends with "length". The step function's own refusal is thus
 never met, and one long request cannot end the others.
 
+Several answers to one prompt (`add_samples`; Kapel's engine shares prompt beginnings through its cache,
+crates/kapel-models/src/cache.rs:74-124) are one request until all but the last of the prompt's tokens are in
+the cache: there it is forked, and every answer feeds the last token by itself, over pages they hold
+together. An answer that then finds no slot or no page waits like any other request and computes its
+prompt when its turn comes, as one that was suspended does.
+
 The scheduler needs of its engine only `cache` (a CacheManager), `step(entries)`, `end(id)` and
-`vocab_size` (and reads `max_positions` and `new_request_ids()` where they exist), so its
+`vocab_size` (and uses `max_positions`, `new_request_ids()` and `fork(id, new_ids)` where they exist), so its
 decisions are tested on the CPU with a stand-in.
 """
 from __future__ import annotations
 
 import itertools
 from collections import deque
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Deque, Dict, List, Optional, Sequence
 
 import numpy as np
@@ -119,6 +125,7 @@ class Scheduler:
             except AttributeError:
                 pass
         self.limit = getattr(engine, "max_positions", None)
+        self.answers: Dict[int, List[int]] = {}      # a request whose prompt is still computed -> the other answers to it
         self.preemptions = 0
         self.passes = 0
         self.staged = None            # (request ids, engine handle) of a decode pass staged ahead of its tokens
@@ -143,11 +150,39 @@ class Scheduler:
         self.waiting.append(rid)
         return rid
 
+    def add_samples(self, request: Request, n: int) -> List[int]:
+        """`n` answers to one prompt, each a request of its own from here on (its events, its cancellation); the i-th draws
+        with the request's seed + i. The prompt is computed once."""
+        if n < 1:
+            raise ValueError(f"{n} answers to a prompt")
+        if getattr(self.engine, "fork", None) is None or len(request.prompt) < 2:
+            return [self.add(replace(request, sampling=replace(request.sampling, seed=request.sampling.seed + i))) for i in range(n)]
+        first = self.add(request)
+        others = []
+        for i in range(1, n):
+            rid = next(self._ids)
+            self.entries[rid] = _Entry(replace(request, sampling=replace(request.sampling, seed=request.sampling.seed + i)))
+            others.append(rid)
+        if others:
+            self.answers[first] = others
+        return [first, *others]
+
     def cancel(self, rid: int) -> None:
         """Ends a request wherever it is; its pages go back (engine.rs:308-318)."""
         entry = self.entries.pop(rid, None)
         if entry is None:
             return
+        others = self.answers.pop(rid, None)
+        if others:                                          # the next answer takes the prompt over
+            self.waiting.appendleft(others[0])
+            if others[1:]:
+                self.answers[others[0]] = others[1:]
+        for first, rest in list(self.answers.items()):
+            if rid in rest:
+                rest.remove(rid)
+                if not rest:
+                    del self.answers[first]
+                return
         if entry.running:
             self.running.remove(rid)
             self.engine.end(rid)
@@ -162,7 +197,7 @@ class Scheduler:
 
     def stats(self) -> EngineStats:
         return EngineStats(
-            waiting=len(self.waiting), running=len(self.running), pages=self.cache.total_pages(),
+            waiting=len(self.waiting) + sum(len(o) for o in self.answers.values()), running=len(self.running), pages=self.cache.total_pages(),
             free_pages=self.cache.free_pages(), preemptions=self.preemptions, passes=self.passes,
             recorded_passes=getattr(self.engine, "recorded_passes", 0), released_pages=self.cache.released_pages,
         )
@@ -210,9 +245,10 @@ class Scheduler:
                 if not self.running and any(needed[g] > total[g] for g in range(n_groups)):
                     # It could never run, even alone in an empty cache: end it instead of waiting forever.
                     self.waiting.popleft()
-                    del self.entries[rid]
                     g = next(g for g in range(n_groups) if needed[g] > total[g])
-                    events.append(Event(rid, None, "error", str(CacheFull(needed[g], total[g], self.cache.groups[g].name))))
+                    for each in (rid, *self.answers.pop(rid, ())):
+                        del self.entries[each]
+                        events.append(Event(each, None, "error", str(CacheFull(needed[g], total[g], self.cache.groups[g].name))))
                     continue
                 break
             for g in range(n_groups):
@@ -222,6 +258,34 @@ class Scheduler:
             entry.running = True
             self.running.append(rid)
         return events
+
+    def _fork(self) -> None:
+        """Answers whose prompt is in the cache but for its last token go on from there, beside the request that computed it, as far
+        as there are slots and pages for them; the others wait, ahead of everybody, as requests of their own."""
+        for first in [rid for rid in self.answers if self.entries[rid].running and self._cached(rid) == self.entries[rid].prompt_len - 1]:
+            others = self.answers.pop(first)
+            promised = [0] * len(self.cache.groups)
+            for rid in self.running:
+                for g, n in enumerate(self._peak_need(rid, self._pending(rid) + 1)):
+                    promised[g] += n
+            each = [n + 1 for n in self._peak_need(first, 2)]       # the copy of the last page, what the next two tokens take
+            total, free = self.cache.total_pages(), self.cache.free_pages()
+            room = [free[g] - promised[g] - int(np.ceil(self.options.reserve * total[g])) for g in range(len(total))]
+            fit = min([self.options.max_sequences - len(self.running), self.cache.free_slots(), len(others)] + [r // e for r, e in zip(room, each)])
+            go, wait = others[: max(0, fit)], others[max(0, fit) :]
+            if go:
+                try:
+                    self.engine.fork(first, go)
+                except Exception as e:
+                    self.waiting.extendleft(reversed(others))
+                    if not isinstance(e, CacheFull):
+                        raise
+                    continue
+                at = self.running.index(first) + 1                  # rows that share pages lie beside one another
+                self.running[at:at] = go
+                for rid in go:
+                    self.entries[rid].running = True
+            self.waiting.extendleft(reversed(wait))
 
     def _suspend_last(self) -> None:
         rid = self.running.pop()
@@ -234,12 +298,14 @@ class Scheduler:
         budget = max(1, self.options.max_pass_tokens)
         out = []
         for rid in self.running:
-            if self._pending(rid) == 1:
+            if self._pending(rid) == 1 and rid not in self.answers:
                 out.append((rid, 1))
                 budget = max(0, budget - 1)
         for rid in self.running:
             pending = self._pending(rid)
-            if pending > 1 and budget > 0:
+            if rid in self.answers:
+                pending -= 1                                # the last token of its prompt is fed behind the fork
+            if (pending > 1 or (pending == 1 and rid in self.answers)) and budget > 0:
                 count = min(pending, budget)
                 out.append((rid, count))
                 budget -= count
@@ -249,7 +315,13 @@ class Scheduler:
     def step(self) -> List[Event]:
         """One pass of the model: a token of every decoding request and portions of prompts.
         Returns the tokens it gave and the requests that ended; nothing when there is no work."""
-        events = self._admit()
+        events: List[Event] = []
+        if self.answers:
+            try:
+                self._fork()
+            except Exception as e:                      # the copies could not be made: as if the pass had failed
+                return self._fail_pass(events, e)
+        events += self._admit()
         ahead, self.ahead = self.ahead, None
         if ahead is not None:
             # This pass is already on its way (enqueued while the host still read the tokens before).

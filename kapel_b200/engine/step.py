@@ -303,6 +303,36 @@ class Engine:
     def recorded_passes(self) -> int:
         return (self.graphs.replays if self.graphs is not None else 0) + (self.prompt_graphs.replays if self.prompt_graphs is not None else 0)
 
+    def fork(self, seq_id, new_ids: Sequence[Hashable]) -> None:
+        """Adds requests that go on where `seq_id` is: they hold the pages of its positions together with it (`CacheManager.fork`), each with a
+        copy of the last one where that is not full and of every state. What they are fed from here on is their own. Raises
+        `CacheFull` and adds none where a slot or a page is lacking. The copies are enqueued on the current stream."""
+        new_ids = list(new_ids)
+        made, copies = [], []
+        try:
+            for new_id in new_ids:
+                copies += self.cache.fork(seq_id, new_id)
+                made.append(new_id)
+            pairs = [[(a, b) for at, a, b in copies if at == g] for g in range(len(self.cache.groups))]
+            slots = [(self.cache.slot(seq_id), self.cache.slot(n)) for n in new_ids] if self.cache.states else []
+            host = torch.tensor([p for group in (*pairs, slots) for p in group], dtype=torch.int32).reshape(-1, 2).t().contiguous()
+            if host.numel():
+                dev = host.pin_memory().to(self.device, non_blocking=True)
+                at = 0
+                for group, of in zip(self.cache.groups, pairs):
+                    source, target = dev[0, at : at + len(of)], dev[1, at : at + len(of)]
+                    at += len(of)
+                    for layer in group.layers if of else ():
+                        K.copy_rows(group.keys[layer], source, target)
+                        if group.values[layer] is not group.keys[layer]:
+                            K.copy_rows(group.values[layer], source, target)
+                for table in self.cache.states.values() if slots else ():
+                    K.copy_rows(table, dev[0, at:], dev[1, at:])
+        except Exception:
+            for new_id in made:
+                self.cache.remove_sequence(new_id)
+            raise
+
     def end(self, seq_id) -> None:
         """The request is finished: everything it holds goes back."""
         if seq_id in self.cache:

@@ -4,6 +4,7 @@
     tokens = model.generate([2, 651, 6037], max_tokens=64)                  # greedy
     tokens = model.generate(prompt_ids, max_tokens=64, temperature=0.8, seed=7)
     for token in model.generate(prompt_ids, stream=True): ...
+    answers = model.generate_samples(prompt_ids, 8, max_tokens=64, temperature=0.8, top_p=0.95)      # eight answers to one prompt
 
 Option names and meanings are Kapel's. Prompts are token ids; a text prompt needs the folder's
 tokenizer.json and the `tokenizers` package, which this engine does not itself provide. Quantized
@@ -184,8 +185,37 @@ class Model:
         self.last_stats = sched.stats()
         return [out[rid] for rid in ids]
 
+    def generate_samples(self, prompt: Union[str, Sequence[int]], n: int, max_tokens: Optional[int] = None,
+                         temperature: Optional[float] = None, top_k: Optional[int] = None, top_p: Optional[float] = None,
+                         min_p: Optional[float] = None, repetition_penalty: Optional[float] = None,
+                         seed: Optional[int] = None, stop: Optional[Sequence] = None, ignore_eos: bool = False,
+                         max_sequences: Optional[int] = None):
+        """`n` answers to one prompt (token ids in, lists of token ids out; text in, texts out); answer i draws with seed + i. The
+        prompt is computed once and its pages are held together; a step reads them once for all answers that run."""
+        as_text = isinstance(prompt, str)
+        ids = self.tokenize(prompt) if as_text else [int(t) for t in prompt]
+        request = self._request(ids, max_tokens, temperature, top_k, top_p, min_p, repetition_penalty, seed, stop, ignore_eos)
+        sched = Scheduler(self.engine, EngineOptions(max_pass_tokens=self.max_pass_tokens,
+                                                     max_sequences=min(self.max_sequences, max(1, n if max_sequences is None else max_sequences))))
+        self.last_scheduler = sched
+        rids = sched.add_samples(request, n)
+        out = {rid: [] for rid in rids}
+        try:
+            while sched.has_work():
+                for ev in sched.step():
+                    if ev.finish == "error":
+                        raise KapelError(ev.error or "the pass failed")
+                    if ev.token is not None and ev.finish != "eos":
+                        out[ev.id].append(ev.token)
+        finally:
+            for rid in rids:
+                sched.cancel(rid)
+        self.last_stats = sched.stats()
+        answers = [out[rid] for rid in rids]
+        return [self.detokenize(a, skip_special_tokens=True) for a in answers] if as_text else answers
+
     def scheduler(self, **options) -> Scheduler:
-        """A scheduler of one's own over this model: `add`, `cancel`, `step`, `stats`."""
+        """A scheduler of one's own over this model: `add`, `add_samples`, `cancel`, `step`, `stats`."""
         options.setdefault("max_pass_tokens", self.max_pass_tokens)
         options.setdefault("max_sequences", self.max_sequences)
         return Scheduler(self.engine, EngineOptions(**options))

@@ -216,6 +216,15 @@ class Attention(Part):
         return CacheNeeds(paged=PagedKV(s.num_kv_heads, s.head_dim, s.window, s.keep_first if s.window else 0,
                                         self.v_dim if self.v_dim != s.head_dim else None))
 
+    def shared_pages(self, q, batch, group, k_table, v_table):
+        """Attention of a step of single tokens some of which share pages, reading those once; None where nothing is shared or that kernel does
+        not take the layer."""
+        s, share = self.spec, getattr(batch, "share", None)
+        if share is None or (s.window and s.keep_first) or not K.shared_prefix_takes(q.dtype, s.num_heads, s.num_kv_heads, s.head_dim, self.v_dim, self.ctx.page_size):
+            return None
+        return K.shared_prefix_attention(q.view(-1, s.num_heads, s.head_dim), k_table, v_table, group.block_table, batch.row_count, share[0], share[1], self.ctx.page_size, s.window,
+                                         s.scale, s.softcap, sinks=getattr(self, "sinks", None))
+
     def forward_pooled(self, h, batch, cache):
         s, dv = self.spec, self.v_dim
         nq, nk = s.num_heads * s.head_dim, s.num_kv_heads * s.head_dim
@@ -301,8 +310,8 @@ class Attention(Part):
                                    s.num_heads, s.num_kv_heads, s.head_dim, dv, cache.owns, self.ctx.dtype)
         heads_per_kv = s.num_heads // s.num_kv_heads
         keep = s.keep_first if s.window else 0
-        y = None
-        if dv == s.head_dim and K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
+        y = self.shared_pages(q, batch, group, k_table, v_table)
+        if y is None and dv == s.head_dim and K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
             # with kept first keys only prompt portions go to the tensor-core kernel; a pass of single tokens stays with
             # the row-wise kernel below
             prompt = "mma" if keep else K.attention_prompt_kernel(s.num_heads, s.num_kv_heads, s.head_dim, self.ctx.page_size, s.softcap,
@@ -345,7 +354,10 @@ class Attention(Part):
                                     self.position.tables(batch) if rotary else None, rotary, group.lines, k_table, v_table,
                                     s.num_heads, s.num_kv_heads, s.head_dim, dv, cache.owns, self.ctx.dtype)
         heads_per_kv = s.num_heads // s.num_kv_heads
-        if dv == s.head_dim and s.head_dim % 16 == 0 and K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
+        y = self.shared_pages(q, batch, group, k_table, v_table)
+        if y is not None:
+            pass
+        elif dv == s.head_dim and s.head_dim % 16 == 0 and K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
             prompt = K.attention_prompt_kernel(s.num_heads, s.num_kv_heads, s.head_dim, self.ctx.page_size, s.softcap, s.scale, self.sinks is None)
             decode, tiles, split, slots, relative = batch.attention_tiles(heads_per_kv, s.num_kv_heads, s.window, s.head_dim, prompt)
             y = K.paged_attention_mma(q, k_table, v_table, group.block_table, batch.row_count, tiles, self.ctx.page_size, s.window,
@@ -376,7 +388,7 @@ class Attention(Part):
         k_table, v_table = cache.tables()
         group = batch.groups[cache.group]
         heads_per_kv = s.num_heads // s.num_kv_heads
-        if K.attention_decode_fused_takes(qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim,
+        if getattr(batch, "share", None) is None and K.attention_decode_fused_takes(qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim,
                                           self.ctx.page_size, self.ctx.dtype):
             decode, tiles, split, slots, relative = batch.attention_tiles(
                 heads_per_kv, s.num_kv_heads, s.window, s.head_dim,
@@ -392,7 +404,10 @@ class Attention(Part):
             s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim, write_kv=cache.owns,
             out_dtype=self.ctx.dtype,
         )
-        if K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
+        y = self.shared_pages(q, batch, group, k_table, v_table)
+        if y is not None:
+            pass
+        elif K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
             prompt = K.attention_prompt_kernel(s.num_heads, s.num_kv_heads, s.head_dim, self.ctx.page_size, s.softcap, s.scale)
             mixed = batch.mixed_tiles(heads_per_kv, s.num_kv_heads, s.window, s.head_dim, prompt) if prompt != "mma" else None
             if mixed is not None:       # single tokens ahead of portions: each by the kernel made for them
