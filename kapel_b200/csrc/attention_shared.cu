@@ -5,7 +5,8 @@
 // computes every eighth position's score out of keys and queries in shared memory, and keeps every eighth group of four components of the
 // sum in registers. All arithmetic is 32-bit. Where some row of the tile does not see all of a unit (its window begins there, its
 // positions end there) what a row does not see is left out of its sum, not multiplied by zero: it may be anything.
-#include "attention_shared.cuh"
+#include "attention_shared_bf16.cuh"
+#include "tensor_map.cuh"
 
 namespace kb {
 
@@ -16,7 +17,8 @@ template <typename T> struct SharedRowsSmem {
     float k[SR_KEYS][SR_DIM + 4];
     float v[SR_KEYS][SR_DIM];
     long long line[SR_KEYS];               // a position's line of this kv head in the tables, -1 for none
-    SharedCut cut;
+    SharedTiles tiles;
+    int upto[SH_ROWS + 1];                 // units before a row
 };
 
 template <typename T>
@@ -28,15 +30,32 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
     const T* q = static_cast<const T*>(p.q);
     const T* kt = static_cast<const T*>(p.k_table);
     const T* vt = static_cast<const T*>(p.v_table);
-    shared_make_cut(p, s.cut, rows_a_tile, SR_KEYS);
-    if (blockIdx.x == 0) shared_leave_cut(p, s.cut);
-    const long long units = (long long)s.cut.units * p.hkv;
-    const int workers = shared_workers(units);
-    if ((int)blockIdx.x >= workers) return;
-    const int begin = shared_begin(blockIdx.x, units, workers), end = shared_begin(blockIdx.x + 1, units, workers);
+    shared_cut_tiles(p, s.tiles, rows_a_tile, SR_KEYS);
+    shared_cut_rows(p, s.upto, SR_KEYS);
+    const SharedRange over[2] = {shared_range(blockIdx.x, gridDim.x, s.tiles.upto[s.tiles.tiles], p.hkv), shared_range(blockIdx.x, gridDim.x, s.upto[p.rows], p.hkv)};
+    if (blockIdx.x == 0) {
+        shared_leave_tiles(p, s.tiles, over[0].workers);
+        shared_leave_rows(p, s.upto, over[1].workers);
+    }
     const int d4 = (p.d + 3) / 4;
-    for (int u = begin; u < end;) {
-        const SharedPart w = shared_part(p, s.cut, u, end, SR_KEYS, SR_PAIRS);
+    for (int kind = 0; kind < 2; ++kind)                     // what is shared, then what each row reads by itself
+    for (int u = over[kind].begin; u < over[kind].end;) {
+        struct { int row0, n, looks, kvh, lo, hi, first_unit, n_units; } w;
+        const int* upto = kind == 0 ? s.tiles.upto : s.upto;
+        const int item = shared_item(upto, kind == 0 ? s.tiles.tiles : p.rows, p.hkv, u);
+        const int units = upto[item + 1] - upto[item], in = u - upto[item] * p.hkv;
+        w.kvh = in / units;
+        w.first_unit = in % units;
+        w.n_units = min(units - w.first_unit, over[kind].end - u);
+        float* pieces;
+        if (kind == 0) {
+            w.row0 = s.tiles.row0[item]; w.n = s.tiles.n[item]; w.looks = s.tiles.looks[item]; w.lo = s.tiles.klo[item]; w.hi = s.tiles.khi[item];
+            pieces = p.tile_pieces + shared_tile_place(p, s.tiles.before[item], w.n, w.kvh, blockIdx.x, SR_PAIRS) * SH_PIECE(p.dv);
+        } else {
+            w.row0 = w.looks = item; w.n = 1;
+            shared_own(p, item, SR_KEYS, w.lo, w.hi);
+            pieces = p.row_pieces + shared_row_place(p, item, w.kvh, blockIdx.x) * SH_PIECE(p.dv);
+        }
         u += w.n_units;
         const int pairs = w.n * group;
         const int row = w.row0 + pair / group;
@@ -130,7 +149,7 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
                 }
         }
         if (own) {
-            float* piece = p.pieces + (w.place + pair) * (p.dv + 2);
+            float* piece = pieces + (size_t)pair * SH_PIECE(p.dv);
 #pragma unroll
             for (int c = 0; c < SR_DIM / 32; ++c) {
                 const int at = 32 * c + 4 * sub;
@@ -144,54 +163,48 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
     }
 }
 
-// Joins a (row, head) pair's pieces: its tile's, block by block, then its own. A block a pair.
+// Joins a (row, head) pair's pieces: its tile's, worker by worker, then its own. A block a pair.
 constexpr int SJ_THREADS = 128;
 template <typename T>
 __global__ void __launch_bounds__(SJ_THREADS) shared_combine_kernel(const SharedParams p, int tile_pairs) {
     const int r = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-    const int group = p.hq / p.hkv, kvh = head / group;
-    const int* cut = p.cut;
-    const int tiles = cut[0], blocks = cut[2], tile_rows_total = cut[3];
-    const int units = cut[1] * p.hkv;
-    const int* upto = cut + SH_CUT_HEAD + 4 * SH_ROWS;
-    const int t = cut[SH_CUT_HEAD + r];
-    long long place[2];
-    int first[2] = {0, 0}, last[2] = {-1, -1};           // blocks that have a piece, of the tile and of the row itself
+    const int group = p.hq / p.hkv, kvh = head / group, width = SH_PIECE(p.dv);
+    const int t = p.cut[SH_CUT_ROW_TILE + r], tiles = p.cut[SH_CUT_COUNTS];
+    const float* piece[2] = {nullptr, nullptr};          // the first of the tile's and of the row's, and the floats from one to the next
+    int count[2] = {0, 0};
+    const size_t step[2] = {(size_t)tile_pairs * width, (size_t)group * width};
     for (int k = 0; k < 2; ++k) {
-        const int item = k == 0 ? t : tiles + r;
-        place[k] = 0;
+        const int item = k == 0 ? t : r;
+        const int* upto = p.cut + (k == 0 ? SH_CUT_TILE_UNITS : SH_CUT_ROW_UNITS);
         if (item < 0) continue;
         const int n = upto[item + 1] - upto[item];
         if (n == 0) continue;
-        const long long u = (long long)upto[item] * p.hkv + (long long)kvh * n;
-        first[k] = shared_block_of(u, units, blocks);
-        last[k] = shared_block_of(u + n - 1, units, blocks);
-        if (k == 0) {
-            const int* tile = cut + SH_CUT_HEAD + SH_ROWS + 3 * t;
-            place[k] = ((long long)tile[2] * p.hkv + (long long)kvh * tile[1] + (r - tile[0])) * group + head % group;
-        } else {
-            place[k] = ((long long)(tile_rows_total + r) * p.hkv + kvh) * group + head % group;
-        }
+        const long long u = (long long)upto[item] * p.hkv + (long long)kvh * n, all = (long long)upto[k == 0 ? tiles : p.rows] * p.hkv;
+        const int workers = p.cut[SH_CUT_COUNTS + 1 + k];
+        const int first = shared_worker_of(u, all, workers);
+        count[k] = shared_worker_of(u + n - 1, all, workers) - first + 1;
+        const int* tile = p.cut + SH_CUT_TILES + 3 * t;
+        piece[k] = k == 0 ? p.tile_pieces + (shared_tile_place(p, tile[2], tile[1], kvh, first, tile_pairs) + (r - tile[0]) * group + head % group) * width
+                          : p.row_pieces + (shared_row_place(p, r, kvh, first) + head % group) * width;
     }
-    const int width = p.dv + 2;
     float m = p.sinks ? p.sinks[head] : -INFINITY;
     for (int k = 0; k < 2; ++k)
-        for (int b = first[k]; b <= last[k]; ++b) m = fmaxf(m, p.pieces[(place[k] + (long long)b * tile_pairs) * width + p.dv]);
+        for (int b = 0; b < count[k]; ++b) m = fmaxf(m, piece[k][b * step[k] + p.dv]);
     float total = p.sinks && m != -INFINITY ? expf(p.sinks[head] - m) : 0.f;
     constexpr int MOST = SR_DIM / SJ_THREADS;
     float sum[MOST];
 #pragma unroll
     for (int j = 0; j < MOST; ++j) sum[j] = 0.f;
     for (int k = 0; k < 2; ++k)
-        for (int b = first[k]; b <= last[k]; ++b) {
-            const float* piece = p.pieces + (place[k] + (long long)b * tile_pairs) * width;
-            const float pm = piece[p.dv];
+        for (int b = 0; b < count[k]; ++b) {
+            const float* x = piece[k] + b * step[k];
+            const float pm = x[p.dv];
             if (pm == -INFINITY) continue;               // a range of which the row sees nothing
             const float fade = expf(pm - m);
-            total = fmaf(fade, piece[p.dv + 1], total);
+            total = fmaf(fade, x[p.dv + 1], total);
 #pragma unroll
             for (int j = 0; j < MOST; ++j)
-                if (tid + j * SJ_THREADS < p.dv) sum[j] = fmaf(fade, piece[tid + j * SJ_THREADS], sum[j]);
+                if (tid + j * SJ_THREADS < p.dv) sum[j] = fmaf(fade, x[tid + j * SJ_THREADS], sum[j]);
         }
     const float inv = total > 0.f ? 1.f / total : 0.f;
     T* out = static_cast<T*>(p.out) + ((size_t)r * p.hq + head) * p.dv;
@@ -216,10 +229,21 @@ using namespace kb;
 
 static int shared_blocks() { return multiprocessors(); }
 
-// Floats of scratch memory: the pieces, then the cut.
-extern "C" long long kb_shared_attention_scratch_floats(int rows, int hq, int dv) {
-    if (rows <= 0 || rows > SH_ROWS || hq <= 0 || dv <= 0) return 0;
-    return shared_places(rows, hq, shared_blocks(), SR_PAIRS) * (dv + 2) + SH_CUT_INTS;
+// Whether the tensor cores take a layer (bfloat16): one head size, whole groups of 16 positions a page, up to 16 query heads a kv head.
+static bool shared_on_tensor_cores(int dtype, int hq, int hkv, int d, int dv, int page_size) {
+    return dtype == KB_DT_BF16 && d == dv && (d == 64 || d == 128 || d == 256) && page_size % 16 == 0 && hq / hkv <= 16;
+}
+
+struct SharedScratch { long long tile_places, row_places; };
+static SharedScratch shared_scratch(int rows, int hq, int hkv, int d) {          // what either path needs at most
+    const int blocks = shared_blocks();
+    return SharedScratch{shared_tile_places(rows, hq, blocks, 128), shared_row_places(rows, hq, hkv, blocks * shared_own_workers(d))};
+}
+// Floats of scratch memory: the tiles' pieces, the rows' pieces, then the cut.
+extern "C" long long kb_shared_attention_scratch_floats(int rows, int hq, int hkv, int d, int dv) {
+    if (rows <= 0 || rows > SH_ROWS || hq <= 0 || hkv <= 0 || hq % hkv || dv <= 0) return 0;
+    const SharedScratch x = shared_scratch(rows, hq, hkv, d);
+    return (x.tile_places + x.row_places) * SH_PIECE(dv) + SH_CUT_INTS;
 }
 
 // 1 where the kernels take these sizes.
@@ -237,16 +261,31 @@ extern "C" int kb_shared_attention(void* out, const void* q, const void* k_table
                "shared_attention: dtype code %d, %d heads over %d of %d / %d, pages of %d are not taken", dtype, hq, hkv, d, dv, page_size);
     KB_REQUIRE(table_width > 0 && n_pages > 0 && window >= 0 && cap >= 0.f, "shared_attention: table width %d, pages %d, window %d, soft cap %g", table_width,
                n_pages, window, cap);
-    KB_REQUIRE((long long)table_width * page_size <= 0x7fffffffll / 4 && ((long long)table_width * page_size / SR_KEYS + 2) * 2 * rows * hkv <= 0x7fffffffll,
+    KB_REQUIRE((long long)table_width * page_size <= 0x7fffffffll / 4 && ((long long)table_width * page_size / 16 + 2) * rows * hkv <= 0x7fffffffll,
                "shared_attention: %d block tables of %d pages of %d positions are too many for one launch", rows, table_width, page_size);
     if (rows == 0) return 0;
-    KB_REQUIRE(scratch != nullptr && scratch_floats >= kb_shared_attention_scratch_floats(rows, hq, dv), "shared_attention: scratch memory of %lld floats",
+    KB_REQUIRE(scratch != nullptr && scratch_floats >= kb_shared_attention_scratch_floats(rows, hq, hkv, d, dv), "shared_attention: scratch memory of %lld floats",
                scratch_floats);
     SharedParams p = {};
     p.q = q; p.k_table = k_table; p.v_table = v_table; p.block_table = block_table; p.row_count = row_count; p.share_id = share_id;
-    p.share_len = share_len; p.sinks = sinks; p.out = out; p.pieces = scratch; p.rows = rows; p.hq = hq; p.hkv = hkv; p.d = d; p.dv = dv;
+    p.share_len = share_len; p.sinks = sinks; p.out = out; p.rows = rows; p.hq = hq; p.hkv = hkv; p.d = d; p.dv = dv;
     p.page_size = page_size; p.table_width = table_width; p.n_pages = n_pages; p.window = window; p.scale = scale; p.cap = cap;
     const int blocks = shared_blocks();
-    p.cut = reinterpret_cast<int*>(scratch + shared_places(rows, hq, blocks, SR_PAIRS) * (dv + 2));
+    const SharedScratch x = shared_scratch(rows, hq, hkv, d);
+    p.tile_pieces = scratch;
+    p.row_pieces = scratch + x.tile_places * SH_PIECE(dv);
+    p.cut = reinterpret_cast<int*>(p.row_pieces + x.row_places * SH_PIECE(dv));
+    if (shared_on_tensor_cores(dtype, hq, hkv, d, dv, page_size)) {
+        KB_REQUIRE((((uintptr_t)q | (uintptr_t)k_table | (uintptr_t)v_table) & 15) == 0, "shared_attention: operands must be 16-byte aligned");
+        const unsigned long long lines = (unsigned long long)n_pages * hkv * page_size;
+        KB_REQUIRE(lines <= 0x7fffffffull, "shared_attention: tables of %llu lines", lines);
+        CUtensorMap mk, mv;
+        if (int e = encode_map_bf16(&mk, k_table, lines, d, d, 16)) return e;
+        if (int e = encode_map_bf16(&mv, v_table, lines, d, d, 16)) return e;
+        if (int e = launch_shared_tiles(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
+        if (int e = launch_shared_own(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
+        shared_combine_kernel<__nv_bfloat16><<<dim3(rows, hq), SJ_THREADS, 0, (cudaStream_t)stream>>>(p, 128);
+        return check_launch("shared_attention");
+    }
     return dtype == KB_DT_F32 ? launch_shared_rows<float>(p, blocks, (cudaStream_t)stream) : launch_shared_rows<__nv_bfloat16>(p, blocks, (cudaStream_t)stream);
 }

@@ -2,24 +2,27 @@
 //
 // Row r is request r: it has seen row_count[r] positions, its own included, and reads those its window leaves. Rows that follow one another with
 // the same share_id and share_len share the pages of their first share_len positions (whole pages, looked up in the block table of the
-// row that sees furthest back: behind a window the others may have given their first pages back). Such a run is cut into tiles of at most `tile_rows` (row, query head) pairs of one kv head; a tile reads the positions that any of
-// its rows sees of what they share, once. What a row has behind that is an item of its own. So
+// row that sees furthest back: behind a window the others may have given their first pages back). Such a run is cut into tiles of at most
+// `tile_pairs` (row, query head) pairs of one kv head; a tile reads the positions that any of its rows sees of what they share, once. What a
+// row has behind that it reads by itself. So
 //   out = sum e^x v / (sum e^x + e^sink) over the row's positions
-// is put together from pieces (sum e^(x - m) v, m, sum e^(x - m)), each over a range of positions.
+// is put together from pieces (sum e^(x - m) v, m, sum e^(x - m)), each over a range of positions, which `shared_combine_kernel` joins.
 //
-// The cut is made on the device (lengths change from step to step, a recorded step's launch does not). An item is (a tile or a row,
-// its positions); its units are `keys` positions each, times the kv heads. All items' units lie one after the other, and block b of G takes the
-// units [U b / G, U (b + 1) / G), with G no more than U: every block the same number, whether a few long prompts or many short answers make them up. Where a block's
-// range ends inside an item its piece is one of several; they are joined by `shared_combine_kernel`.
+// The cut is made on the device (lengths change from step to step, a recorded step's launch does not), for tiles and for rows alike. An
+// item is a tile or a row with its positions; its units are so many positions each, times the kv heads. All items' units lie one
+// after the other, and worker w of W (a block, or a warp) takes the units [U w / W, U (w + 1) / W), with W no more than U: every worker the
+// same number, whether a few long prompts or many short answers make them up. Where a worker's range ends inside an item its piece is
+// one of several.
 //
-// Pieces are written by (row, head) to a place that follows from the cut alone: the items' rows before it plus `tile_rows` for each block
-// before the one that writes: a block's pieces of different items cannot meet, nor those of different blocks of one item.
+// Pieces go to a place that follows from the cut alone: the pairs of the items before, plus a full item's pairs for each worker before the
+// one that writes: a worker's pieces of different items cannot meet, nor those of different workers of one item.
 #pragma once
 #include "common.cuh"
 
 namespace kb {
 
 constexpr int SH_ROWS = 512;                 // requests of one call
+__host__ __device__ constexpr int SH_PIECE(int dv) { return (dv + 3) / 4 * 4 + 4; }      // floats of a piece: dv, then m and the sum of weights; rows of 16 bytes
 
 struct SharedParams {
     const void* q;             // [rows, hq, d]
@@ -31,25 +34,27 @@ struct SharedParams {
     const int* share_len;      // [rows]
     const float* sinks;        // [hq] or null
     void* out;                 // [rows, hq, dv]
-    float* pieces;             // [places, dv + 2]: (sum, m, sum of weights), m in natural units
-    int* cut;                  // what block 0 leaves for the kernel that joins: see SharedCut
+    float* tile_pieces;        // [places, SH_PIECE]: (sum, m, sum of weights), m in natural units; of tiles,
+    float* row_pieces;         // ... and of rows
+    int* cut;                  // what the kernels leave for the one that joins: see SH_CUT_*
     int rows, hq, hkv, d, dv, page_size, table_width, n_pages, window;
     float scale, cap;
 };
 
-// The cut as the joining kernel reads it, in p.cut: [0] tiles, [1] units, [2] blocks, [3] rows in tiles; then SH_ROWS tiles of each row (-1:
-// none), then for each tile {first row, rows, rows in tiles before}, then the running total of units over tiles and rows (one more than items).
-constexpr int SH_CUT_HEAD = 4;
-constexpr int SH_CUT_INTS = SH_CUT_HEAD + SH_ROWS + 3 * SH_ROWS + 2 * SH_ROWS + 1;
+// The cut as the joining kernel reads it, in p.cut: the tile of each row (-1: none), for each tile {first row, rows, rows in tiles before}, and for tiles
+// and rows the running total of their units (of one kv head; one more than there are), the number of items and of workers.
+constexpr int SH_CUT_ROW_TILE = 0, SH_CUT_TILES = SH_ROWS, SH_CUT_TILE_UNITS = 4 * SH_ROWS, SH_CUT_ROW_UNITS = 5 * SH_ROWS + 1;
+constexpr int SH_CUT_COUNTS = 6 * SH_ROWS + 2;           // tiles, workers over tiles, workers over rows
+constexpr int SH_CUT_INTS = SH_CUT_COUNTS + 3;
 
-// A block's copy of the cut.
-struct SharedCut {
-    int tiles, units, tile_rows_total;
-    int row_tile[SH_ROWS];                   // a row's tile, -1 where it shares nothing that it sees
-    int row0[SH_ROWS], n[SH_ROWS], before[SH_ROWS];      // by tile
+// A block's copy of the cut into tiles.
+struct SharedTiles {
+    int tiles;
+    int row_tile[SH_ROWS];                   // a row's tile, -1 where it shares nothing
+    int row0[SH_ROWS], n[SH_ROWS], before[SH_ROWS + 1];      // by tile
     int looks[SH_ROWS];                      // by tile: the row whose block table has the pages
     int klo[SH_ROWS], khi[SH_ROWS];          // by tile: the positions [klo, khi) that any row sees of what they share
-    int upto[2 * SH_ROWS + 1];               // units (of one kv head) before item i: tiles, then rows
+    int upto[SH_ROWS + 1];                   // units before tile i
 };
 
 __device__ __forceinline__ int shared_first(const SharedParams& p, int count) {      // the first position a row sees
@@ -60,14 +65,34 @@ __device__ __forceinline__ int shared_length(const SharedParams& p, int r) {
     const int n = min(min(p.share_len[r], p.row_count[r]), p.table_width * p.page_size);
     return n > 0 ? n / p.page_size * p.page_size : 0;
 }
-__device__ __forceinline__ int shared_own_units(const SharedParams& p, int r, int length, int keys, int& lo, int& hi) {
+// The positions [lo, hi) that a row reads by itself; returns their units of `keys`, counted from a multiple of `keys`.
+__device__ __forceinline__ int shared_own(const SharedParams& p, int r, int keys, int& lo, int& hi) {
     hi = min(p.row_count[r], p.table_width * p.page_size);
-    lo = max(length, shared_first(p, p.row_count[r]));
+    lo = max(shared_length(p, r), shared_first(p, p.row_count[r]));
     return lo < hi ? (hi - lo / keys * keys + keys - 1) / keys : 0;
 }
 
-// Makes the cut with the whole block (any number of warps); `rows_a_tile` requests to a tile, `keys` positions to a unit.
-__device__ void shared_make_cut(const SharedParams& p, SharedCut& c, int rows_a_tile, int keys) {
+// Running totals over n items, by the block's first warp: upto[i] = what `of` gives for the items before i. No barrier.
+template <typename F> __device__ __forceinline__ void shared_totals(int* upto, int n, F of) {
+    const int lane = threadIdx.x & 31;
+    int total = 0;
+    for (int base = 0; base < n; base += 32) {
+        const int i = base + lane;
+        const int mine = i < n ? of(i) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        if (i < n) upto[i] = total + sum - mine;
+        total += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) upto[n] = total;
+}
+
+// The cut into tiles, by the whole block; `rows_a_tile` requests to a tile, `keys` positions to a unit.
+__device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, int rows_a_tile, int keys) {
     const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x;
     for (int i = tid; i < p.rows; i += nt) { c.klo[i] = 0x7fffffff; c.khi[i] = 0; c.n[i] = 0; c.row0[i] = 0x7fffffff; c.looks[i] = 0x7fffffff; }
     if (tid < 32) {
@@ -107,97 +132,62 @@ __device__ void shared_make_cut(const SharedParams& p, SharedCut& c, int rows_a_
         if (t >= 0 && shared_first(p, p.row_count[r]) <= c.klo[t]) atomicMin(&c.looks[t], r);
     }
     if (tid < 32) {
-        int units = 0, rows_before = 0;
-        const int tiles = c.tiles, items = tiles + p.rows;
-        for (int base = 0; base < items; base += 32) {
-            const int i = base + lane;
-            int u = 0, n = 0;
-            if (i < tiles) {
-                n = c.n[i];
-                if (c.klo[i] < c.khi[i]) u = (c.khi[i] - c.klo[i] / keys * keys + keys - 1) / keys;
-            } else if (i < items) {
-                int lo, hi;
-                u = shared_own_units(p, i - tiles, shared_length(p, i - tiles), keys, lo, hi);
-            }
-            int uu = u, nn = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int a = __shfl_up_sync(0xffffffffu, uu, o), b = __shfl_up_sync(0xffffffffu, nn, o);
-                if (lane >= o) { uu += a; nn += b; }
-            }
-            if (i < items) c.upto[i] = units + uu - u;
-            if (i < tiles) c.before[i] = rows_before + nn - n;
-            units += __shfl_sync(0xffffffffu, uu, 31);
-            rows_before += __shfl_sync(0xffffffffu, nn, 31);
-        }
-        if (lane == 0) { c.upto[items] = units; c.units = units; c.tile_rows_total = rows_before; }
+        shared_totals(c.before, c.tiles, [&](int i) { return c.n[i]; });
+        shared_totals(c.upto, c.tiles, [&](int i) { return c.klo[i] < c.khi[i] ? (c.khi[i] - c.klo[i] / keys * keys + keys - 1) / keys : 0; });
     }
     __syncthreads();
 }
 
-// Blocks that have work: one a unit at least, so that no block between two that share an item is without a piece of it.
-__device__ __forceinline__ int shared_workers(long long units) { return (int)min((long long)gridDim.x, units); }
-
-// Block 0 leaves the cut for the joining kernel.
-__device__ void shared_leave_cut(const SharedParams& p, const SharedCut& c) {
-    int* out = p.cut;
-    if (threadIdx.x == 0) { out[0] = c.tiles; out[1] = c.units; out[2] = shared_workers((long long)c.units * p.hkv); out[3] = c.tile_rows_total; }
-    for (int i = threadIdx.x; i < p.rows; i += blockDim.x) out[SH_CUT_HEAD + i] = c.row_tile[i];
-    for (int i = threadIdx.x; i < c.tiles; i += blockDim.x) {
-        int* t = out + SH_CUT_HEAD + SH_ROWS + 3 * i;
-        t[0] = c.row0[i]; t[1] = c.n[i]; t[2] = c.before[i];
-    }
-    for (int i = threadIdx.x; i <= c.tiles + p.rows; i += blockDim.x) out[SH_CUT_HEAD + 4 * SH_ROWS + i] = c.upto[i];
+// The cut into rows: upto[r] = units before row r. By the whole block.
+__device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int keys) {
+    if (threadIdx.x < 32) shared_totals(upto, p.rows, [&](int r) { int lo, hi; return shared_own(p, r, keys, lo, hi); });
+    __syncthreads();
 }
 
-// The block that has unit u of U, and a block's first unit.
-__device__ __forceinline__ int shared_block_of(long long u, int units, int blocks) { return (int)(((u + 1) * blocks - 1) / units); }
-__device__ __forceinline__ int shared_begin(int b, long long units, int blocks) { return (int)(units * b / blocks); }
-
-// One item's part of a block's range.
-struct SharedPart {
-    int item, kvh;             // tiles first, then rows
-    int row0, n;               // its requests
-    int looks;                 // the one whose block table has the pages
-    int lo, hi;                // positions of the item
-    int first_unit, n_units;   // of the item's units those that this block takes (n_units of them)
-    int whole;                 // whether that is all of them
-    long long place;           // where this block's pieces of it go
-};
-
-// The part that holds the block's unit u (u < end); `tile_pairs` the (row, head) pairs of a full tile.
-__device__ SharedPart shared_part(const SharedParams& p, const SharedCut& c, int u, int end, int keys, int tile_pairs) {
-    SharedPart s;
-    const int items = c.tiles + p.rows;
-    int lo = 0, hi = items;                              // the last item that begins at or before u
+// A worker's units, the items' one after the other and each item's kv head by kv head.
+struct SharedRange { int begin, end, workers; };
+__device__ __forceinline__ SharedRange shared_range(int worker, int most, int units, int hkv) {
+    const long long all = (long long)units * hkv;
+    SharedRange r;
+    r.workers = (int)min((long long)most, all);
+    r.begin = worker < r.workers ? (int)(all * worker / r.workers) : 0;
+    r.end = worker < r.workers ? (int)(all * (worker + 1) / r.workers) : 0;
+    return r;
+}
+__device__ __forceinline__ int shared_worker_of(long long u, long long units, int workers) { return (int)(((u + 1) * workers - 1) / units); }
+// The item that unit u belongs to: the last that begins at or before it (one without units ends where it begins).
+__device__ __forceinline__ int shared_item(const int* upto, int items, int hkv, int u) {
+    int lo = 0, hi = items;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if ((long long)c.upto[mid] * p.hkv <= u) lo = mid; else hi = mid;
+        if ((long long)upto[mid] * hkv <= u) lo = mid; else hi = mid;
     }
-    s.item = lo;
-    const int units = c.upto[lo + 1] - c.upto[lo];       // of a kv head; not 0, or a later item would begin here too
-    const int in = u - c.upto[lo] * p.hkv;
-    s.kvh = in / units;
-    s.first_unit = in % units;
-    s.n_units = min(units - s.first_unit, end - u);
-    s.whole = s.n_units == units;
-    const int group = p.hq / p.hkv;
-    long long rows_before;
-    if (lo < c.tiles) {
-        s.row0 = c.row0[lo]; s.n = c.n[lo]; s.looks = c.looks[lo]; s.lo = c.klo[lo]; s.hi = c.khi[lo];
-        rows_before = (long long)c.before[lo] * p.hkv + (long long)s.kvh * s.n;
-    } else {
-        s.row0 = s.looks = lo - c.tiles; s.n = 1;
-        shared_own_units(p, s.row0, shared_length(p, s.row0), keys, s.lo, s.hi);
-        rows_before = (long long)(c.tile_rows_total + s.row0) * p.hkv + s.kvh;
-    }
-    s.place = rows_before * group + (long long)blockIdx.x * tile_pairs;
-    return s;
+    return lo;
 }
 
-// Places for pieces: every (row, head) once as a tile's and once as its own, and a full tile for each block.
-__host__ __device__ inline long long shared_places(int rows, int hq, int blocks, int tile_pairs) {
-    return 2ll * rows * hq + (long long)blocks * tile_pairs;
+// One block leaves what it knows of the cut for the joining kernel.
+__device__ inline void shared_leave_tiles(const SharedParams& p, const SharedTiles& c, int workers) {
+    for (int i = threadIdx.x; i < p.rows; i += blockDim.x) p.cut[SH_CUT_ROW_TILE + i] = c.row_tile[i];
+    for (int i = threadIdx.x; i < c.tiles; i += blockDim.x) {
+        int* t = p.cut + SH_CUT_TILES + 3 * i;
+        t[0] = c.row0[i]; t[1] = c.n[i]; t[2] = c.before[i];
+    }
+    for (int i = threadIdx.x; i <= c.tiles; i += blockDim.x) p.cut[SH_CUT_TILE_UNITS + i] = c.upto[i];
+    if (threadIdx.x == 0) { p.cut[SH_CUT_COUNTS] = c.tiles; p.cut[SH_CUT_COUNTS + 1] = workers; }
 }
+__device__ inline void shared_leave_rows(const SharedParams& p, const int* upto, int workers) {
+    for (int i = threadIdx.x; i <= p.rows; i += blockDim.x) p.cut[SH_CUT_ROW_UNITS + i] = upto[i];
+    if (threadIdx.x == 0) p.cut[SH_CUT_COUNTS + 2] = workers;
+}
+
+// Where worker w's pieces of an item go.
+__device__ __forceinline__ long long shared_tile_place(const SharedParams& p, int before, int n, int kvh, int worker, int tile_pairs) {
+    return ((long long)before * p.hkv + (long long)kvh * n) * (p.hq / p.hkv) + (long long)worker * tile_pairs;
+}
+__device__ __forceinline__ long long shared_row_place(const SharedParams& p, int r, int kvh, int worker) {
+    return ((long long)r * p.hkv + kvh + worker) * (p.hq / p.hkv);
+}
+inline long long shared_tile_places(int rows, int hq, int workers, int tile_pairs) { return (long long)rows * hq + (long long)workers * tile_pairs; }
+inline long long shared_row_places(int rows, int hq, int hkv, int workers) { return (long long)rows * hq + (long long)workers * (hq / hkv); }
 
 }  // namespace kb

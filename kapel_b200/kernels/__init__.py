@@ -89,6 +89,8 @@ def check_async_errors() -> None:
         bad.append("tcgen05 attention (a TMA load, an MMA commit or a softmax warp never arrived)")
     if lib.kb_attention_flash_error() != 0:
         bad.append("tcgen05 attention without a soft cap (a TMA load, an MMA commit or a softmax warp never arrived)")
+    if lib.kb_shared_tiles_error() != 0 or lib.kb_shared_own_error() != 0:
+        bad.append("attention over shared pages (a TMA load, an MMA commit or a softmax warp never arrived)")
     if lib.kb_gemm_f32_split_error() != 0:
         bad.append("32-bit product (a TMA load, an MMA commit or a warp of the block never arrived)")
     if lib.kb_delta_chain_error() != 0:
@@ -1076,7 +1078,7 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
         raise KernelError(f"shared attention: a window of {window}")
     out = _fresh((rows, hq, dv), q.dtype, q.device)
     lib = library()
-    need = int(lib.kb_shared_attention_scratch_floats(rows, hq, dv))
+    need = int(lib.kb_shared_attention_scratch_floats(rows, hq, hkv, d, dv))
     scratch = _fresh((need,), torch.float32, q.device) if need else None
     _check(lib.kb_shared_attention(_ptr(out), _ptr(q), _ptr(k_table), _ptr(v_table), dt, _ptr(block_table), _ptr(row_count), _ptr(share_id),
                                    _ptr(share_len), rows, hq, hkv, d, dv, int(page_size), int(block_table.shape[1]), int(n_pages),
