@@ -163,54 +163,85 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
     }
 }
 
-// Joins a (row, head) pair's pieces: its tile's, worker by worker, then its own. A block a pair.
-constexpr int SJ_THREADS = 128;
+// Joins a (row, head) pair's pieces: its tile's, worker by worker, then its own. A block a pair: the pieces' references and sums all at once, then
+// LANES threads a piece, four components each, several pieces side by side; their sums in the order of the threads' groups.
+constexpr int SJ_THREADS = 256, SJ_PIECES = 512;
 template <typename T>
 __global__ void __launch_bounds__(SJ_THREADS) shared_combine_kernel(const SharedParams p, int tile_pairs) {
+    __shared__ float weight[SJ_PIECES];
+    __shared__ float scratch[32];
+    __shared__ float4 part[SJ_THREADS];
     const int r = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
     const int group = p.hq / p.hkv, kvh = head / group, width = SH_PIECE(p.dv);
     const int t = p.cut[SH_CUT_ROW_TILE + r], tiles = p.cut[SH_CUT_COUNTS];
+    const int row_units = p.cut[SH_CUT_ROW_UNITS + r + 1] - p.cut[SH_CUT_ROW_UNITS + r];
     const float* piece[2] = {nullptr, nullptr};          // the first of the tile's and of the row's, and the floats from one to the next
     int count[2] = {0, 0};
     const size_t step[2] = {(size_t)tile_pairs * width, (size_t)group * width};
-    for (int k = 0; k < 2; ++k) {
-        const int item = k == 0 ? t : r;
-        const int* upto = p.cut + (k == 0 ? SH_CUT_TILE_UNITS : SH_CUT_ROW_UNITS);
-        if (item < 0) continue;
-        const int n = upto[item + 1] - upto[item];
-        if (n == 0) continue;
-        const long long u = (long long)upto[item] * p.hkv + (long long)kvh * n, all = (long long)upto[k == 0 ? tiles : p.rows] * p.hkv;
-        const int workers = p.cut[SH_CUT_COUNTS + 1 + k];
-        const int first = shared_worker_of(u, all, workers);
-        count[k] = shared_worker_of(u + n - 1, all, workers) - first + 1;
+    const int tile_units = t < 0 ? 0 : p.cut[SH_CUT_TILE_UNITS + t + 1] - p.cut[SH_CUT_TILE_UNITS + t];
+    if (tile_units > 0) {
         const int* tile = p.cut + SH_CUT_TILES + 3 * t;
-        piece[k] = k == 0 ? p.tile_pieces + (shared_tile_place(p, tile[2], tile[1], kvh, first, tile_pairs) + (r - tile[0]) * group + head % group) * width
-                          : p.row_pieces + (shared_row_place(p, r, kvh, first) + head % group) * width;
+        const long long u = (long long)p.cut[SH_CUT_TILE_UNITS + t] * p.hkv + (long long)kvh * tile_units, all = (long long)p.cut[SH_CUT_TILE_UNITS + tiles] * p.hkv;
+        const int workers = p.cut[SH_CUT_COUNTS + 1], first = shared_worker_of(u, all, workers);
+        count[0] = shared_worker_of(u + tile_units - 1, all, workers) - first + 1;
+        piece[0] = p.tile_pieces + (shared_tile_place(p, tile[2], tile[1], kvh, first, tile_pairs) + (r - tile[0]) * group + head % group) * width;
     }
-    float m = p.sinks ? p.sinks[head] : -INFINITY;
-    for (int k = 0; k < 2; ++k)
-        for (int b = 0; b < count[k]; ++b) m = fmaxf(m, piece[k][b * step[k] + p.dv]);
-    float total = p.sinks && m != -INFINITY ? expf(p.sinks[head] - m) : 0.f;
-    constexpr int MOST = SR_DIM / SJ_THREADS;
-    float sum[MOST];
-#pragma unroll
-    for (int j = 0; j < MOST; ++j) sum[j] = 0.f;
-    for (int k = 0; k < 2; ++k)
-        for (int b = 0; b < count[k]; ++b) {
-            const float* x = piece[k] + b * step[k];
-            const float pm = x[p.dv];
-            if (pm == -INFINITY) continue;               // a range of which the row sees nothing
-            const float fade = expf(pm - m);
-            total = fmaf(fade, x[p.dv + 1], total);
-#pragma unroll
-            for (int j = 0; j < MOST; ++j)
-                if (tid + j * SJ_THREADS < p.dv) sum[j] = fmaf(fade, x[tid + j * SJ_THREADS], sum[j]);
+    if (row_units > 0) {
+        const long long u = (long long)p.cut[SH_CUT_ROW_UNITS + r] * p.hkv + (long long)kvh * row_units, all = (long long)p.cut[SH_CUT_ROW_UNITS + p.rows] * p.hkv;
+        const int workers = p.cut[SH_CUT_COUNTS + 2], first = shared_worker_of(u, all, workers);
+        count[1] = shared_worker_of(u + row_units - 1, all, workers) - first + 1;
+        piece[1] = p.row_pieces + (shared_row_place(p, r, kvh, first) + head % group) * width;
+    }
+    const int n = count[0] + count[1];
+    auto at = [&](int b) { return b < count[0] ? piece[0] + b * step[0] : piece[1] + (b - count[0]) * step[1]; };
+    const int lanes = (p.dv + 3) / 4, groups = SJ_THREADS / lanes, mine = tid / lanes, c = tid % lanes * 4;
+    const float sink = p.sinks ? p.sinks[head] : -INFINITY;
+    float m = sink, total = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = 0; base < n; base += SJ_PIECES) {    // (one turn but for very many workers)
+        const int here = min(SJ_PIECES, n - base);
+        float most = -INFINITY;
+        for (int b = tid; b < here; b += SJ_THREADS) most = fmaxf(most, at(base + b)[p.dv]);
+        most = fmaxf(block_max(most, scratch), m);
+        const float fade = most == -INFINITY ? 1.f : expf(m - most);
+        m = most;
+        sum.x *= fade; sum.y *= fade; sum.z *= fade; sum.w *= fade;
+        float l = 0.f;
+        for (int b = tid; b < here; b += SJ_THREADS) {
+            const float* x = at(base + b);
+            const float w = x[p.dv] == -INFINITY ? 0.f : expf(x[p.dv] - m);          // a range of which the row sees nothing
+            weight[b] = w;
+            l = w > 0.f ? fmaf(w, x[p.dv + 1], l) : l;
         }
+        total = total * (base ? fade : 0.f) + block_sum(l, scratch);     // its barriers show the weights to all
+        if (mine < groups) {
+#pragma unroll 4
+            for (int b = mine; b < here; b += groups) {
+                const float w = weight[b];
+                if (w == 0.f) continue;
+                const float4 x = *reinterpret_cast<const float4*>(at(base + b) + c);
+                sum.x = fmaf(w, x.x, sum.x);
+                sum.y = fmaf(w, x.y, sum.y);
+                sum.z = fmaf(w, x.z, sum.z);
+                sum.w = fmaf(w, x.w, sum.w);
+            }
+        }
+        __syncthreads();
+    }
+    if (p.sinks && m != -INFINITY) total += expf(sink - m);
+    part[tid] = sum;
+    __syncthreads();
+    if (tid >= lanes) return;
+    for (int k = 1; k < groups; ++k) {
+        const float4 x = part[k * lanes + tid];
+        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+    }
     const float inv = total > 0.f ? 1.f / total : 0.f;
     T* out = static_cast<T*>(p.out) + ((size_t)r * p.hq + head) * p.dv;
+    const float v[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
 #pragma unroll
-    for (int j = 0; j < MOST; ++j)
-        if (tid + j * SJ_THREADS < p.dv) Elem<T>::store(out + tid + j * SJ_THREADS, sum[j] * inv);
+    for (int j = 0; j < 4; ++j)
+        if (c + j < p.dv) Elem<T>::store(out + c + j, v[j]);
 }
 
 template <typename T> static int launch_shared_rows(const SharedParams& p, int blocks, cudaStream_t s) {

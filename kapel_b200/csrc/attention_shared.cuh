@@ -51,6 +51,7 @@ constexpr int SH_CUT_INTS = SH_CUT_COUNTS + 3;
 struct SharedTiles {
     int tiles;
     int row_tile[SH_ROWS];                   // a row's tile, -1 where it shares nothing
+    int length[SH_ROWS], id[SH_ROWS], first[SH_ROWS];    // by row: positions it shares, with whom, the first it sees
     int row0[SH_ROWS], n[SH_ROWS], before[SH_ROWS + 1];      // by tile
     int looks[SH_ROWS];                      // by tile: the row whose block table has the pages
     int klo[SH_ROWS], khi[SH_ROWS];          // by tile: the positions [klo, khi) that any row sees of what they share
@@ -72,13 +73,13 @@ __device__ __forceinline__ int shared_own(const SharedParams& p, int r, int keys
     return lo < hi ? (hi - lo / keys * keys + keys - 1) / keys : 0;
 }
 
-// Running totals over n items, by the block's first warp: upto[i] = what `of` gives for the items before i. No barrier.
-template <typename F> __device__ __forceinline__ void shared_totals(int* upto, int n, F of) {
+// upto[0 .. n] holds n numbers and becomes their running totals (what lies before each, then all), by one warp. No barrier.
+__device__ __forceinline__ void shared_totals(int* upto, int n) {
     const int lane = threadIdx.x & 31;
     int total = 0;
     for (int base = 0; base < n; base += 32) {
         const int i = base + lane;
-        const int mine = i < n ? of(i) : 0;
+        const int mine = i < n ? upto[i] : 0;
         int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -94,15 +95,21 @@ template <typename F> __device__ __forceinline__ void shared_totals(int* upto, i
 // The cut into tiles, by the whole block; `rows_a_tile` requests to a tile, `keys` positions to a unit.
 __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, int rows_a_tile, int keys) {
     const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x;
-    for (int i = tid; i < p.rows; i += nt) { c.klo[i] = 0x7fffffff; c.khi[i] = 0; c.n[i] = 0; c.row0[i] = 0x7fffffff; c.looks[i] = 0x7fffffff; }
+    for (int i = tid; i < p.rows; i += nt) {
+        c.klo[i] = 0x7fffffff; c.khi[i] = 0; c.before[i] = 0; c.row0[i] = 0x7fffffff; c.looks[i] = 0x7fffffff;
+        c.length[i] = shared_length(p, i);               // every load of the cut is asked for here, all rows at once
+        c.id[i] = p.share_id[i];
+        c.first[i] = shared_first(p, p.row_count[i]);
+    }
+    __syncthreads();
     if (tid < 32) {
         // Where each row's run begins, and with it the row's place in the run: rows_a_tile of them to a tile.
         int run = 0, tiles = 0;
         for (int base = 0; base < p.rows; base += 32) {
             const int r = base + lane;
             const bool in = r < p.rows;
-            const int length = in ? shared_length(p, r) : 0;
-            const bool starts = in && (r == 0 || length == 0 || shared_length(p, r - 1) != length || p.share_id[r] != p.share_id[r - 1]);
+            const int length = in ? c.length[r] : 0;
+            const bool starts = in && (r == 0 || length == 0 || c.length[r - 1] != length || c.id[r] != c.id[r - 1]);
             const unsigned who = __ballot_sync(0xffffffffu, starts);
             const unsigned mine = who & (0xffffffffu >> (31 - lane));
             const int begins = mine ? base + 31 - __clz(mine) : run;
@@ -119,28 +126,37 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
         const int t = c.row_tile[r];
         if (t < 0) continue;
         atomicMin(&c.row0[t], r);
-        atomicAdd(&c.n[t], 1);
-        const int length = shared_length(p, r), first = shared_first(p, p.row_count[r]);
-        if (first < length) {                            // else the window has passed what it shares
-            atomicMin(&c.klo[t], first);
-            atomicMax(&c.khi[t], length);
+        atomicAdd(&c.before[t], 1);
+        if (c.first[r] < c.length[r]) {                  // else the window has passed what it shares
+            atomicMin(&c.klo[t], c.first[r]);
+            atomicMax(&c.khi[t], c.length[r]);
         }
     }
     __syncthreads();
     for (int r = tid; r < p.rows; r += nt) {
         const int t = c.row_tile[r];
-        if (t >= 0 && shared_first(p, p.row_count[r]) <= c.klo[t]) atomicMin(&c.looks[t], r);
+        if (t >= 0 && c.first[r] <= c.klo[t]) atomicMin(&c.looks[t], r);
     }
+    for (int i = tid; i < c.tiles; i += nt) {
+        c.n[i] = c.before[i];
+        c.upto[i] = c.klo[i] < c.khi[i] ? (c.khi[i] - c.klo[i] / keys * keys + keys - 1) / keys : 0;
+    }
+    __syncthreads();
     if (tid < 32) {
-        shared_totals(c.before, c.tiles, [&](int i) { return c.n[i]; });
-        shared_totals(c.upto, c.tiles, [&](int i) { return c.klo[i] < c.khi[i] ? (c.khi[i] - c.klo[i] / keys * keys + keys - 1) / keys : 0; });
+        shared_totals(c.before, c.tiles);
+        shared_totals(c.upto, c.tiles);
     }
     __syncthreads();
 }
 
 // The cut into rows: upto[r] = units before row r. By the whole block.
 __device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int keys) {
-    if (threadIdx.x < 32) shared_totals(upto, p.rows, [&](int r) { int lo, hi; return shared_own(p, r, keys, lo, hi); });
+    for (int r = threadIdx.x; r < p.rows; r += blockDim.x) {
+        int lo, hi;
+        upto[r] = shared_own(p, r, keys, lo, hi);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) shared_totals(upto, p.rows);
     __syncthreads();
 }
 

@@ -28,12 +28,18 @@ __device__ __forceinline__ uint32_t sh_transpose(uint32_t a) {           // an 8
 // A product q.k as a score in powers of two: scale, and the soft cap where there is one. tanh x = 1 - 2 / (1 + e^2x): its error is some 1e-7
 // whatever x, which a cap of 50 makes 1e-5 of a score; the hardware's own tanh is off by up to 2^-11 of its value, 0.01 of a score of 20.
 struct SharedScore {
-    float in, out;
+    float in, out, u;
     bool cap;
     __device__ __forceinline__ SharedScore(float scale, float c) {
         cap = c > 0.f;
         in = cap ? scale / c * 2.885390081777927f : scale * 1.4426950408889634f;
         out = c * 1.4426950408889634f;
+        u = cap ? scale / c : 0.f;
+    }
+    __device__ __forceinline__ float of_u(float x) const {   // the same of a product already divided by the cap
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + at_exp2(x * 2.885390081777927f)));
+        return fmaf(-2.f * out, r, out);
     }
     __device__ __forceinline__ float operator()(float x) const {
         if (!cap) return x * in;
@@ -44,6 +50,64 @@ struct SharedScore {
 };
 
 int shared_own_workers(int d);                               // warps a block
+// Two 32-bit values at a time.
+__device__ __forceinline__ unsigned long long sh_pair(uint32_t a, uint32_t b) {
+    unsigned long long d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ unsigned long long sh_pair(float a, float b) { return sh_pair(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void sh_split(unsigned long long x, uint32_t& a, uint32_t& b) { asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(x)); }
+__device__ __forceinline__ unsigned long long sh_mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ unsigned long long sh_add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ unsigned long long sh_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// Scores of a thread's N products in place, none of them masked, and their largest. Without a cap x scale; with one, where every product of the warp is
+// below 3/4 of it, cap tanh(x) by an odd polynomial of degree 9 fitted to tanh x / x on [0, 9/16] of x^2 (6e-7 of the value), two
+// values an instruction: the hardware's exponential, reciprocal and exponential again for each score are three of sixteen a clock and bound the
+// kernel; this leaves one.
+template <int N> __device__ __forceinline__ float sh_scores(uint32_t (&x)[N], const SharedScore& score) {
+    const float first = score.cap ? score.u : score.in;
+    const unsigned long long in = sh_pair(first, first);
+    float top = -INFINITY, far = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        sh_split(sh_mul2(sh_pair(x[j], x[j + 1]), in), x[j], x[j + 1]);
+        top = fmaxf(fmaxf(top, __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
+    }
+    if (!score.cap) return top;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) far = fmaxf(fmaxf(far, fabsf(__uint_as_float(x[j]))), fabsf(__uint_as_float(x[j + 1])));
+    // (a NaN is passed over by fmaxf and goes through the polynomial as well as through the other)
+    if (!__all_sync(0xffffffffu, far <= 0.75f)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = __float_as_uint(score.of_u(__uint_as_float(x[j])));
+        return score.of_u(top);
+    }
+    constexpr float C0 = 0.999999463558197f, C1 = -0.3332834839820862f, C2 = 0.13259831070899963f, C3 = -0.05008019134402275f, C4 = 0.012950727716088295f;
+    const float o = score.out;
+    const unsigned long long c0 = sh_pair(C0 * o, C0 * o), c1 = sh_pair(C1 * o, C1 * o), c2 = sh_pair(C2 * o, C2 * o), c3 = sh_pair(C3 * o, C3 * o), c4 = sh_pair(C4 * o, C4 * o);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const unsigned long long u = sh_pair(x[j], x[j + 1]), z = sh_mul2(u, u);
+        sh_split(sh_mul2(u, sh_fma2(sh_fma2(sh_fma2(sh_fma2(c4, z, c3), z, c2), z, c1), z, c0)), x[j], x[j + 1]);
+    }
+    const float z = top * top;
+    return top * fmaf(fmaf(fmaf(fmaf(C4 * o, z, C3 * o), z, C2 * o), z, C1 * o), z, C0 * o);
+}
+
 int launch_shared_tiles(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s);
 int launch_shared_own(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s);
 

@@ -242,17 +242,21 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
 #pragma unroll
                     for (int k = 0; k < HALF / 32; ++k) at_ld32(lanes + (uint32_t)(C::COL_S + b * KEYS + half * HALF + k * 32), x[k]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    const bool edge = j0 < lo_max || j0 + HALF > hi_min;          // the same for the whole warp
                     float top = -INFINITY;
+                    if (j0 < lo_max || j0 + HALF > hi_min) {     // some pair does not see all of it: the same for the whole warp
 #pragma unroll
-                    for (int k = 0; k < HALF / 32; ++k)
+                        for (int k = 0; k < HALF / 32; ++k)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float v = score(__uint_as_float(x[k][j]));
-                            if (edge && (j0 + k * 32 + j < lo || j0 + k * 32 + j >= hi)) v = -INFINITY;
-                            x[k][j] = __float_as_uint(v);
-                            top = fmaxf(top, v);
-                        }
+                            for (int j = 0; j < 32; ++j) {
+                                float v = score(__uint_as_float(x[k][j]));
+                                if (j0 + k * 32 + j < lo || j0 + k * 32 + j >= hi) v = -INFINITY;
+                                x[k][j] = __float_as_uint(v);
+                                top = fmaxf(top, v);
+                            }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < HALF / 32; ++k) top = fmaxf(top, sh_scores(x[k], score));
+                    }
                     // The quarter's two warps tell each other their halves' maxima; behind this barrier both have their scores in registers,
                     // so P may be written over them. Two sets of places in turn.
                     float* turn = exchange + (c & 1) * 2 * ST_PAIRS;
@@ -280,18 +284,22 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
                     const float base = ref == -INFINITY ? 0.f : ref;
-                    float la = 0.f, lb = 0.f;
+                    const unsigned long long less = sh_pair(-base, -base);
+                    unsigned long long sums = 0ull;
                     uint32_t pr[HALF / 2];
 #pragma unroll
                     for (int k = 0; k < HALF / 32; ++k)
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            const uint32_t two = at_pack(at_exp2(__uint_as_float(x[k][j]) - base), at_exp2(__uint_as_float(x[k][j + 1]) - base));
-                            la += __uint_as_float(two << 16);
-                            lb += __uint_as_float(two & 0xffff0000u);
+                            uint32_t a, c2;
+                            sh_split(sh_add2(sh_pair(x[k][j], x[k][j + 1]), less), a, c2);
+                            const uint32_t two = at_pack(at_exp2(__uint_as_float(a)), at_exp2(__uint_as_float(c2)));
+                            sums = sh_add2(sums, sh_pair(two << 16, two & 0xffff0000u));
                             pr[k * 16 + (j >> 1)] = two;
                         }
-                    l += la + lb;
+                    uint32_t la, lb;
+                    sh_split(sums, la, lb);
+                    l += __uint_as_float(la) + __uint_as_float(lb);
                     if constexpr (HALF == 64) at_st32(lanes + (uint32_t)(C::COL_S + b * KEYS + half * 32), pr);
                     else at_st16(lanes + (uint32_t)(C::COL_S + b * KEYS + half * 16), pr);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

@@ -5,11 +5,47 @@
 // unless every value is one; a draw is the first index whose running total of probabilities
 // exceeds u, and the last possible index if rounding left u above the total. Softmax in 32-bit
 // here (the host sampler of the engine does it in 64-bit).
-#include "sampling.cuh"
+#include "common.cuh"
 
 namespace kb {
 
 constexpr int SMP_THREADS = 1024;
+
+struct Best { float v; int i; };
+
+__device__ __forceinline__ Best better(Best a, Best b) {
+    // larger value wins; on a tie the smaller index; index -1 means "none yet"
+    if (b.i < 0) return a;
+    if (a.i < 0) return b;
+    if (b.v > a.v || (b.v == a.v && b.i < a.i)) return b;
+    return a;
+}
+
+__device__ Best block_best(Best x, Best* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Best y;
+        y.v = __shfl_xor_sync(0xffffffffu, x.v, o);
+        y.i = __shfl_xor_sync(0xffffffffu, x.i, o);
+        x = better(x, y);
+    }
+    __syncthreads();
+    if (lane == 0) scratch[warp] = x;
+    __syncthreads();
+    const int nwarps = (blockDim.x + 31) >> 5;
+    Best t;
+    t.v = 0.f; t.i = -1;
+    if (lane < nwarps) t = scratch[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Best y;
+        y.v = __shfl_xor_sync(0xffffffffu, t.v, o);
+        y.i = __shfl_xor_sync(0xffffffffu, t.i, o);
+        t = better(t, y);
+    }
+    return t;
+}
 
 // One block a row. temperature[r] <= 0 (or temperature == null): argmax.
 __global__ void __launch_bounds__(SMP_THREADS)

@@ -8,24 +8,35 @@
 //
 // A row is one cluster's: its blocks read the row once and keep their shares in shared memory; everything after works on chip.
 //   1. The largest logit, whether a NaN is there.
-//   2. For top_k or top_p a histogram over 2,048 bins of equal steps of x below the largest: counts, and for top_p the sums of e^(x - max)
-//      in fixed point (44 bits behind the point: whole numbers, so the order of the atomics changes nothing; a row's sum, 2^18
-//      tokens, fits 64 bits). The bins are added up in the cluster's first block, which finds the bin the cut falls in.
-//   3. Where the bins down to there hold no more than LIST tokens (a top_k, a peaked nucleus), they are gathered in the first block,
-//      sorted, cut and drawn from there. Otherwise only the bin of the cut is gathered and sorted to find the cut (a bin too full
-//      for that is divided again between its smallest and largest key), and the draw goes over the whole share of every block.
+//   2. For a top_k up to LIST / 2: as many of the threads' own largest logits lie above the cut's lower bound that a histogram of those few
+//      finds; what lies above it is gathered in the cluster's first block, sorted, cut and drawn from there. (Sorted logits may leave more
+//      than LIST above it: then as below.)
+//   3. Else a histogram of counts over 2,048 bins of equal steps of x below the largest. top_k: the bin in which the k-th lies. top_p: a
+//      bin's weight lies between its count times the weights at its ends, so the histogram bounds where the cut is to a few bins; what is
+//      above those is added up exactly (in fixed point, 44 bits behind the point: whole numbers, whose order changes nothing; a row's
+//      sum, 2^19 tokens, fits 64 bits). The bins in question, or all down to them where they hold no more than LIST tokens, are gathered and
+//      sorted for the exact cut; bins too full for that are divided again between their smallest and largest key. (Weights
+//      added up by atomics instead took 1.1 ms a row of 256,000: shared memory has none of 64 bits.)
+//   4. The draw goes over the whole share of every block: totals of warps, of the 32 rows of the warp's that the target falls in,
+//      then along that row.
 // e^x is in 64 bits, and so are the draw's sums, as on the host: a seed gives the tokens it gave there, but for borders that lie within a
-// few units of the 13th digit.
+// few units of the 13th digit. It is made of 2^(n / 32) = 2^k T[n mod 32], n an integer within a roundoff of the nearest to 32 x / ln 2 (found in 32 bits), and a
+// polynomial of degree 5 for what is left (the series' next term is below 3e-15): nine 64-bit operations, of which a multiprocessor does some 37 a
+// clock. Two entries of T share a bank, so a warp's loads take two turns at most.
 #include <cooperative_groups.h>
-#include "sampling.cuh"
+#include <cfloat>
+#include "common.cuh"
 
 namespace kb {
 namespace cg = cooperative_groups;
 
 constexpr int SF_THREADS = 1024, SF_WARPS = SF_THREADS / 32;
 constexpr int SF_BINS = 2048, SF_LIST = 2048, SF_MAX_CLUSTER = 8;
+constexpr int SF_SMALL = 256;                            // lists up to here are ordered by counting
+constexpr int SF_ROWS = 64;                              // rows of 32 columns a warp has at most: a share of 2^16, a vocabulary of 2^19 over eight blocks
 constexpr float SF_SPAN = 24.f;                          // the bins reach e^-24 below the largest; the last holds all that is below
 constexpr double SF_FIXED = 17592186044416.0;            // 2^44
+constexpr double SF_STEP = 0.6931471805599453 / 32.0;    // ln 2 / 32
 
 struct SfParams {
     int* tokens;
@@ -40,31 +51,31 @@ struct SfParams {
     int cached;                                          // of them in shared memory; the rest is read again from the row
 };
 
-struct SfTop { Best best; int nan; int unused; };
+struct SfTop { float v; int nan; };
 struct SfCut { unsigned key; int index; };               // what is left: key above, or equal and the index no larger
 struct SfFound {                                         // what the first block tells the others about a histogram
-    int bin, in_bin;                                     // the cut's bin and how many tokens it holds
-    unsigned upto;                                       // tokens in the bins down to and with it
-    unsigned above;                                      // tokens above it
-    unsigned long long weight_above, weight_all;
+    int from, to;                                        // the bins the cut may be in
+    unsigned above, upto;                                // tokens above them, and down to their end
 };
 
 struct SfShared {
+    double powers[32];                                   // 2^(j / 32)
     unsigned counts[SF_BINS];
-    unsigned long long weights[SF_BINS];
     unsigned long long list[SF_LIST];                    // first block: key << 32 | ~index, the largest first once sorted
     SfTop tops[SF_MAX_CLUSTER];
     double sums[SF_MAX_CLUSTER];
-    double warp_sum[SF_WARPS];
-    unsigned long long warp_fixed[SF_WARPS];
+    unsigned long long fixed_sums[SF_MAX_CLUSTER][2];
+    double warp_sum[SF_WARPS], warp_sum2[SF_WARPS];
+    double row_sum[SF_ROWS];
+    unsigned long long warp_fixed[SF_WARPS], warp_fixed2[SF_WARPS];
     unsigned warp_count[SF_WARPS];
+    float warp_max[SF_WARPS];
     SfFound found;
     SfCut cut;
-    unsigned lo_key, hi_key;                             // the smallest and largest key of a bin
+    unsigned lo_key, hi_key;                             // the smallest and largest key of some bins
     int listed;
-    int owner;
+    int owner, owner2;
     int kept;
-    Best best[32];
 };
 
 // Keys that order as the values do; both zeros are one.
@@ -79,16 +90,55 @@ __device__ __forceinline__ float sf_value(unsigned key) {
 struct SfRow {
     const float* row;                                    // this block's share begins here
     const float* cache;
+    const double* powers;
     int n, cached, first;                                // columns of the share, how many are in `cache`, the share's first column
-    double inv;                                          // 1 / temperature
-    float largest;
+    double inv, steps;                                   // 1 / temperature, and in steps of ln 2 / 32
+    float largest, steps32, lowest;                      // below `lowest` a weight is under e^-690: none
     __device__ __forceinline__ float at(int i) const { return i < cached ? cache[i] : row[i]; }
-    __device__ __forceinline__ double weight(float v) const { return exp(((double)v - (double)largest) * inv); }
+    __device__ __forceinline__ void scale(float top, double temperature, const double* table) {
+        largest = top;
+        inv = isinf(temperature) ? 0.0 : fmin(1.0 / temperature, 1e300);
+        steps = inv / SF_STEP;
+        steps32 = (float)fmin(steps, 1e38);
+        lowest = (float)fmax((double)top - 690.0 / inv, (double)-FLT_MAX);
+        powers = table;
+    }
+    // e^((v - largest) / temperature), which is at most 1
+    __device__ __forceinline__ double weight(float v) const {
+        if (v < lowest) return 0.0;
+        const float magic32 = 12582912.f;                // 1.5 2^23: a sum's last bits are the nearest integer
+        const int n = __float_as_int(fmaf(v - largest, steps32, magic32)) - __float_as_int(magic32);
+        const double x = fma((double)v - (double)largest, steps, 6755399441055744.0 - __hiloint2double(0x43380000 + (n >> 31), n));      // half a step, and what 32 bits round
+        constexpr double A = SF_STEP, A2 = A * A / 2, A3 = A2 * A / 3, A4 = A3 * A / 4, A5 = A4 * A / 5;
+        const double e = powers[n & 31] * fma(x, fma(x, fma(x, fma(x, fma(x, A5, A4), A3), A2), A), 1.0);
+        return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
+    }
+    // Calls f(column, value) for the block's columns whose value is `floor` or more, a thread every SF_THREADS-th.
+    template <typename F> __device__ __forceinline__ void each(float floor, F f) const {
+        constexpr int DEEP = 8;
+        if (cached == n) {
+            for (int base = threadIdx.x; base < n; base += DEEP * SF_THREADS) {
+                float v[DEEP];
+#pragma unroll
+                for (int k = 0; k < DEEP; ++k) v[k] = base + k * SF_THREADS < n ? cache[base + k * SF_THREADS] : -INFINITY;
+#pragma unroll
+                for (int k = 0; k < DEEP; ++k)
+                    if (v[k] >= floor) f(base + k * SF_THREADS, v[k]);
+            }
+        } else {
+            for (int i = threadIdx.x; i < n; i += SF_THREADS) {
+                const float v = at(i);
+                if (v >= floor) f(i, v);
+            }
+        }
+    }
 };
+constexpr float SF_LOWEST = -FLT_MAX;                    // the floor of all that is possible
 
 __device__ __forceinline__ bool sf_left(const SfCut& cut, unsigned key, int index) {
     return key > cut.key || (key == cut.key && index <= cut.index);
 }
+__device__ __forceinline__ float sf_floor(const SfCut& cut) { return cut.key == 0u ? SF_LOWEST : fmaxf(SF_LOWEST, sf_value(cut.key)); }
 
 // A level's bins: equal steps below the largest at first, then equal steps of the key between two keys.
 struct SfBins {
@@ -97,141 +147,201 @@ struct SfBins {
     unsigned lo, hi;                                     // keys that count; bin = (hi - key) >> shift
     int shift;
     __device__ __forceinline__ int of(float v, unsigned key) const {
-        if (key < lo || key > hi) return -1;
-        if (by_key) return (int)((hi - key) >> shift);
+        if (by_key) return key < lo || key > hi ? -1 : (int)((hi - key) >> shift);
         const float x = (largest - v) * step;
         return x < (float)(SF_BINS - 1) ? (int)x : (x == x ? SF_BINS - 1 : 0);
     }
+    // No value below this is in the bins down to b.
+    __device__ __forceinline__ float floor(int b) const {
+        if (b >= SF_BINS - 1) return SF_LOWEST;
+        if (by_key) {
+            const unsigned span = (((unsigned)b + 1u) << shift) - 1u;
+            return fmaxf(SF_LOWEST, sf_value(hi - lo < span ? lo : hi - span));
+        }
+        const float reach = (float)(b + 1) / step;       // infinite where the steps are nothing
+        return fmaxf(SF_LOWEST, largest - reach * 1.00001f - fabsf(largest) * 1e-6f);
+    }
+    // Bounds of a token's weight in bin b (32-bit steps: an edge may lie a few roundings off).
+    __device__ __forceinline__ void bounds(const SfRow& r, int b, double& least, double& most) const {
+        if (by_key) {
+            const unsigned top = hi - ((unsigned)b << shift), span = (1u << shift) - 1u;
+            most = r.weight(sf_value(top));
+            least = r.weight(sf_value(top - lo < span ? lo : top - span));
+        } else {
+            const bool plain = step > 0.f && step < 1e30f;
+            const double wide = 1.0 / ((double)step * (1.0 - 1e-6)), narrow = 1.0 / ((double)step * (1.0 + 1e-6));
+            most = b == 0 || !plain ? 1.0 : exp(-(double)b * narrow * r.inv);
+            least = b == SF_BINS - 1 || !plain ? 0.0 : exp(-(double)(b + 1) * wide * r.inv);
+        }
+    }
 };
 
-// Sorts list[0 .. n), largest first; n up to SF_LIST, padded with zeros to a power of two.
-__device__ void sf_sort(unsigned long long* list, int n) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = threadIdx.x; i < size; i += SF_THREADS)
-        if (i >= n) list[i] = 0ull;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int t = threadIdx.x; t < size / 2; t += SF_THREADS) {
-                const int i = (t / j) * 2 * j + t % j;
-                const unsigned long long a = list[i], b = list[i + j];
-                if (((i & k) == 0) ? a < b : a > b) { list[i] = b; list[i + j] = a; }
-            }
-            __syncthreads();
-        }
+// e in fixed point: 2^52 added, the sum's last bits are the whole number.
+__device__ __forceinline__ unsigned long long sf_fixed(double e) {
+    return (unsigned long long)__double_as_longlong(fma(e, SF_FIXED, 4503599627370496.0)) & 0xfffffffffffffull;
 }
-
 // run >= top_p all, the product not rounded before it is compared: equal weights reach a round share of the whole exactly.
 __device__ __forceinline__ bool sf_reached(unsigned long long run, double top_p, unsigned long long all) {
     return fma(top_p, (double)all, -(double)run) <= 0.0;
 }
-__device__ __forceinline__ unsigned long long sf_fixed(double e) { return (unsigned long long)(e * SF_FIXED + 0.5); }
 
-// The bins' histogram over what is left, added up in the first block; there the bin of the cut is found: the first in which the count
-// down to it reaches `want`, or, by weight, in which the weight down to it reaches top_p of the whole. `base` (count, weight) lies above
-// the level's keys. Every block leaves with the answer in `found`.
-__device__ void sf_histogram(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, const SfCut& cut, bool by_weight,
-                             unsigned want, double top_p, unsigned base_count, unsigned long long base_weight, unsigned long long all_weight) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int i = tid; i < SF_BINS; i += SF_THREADS) { s.counts[i] = 0u; s.weights[i] = 0ull; }
-    __syncthreads();
-    for (int i = tid; i < r.n; i += SF_THREADS) {
-        const float v = r.at(i);
-        if (!(v > -INFINITY)) continue;
-        const unsigned key = sf_key(v);
-        if (!sf_left(cut, key, r.first + i)) continue;
-        const int b = bins.of(v, key);
-        if (b < 0) continue;
-        atomicAdd(&s.counts[b], 1u);
-        if (by_weight) atomicAdd(&s.weights[b], sf_fixed(r.weight(v)));
+// Inclusive running totals over the block's first `warps` warps (the others have nothing), in thread order.
+template <typename V> __device__ __forceinline__ V sf_warp_scan(V v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
     }
+    return v;
+}
+template <typename V> __device__ __forceinline__ V sf_scan(V v, V* per_warp, V* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    v = sf_warp_scan(v);
+    __syncthreads();
+    if (lane == 31) per_warp[warp] = v;
+    __syncthreads();
+    const V sums = sf_warp_scan(per_warp[lane]);
+    *total = __shfl_sync(0xffffffffu, sums, 31);
+    const V before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+    return warp ? before + v : v;
+}
+
+// Sorts list[0 .. n), largest first; n up to SF_LIST. A few entries go to where as many are larger; more by exchanges, those
+// within 64 neighbours by one warp each.
+__device__ void sf_sort(unsigned long long* list, int n) {
+    __syncthreads();
+    if (n <= SF_SMALL) {
+        // four threads an entry, a quarter of the others each
+        const int i = threadIdx.x >> 2;
+        const unsigned long long mine = i < n ? list[i] : 0ull;
+        int rank = 0;
+        if (i < n)
+            for (int j = threadIdx.x & 3; j < n; j += 4) rank += list[j] > mine ? 1 : 0;
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        __syncthreads();
+        if (i < n && (threadIdx.x & 3) == 0) list[rank] = mine;          // entries differ: their indices do
+        __syncthreads();
+        return;
+    }
+    int size = 512;
+    while (size < n) size <<= 1;
+    for (int i = threadIdx.x; i < size; i += SF_THREADS)
+        if (i >= n) list[i] = 0ull;
+    __syncthreads();
+    const int t = threadIdx.x;
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            if (t < size / 2) {
+                const int i = (t / j) * 2 * j + t % j;
+                const unsigned long long a = list[i], b = list[i + j];
+                if (((i & k) == 0) ? a < b : a > b) { list[i] = b; list[i + j] = a; }
+            }
+            // the next exchange's neighbours are this warp's own 64 where it and this one reach no farther than 32
+            const int next = j > 1 ? j >> 1 : k;
+            if (j > 32 || next > 32) __syncthreads(); else __syncwarp();
+        }
+    __syncthreads();
+}
+
+__device__ __forceinline__ void sf_clear(SfShared& s) {
+    for (int i = threadIdx.x; i < SF_BINS; i += SF_THREADS) s.counts[i] = 0u;
+    __syncthreads();
+}
+
+// The counts of every block added up in the first, and there the bins in which the cut may be: by count (`want` > 0) the one in which it reaches
+// `want`; by weight from the first in which it may reach top_p of `all` to the first in which it does. `above` and `weight_above` lie above the
+// level's keys. Where nothing reaches it (fewer tokens, or rounding) the last bin that holds a token. Every block leaves with `found`.
+__device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, unsigned want, double top_p, unsigned above,
+                        unsigned long long weight_above, unsigned long long all) {
+    const int tid = threadIdx.x;
+    if (cluster.block_rank() == 0 && tid == 0) { s.owner = SF_BINS; s.owner2 = SF_BINS; s.kept = -1; }
     cluster.sync();
-    SfShared* home = cluster.map_shared_rank(&s, 0);
     if (cluster.block_rank() != 0) {
+        SfShared* home = cluster.map_shared_rank(&s, 0);
         for (int i = tid; i < SF_BINS; i += SF_THREADS) {
             const unsigned c = s.counts[i];
-            if (c == 0u) continue;
-            atomicAdd(&home->counts[i], c);
-            if (by_weight) atomicAdd(&home->weights[i], s.weights[i]);
+            if (c != 0u) atomicAdd(&home->counts[i], c);
         }
     }
     cluster.sync();
     if (cluster.block_rank() == 0) {
         constexpr int EACH = SF_BINS / SF_THREADS;
-        unsigned c[EACH], count = 0;
-        unsigned long long w[EACH], weight = 0;
+        const bool by_weight = want == 0u;
+        unsigned c[EACH], count = 0, total_c;
+        double least[EACH], most[EACH], lower = 0.0, upper = 0.0, unused;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             c[j] = s.counts[tid * EACH + j];
-            w[j] = by_weight ? s.weights[tid * EACH + j] : 0ull;
             count += c[j];
-            weight += w[j];
+            least[j] = most[j] = 0.0;
+            if (by_weight && c[j]) {
+                bins.bounds(r, tid * EACH + j, least[j], most[j]);
+                least[j] = fmax(least[j] * c[j] * (1.0 - 1e-9) * SF_FIXED - 0.5 * c[j], 0.0);            // each rounded to a whole number
+                most[j] = most[j] * c[j] * (1.0 + 1e-9) * SF_FIXED + 0.5 * c[j];
+            }
+            lower += least[j];
+            upper += most[j];
         }
-        unsigned upto_c = count;
-        unsigned long long upto_w = weight;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned yc = __shfl_up_sync(0xffffffffu, upto_c, o);
-            const unsigned long long yw = __shfl_up_sync(0xffffffffu, upto_w, o);
-            if (lane >= o) { upto_c += yc; upto_w += yw; }
+        unsigned run_c = above + sf_scan(count, s.warp_count, &total_c) - count;
+        double run_l = 0.0, run_u = 0.0;
+        if (by_weight) {
+            run_l = (double)weight_above + sf_scan(lower, s.warp_sum, &unused) - lower;
+            run_u = (double)weight_above + sf_scan(upper, s.warp_sum2, &unused) - upper;
         }
-        if (lane == 31) { s.warp_count[warp] = upto_c; s.warp_fixed[warp] = upto_w; }
-        if (tid == 0) s.owner = SF_BINS;
-        __syncthreads();
-        unsigned long long all = base_weight;
-        unsigned before_c = base_count;
-        unsigned long long before_w = base_weight;
-        for (int k = 0; k < SF_WARPS; ++k) {
-            if (k < warp) { before_c += s.warp_count[k]; before_w += s.warp_fixed[k]; }
-            all += s.warp_fixed[k];
-        }
-        if (all_weight) all = all_weight;                // a deeper level: the whole is the first level's
-        before_c += upto_c - count;
-        before_w += upto_w - weight;
-        int mine = -1;
-        unsigned above = before_c;
-        unsigned long long above_w = before_w;
-        unsigned run_c = before_c;
-        unsigned long long run_w = before_w;
+        const double target = top_p * (double)all;
+        unsigned at[EACH];                               // tokens above each bin
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            const unsigned next_c = run_c + c[j];
-            const unsigned long long next_w = run_w + w[j];
-            if (mine < 0 && c[j] && (by_weight ? sf_reached(next_w, top_p, all) : next_c >= want)) { mine = tid * EACH + j; above = run_c; above_w = run_w; }
-            run_c = next_c;
-            run_w = next_w;
-        }
-        if (mine >= 0) atomicMin(&s.owner, mine);
-        __syncthreads();
-        // No bin reaches it (fewer tokens than `want`, or rounding): the last bin that holds a token.
-        const bool none = s.owner == SF_BINS;
-        __syncthreads();
-        if (none) {
-            int last = -1;
-            run_c = before_c; run_w = before_w;
-#pragma unroll
-            for (int j = 0; j < EACH; ++j) {
-                if (c[j]) { last = tid * EACH + j; above = run_c; above_w = run_w; }
-                run_c += c[j];
-                run_w += w[j];
+            at[j] = run_c;
+            run_c += c[j];
+            run_l += least[j];
+            run_u += most[j];
+            if (c[j]) {
+                const int b = tid * EACH + j;
+                atomicMax(&s.kept, b);
+                if (by_weight ? run_u * (1.0 + 1e-12) >= target : run_c >= want) atomicMin(&s.owner, b);
+                if (by_weight ? run_l * (1.0 - 1e-12) >= target : run_c >= want) atomicMin(&s.owner2, b);
             }
-            mine = last;
-            if (tid == 0) s.owner = -1;
-            __syncthreads();
-            if (last >= 0) atomicMax(&s.owner, last);
-            __syncthreads();
         }
-        if (mine >= 0 && mine == s.owner) {
-            unsigned in = 0;
+        __syncthreads();
+        const int last = s.kept, from = min(s.owner, last), to = min(s.owner2, last);
 #pragma unroll
-            for (int j = 0; j < EACH; ++j) if (tid * EACH + j == mine) in = c[j];
-            SfFound f;
-            f.bin = mine; f.in_bin = (int)in; f.above = above; f.upto = above + in; f.weight_above = above_w; f.weight_all = all;
-            for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->found = f;
+        for (int j = 0; j < EACH; ++j) {
+            const int b = tid * EACH + j;
+            if (b != from && b != to) continue;
+            for (unsigned k = 0; k < cluster.num_blocks(); ++k) {
+                SfFound* f = &cluster.map_shared_rank(&s, k)->found;
+                if (b == from) { f->from = from; f->to = to; f->above = at[j]; }
+                if (b == to) f->upto = at[j] + c[j];
+            }
         }
     }
     cluster.sync();
+}
+
+// Two sums over the whole row of what each thread brings, in fixed point.
+__device__ void sf_sum(cg::cluster_group& cluster, SfShared& s, unsigned long long& a, unsigned long long& b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+    if (lane == 0) { s.warp_fixed[warp] = a; s.warp_fixed2[warp] = b; }
+    __syncthreads();
+    if (warp == 0) {
+        a = s.warp_fixed[lane];
+        b = s.warp_fixed2[lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+        if (lane < (int)cluster.num_blocks()) {
+            unsigned long long* there = cluster.map_shared_rank(&s, lane)->fixed_sums[cluster.block_rank()];
+            there[0] = a;
+            there[1] = b;
+        }
+    }
+    cluster.sync();
+    a = b = 0;
+    for (unsigned k = 0; k < cluster.num_blocks(); ++k) { a += s.fixed_sums[k][0]; b += s.fixed_sums[k][1]; }
 }
 
 // What is left in the bins from `from` to `to` into the first block's list.
@@ -239,46 +349,42 @@ __device__ void sf_gather(cg::cluster_group& cluster, SfShared& s, const SfRow& 
     SfShared* home = cluster.map_shared_rank(&s, 0);
     if (cluster.block_rank() == 0 && threadIdx.x == 0) s.listed = 0;
     cluster.sync();
-    const int lane = threadIdx.x & 31;
-    for (int base = 0; base < r.n; base += SF_THREADS) {
-        const int i = base + (int)threadIdx.x;
-        bool in = false;
-        unsigned key = 0;
-        if (i < r.n) {
-            const float v = r.at(i);
-            if (v > -INFINITY) {
-                key = sf_key(v);
-                const int b = sf_left(cut, key, r.first + i) ? bins.of(v, key) : -1;
-                in = b >= from && b <= to;
-            }
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, in);
-        if (who == 0u) continue;
-        int at = 0;
-        if (lane == __ffs(who) - 1) at = atomicAdd(&home->listed, __popc(who));
-        at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1u));
-        if (in && at < SF_LIST) home->list[at] = ((unsigned long long)key << 32) | (unsigned)~(r.first + i);
-    }
+    r.each(fmaxf(sf_floor(cut), bins.floor(to)), [&](int i, float v) {
+        const unsigned key = sf_key(v);
+        if (!sf_left(cut, key, r.first + i)) return;
+        const int b = bins.of(v, key);
+        if (b < from || b > to) return;
+        const int at = atomicAdd(&home->listed, 1);
+        if (at < SF_LIST) home->list[at] = ((unsigned long long)key << 32) | (unsigned)~(r.first + i);
+    });
     cluster.sync();
 }
 
-// The first index, over the whole row in order, whose running total of `weight_of` exceeds the target that `target_of` makes of
-// the whole; the last index with a weight where rounding leaves the target at or above it. -1 in every block but the one that has it.
+// The first index, over the whole row in order, whose running total of `weight_of(column, value)` (nothing below `floor`) exceeds the target that
+// `target_of` makes of the whole; the last index with a weight where rounding leaves the target at or above it. -1 in every thread but one of
+// the block that has it.
 template <typename W, typename T>
-__device__ int sf_locate(cg::cluster_group& cluster, SfShared& s, const SfRow& r, W weight_of, T target_of) {
+__device__ int sf_locate(cg::cluster_group& cluster, SfShared& s, const SfRow& r, float floor, W weight_of, T target_of) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = ((r.n + SF_WARPS - 1) / SF_WARPS + 31) / 32 * 32;      // a warp's columns lie together: totals follow their order
     const int begin = min(r.n, warp * each), end = min(r.n, begin + each);
     double local = 0.0;
-    for (int i = begin + lane; i < end; i += 32) local += weight_of(i);
+    constexpr int DEEP = 8;
+    for (int base = begin + lane; base < end; base += 32 * DEEP) {
+        float v[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) v[k] = base + 32 * k < end ? r.at(base + 32 * k) : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k)
+            if (v[k] >= floor) local += weight_of(base + 32 * k, v[k]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) local += __shfl_xor_sync(0xffffffffu, local, o);
     if (lane == 0) s.warp_sum[warp] = local;
     __syncthreads();
-    if (tid == 0) {
-        double mine = 0.0;
-        for (int w = 0; w < SF_WARPS; ++w) mine += s.warp_sum[w];
-        for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->sums[cluster.block_rank()] = mine;
+    if (warp == 0) {
+        const double mine = __shfl_sync(0xffffffffu, sf_warp_scan(s.warp_sum[lane]), 31);
+        if (lane < (int)cluster.num_blocks()) cluster.map_shared_rank(&s, lane)->sums[cluster.block_rank()] = mine;
     }
     cluster.sync();
     double total = 0.0;
@@ -294,61 +400,41 @@ __device__ int sf_locate(cg::cluster_group& cluster, SfShared& s, const SfRow& r
     }
     const bool beyond = owner < 0;
     if (beyond) owner = last;
-    int pick = -1;
-    if (owner == (int)cluster.block_rank()) {
-        int mine = -1, last_warp = -1;
-        double warp_before = 0.0;
-        run = before;
-        for (int w = 0; w < SF_WARPS; ++w) {
-            const double next = run + s.warp_sum[w];
-            if (s.warp_sum[w] > 0.0) { last_warp = w; if (mine < 0 && !beyond && target < next) { mine = w; warp_before = run; } }
-            run = next;
-        }
-        bool to_end = beyond || mine < 0;                // the crossing hid in rounding: the last possible token
-        if (to_end) mine = last_warp;
-        if (warp == mine) {
-            run = warp_before;
-            int seen = -1;
-            for (int base = begin; base < end && pick < 0; base += 32) {
-                const int i = base + lane;
-                const double e = i < end ? weight_of(i) : 0.0;
-                double upto = e;
+    if (owner != (int)cluster.block_rank()) return -1;
+    // The first of the warps' ranges that holds the target; where rounding hid it, the last that holds anything.
+    const double sum = s.warp_sum[lane], after = before + sf_warp_scan(sum);
+    const unsigned some_warps = __ballot_sync(0xffffffffu, sum > 0.0), holds = __ballot_sync(0xffffffffu, sum > 0.0 && !beyond && target < after);
+    bool to_end = holds == 0u;
+    const int mine = to_end ? 31 - __clz(some_warps) : __ffs(holds) - 1;
+    double upto_warp = __shfl_sync(0xffffffffu, after, (mine + 31) & 31);
+    if (mine == 0) upto_warp = before;
+    // Its rows of 32 columns, dealt out to all warps: their sums, then along the row that holds the target.
+    const int from = min(r.n, mine * each), rows = (min(r.n, from + each) - from + 31) / 32;
+    auto of = [&](int i) -> double {
+        if (i >= r.n || i >= from + each) return 0.0;
+        const float v = r.at(i);
+        return v >= floor ? weight_of(i, v) : 0.0;
+    };
+    for (int k = warp; k < SF_ROWS; k += SF_WARPS) {
+        double e = k < rows ? of(from + k * 32 + lane) : 0.0;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += y;
-                }
-                const unsigned some = __ballot_sync(0xffffffffu, e > 0.0);
-                const unsigned passed = __ballot_sync(0xffffffffu, e > 0.0 && !to_end && target < run + upto);
-                if (some) seen = base + 31 - __clz(some);
-                if (passed) pick = base + __ffs(passed) - 1;
-                run += __shfl_sync(0xffffffffu, upto, 31);
-            }
-            if (pick < 0) pick = seen;
-            if (lane != 0) pick = -1;
-        }
-    }
-    return pick;
-}
-
-// Inclusive running totals over the block, in thread order.
-template <typename V> __device__ V sf_scan(V v, V* per_warp, V* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const V y = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += y;
+        for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+        if (lane == 0) s.row_sum[k] = e;
     }
     __syncthreads();
-    if (lane == 31) per_warp[warp] = v;
-    __syncthreads();
-    V before = 0, all = 0;
-    for (int w = 0; w < SF_WARPS; ++w) {
-        if (w < warp) before += per_warp[w];
-        all += per_warp[w];
-    }
-    *total = all;
-    return before + v;
+    if (warp != 0) return -1;
+    const double a = s.row_sum[lane], b = s.row_sum[lane + 32];
+    const double after_a = upto_warp + sf_warp_scan(a), half = __shfl_sync(0xffffffffu, after_a, 31), after_b = half + sf_warp_scan(b);
+    const unsigned long long some_rows = ((unsigned long long)__ballot_sync(0xffffffffu, b > 0.0) << 32) | __ballot_sync(0xffffffffu, a > 0.0);
+    const unsigned long long hold_rows = ((unsigned long long)__ballot_sync(0xffffffffu, b > 0.0 && target < after_b) << 32) |
+                                         __ballot_sync(0xffffffffu, a > 0.0 && target < after_a);
+    to_end = to_end || hold_rows == 0ull;
+    const int k = to_end ? 63 - __clzll(some_rows) : __ffsll(hold_rows) - 1;
+    const double before_a = __shfl_sync(0xffffffffu, after_a, (k + 31) & 31), before_b = __shfl_sync(0xffffffffu, after_b, (k + 31) & 31);
+    const double row_before = k == 0 ? upto_warp : k <= 32 ? before_a : before_b;          // row 32 begins where row 31 ends
+    const double e = of(from + k * 32 + lane), upto = row_before + sf_warp_scan(e);
+    const unsigned some = __ballot_sync(0xffffffffu, e > 0.0), passed = __ballot_sync(0xffffffffu, e > 0.0 && !to_end && target < upto);
+    return lane == 0 ? from + k * 32 + (passed ? __ffs(passed) - 1 : 31 - __clz(some)) : -1;
 }
 
 constexpr int SF_EACH = SF_LIST / SF_THREADS;            // entries of the list a thread has
@@ -379,19 +465,25 @@ __device__ int sf_kept_by_weight(SfShared& s, const SfRow& r, int n, unsigned lo
     return kept;
 }
 
+// The first of the sorted list's n entries that `cuts` (a property that all behind it have too), or n.
+template <typename F> __device__ int sf_first(SfShared& s, int n, F cuts) {
+    if (threadIdx.x == 0) s.kept = n;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += SF_THREADS)
+        if (cuts(s.list[i])) { atomicMin(&s.kept, i); break; }
+    __syncthreads();
+    const int kept = s.kept;
+    __syncthreads();
+    return kept;
+}
+
 // The whole choice from the first block's list of the n largest.
 __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, double top_p, double min_p, double u, unsigned long long all) {
     sf_sort(s.list, n);
     int kept = n;
     if (top_k > 0 && top_k < n) {
         const unsigned kth = sf_key_of(s.list[top_k - 1]);
-        if (threadIdx.x == 0) s.kept = n;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += SF_THREADS)
-            if (sf_key_of(s.list[i]) < kth) atomicMin(&s.kept, i);
-        __syncthreads();
-        kept = s.kept;
-        __syncthreads();
+        kept = sf_first(s, n, [&](unsigned long long x) { return sf_key_of(x) < kth; });
     }
     if (top_p < 1.0) {
         if (top_k > 0) {                                 // the whole is what top_k left
@@ -401,18 +493,9 @@ __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, 
         }
         kept = sf_kept_by_weight(s, r, kept, 0ull, top_p, all);
     }
-    if (min_p > 0.0) {
-        if (threadIdx.x == 0) s.kept = kept;
-        __syncthreads();
-        for (int i = threadIdx.x; i < kept; i += SF_THREADS)
-            if (r.weight(sf_value(sf_key_of(s.list[i]))) < min_p) atomicMin(&s.kept, i);
-        __syncthreads();
-        kept = s.kept;
-        __syncthreads();
-    }
+    if (min_p > 0.0) kept = sf_first(s, kept, [&](unsigned long long x) { return r.weight(sf_value(sf_key_of(x))) < min_p; });
     // In the vocabulary's order: the index above the key, turned around so that the largest entry is the lowest index.
     for (int i = threadIdx.x; i < kept; i += SF_THREADS) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
-    __syncthreads();
     sf_sort(s.list, kept);
     double e[SF_EACH], mine = 0.0, total;
 #pragma unroll
@@ -438,18 +521,42 @@ __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, 
     return (int)~(unsigned)(s.list[at] >> 32);
 }
 
-// The exact cut inside the bin that a histogram found: every block leaves with it in `s.cut`.
-__device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& r, SfBins bins, const SfCut cut, bool by_weight, unsigned want, double top_p) {
+// The exact cut inside the bins that a histogram found: every block leaves with it in `s.cut`. `weight_above` lies above the level's keys.
+__device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& r, SfBins bins, const SfCut cut, unsigned want, double top_p,
+                          unsigned long long weight_above, unsigned long long all) {
     SfShared* home = cluster.map_shared_rank(&s, 0);
+    const bool by_weight = want == 0u;
     for (;;) {
         const SfFound f = s.found;
-        if (f.in_bin <= SF_LIST) {
-            sf_gather(cluster, s, r, bins, cut, f.bin, f.bin);
+        int from = f.from, to = f.to;
+        const unsigned within = f.upto - f.above;
+        if (by_weight) {
+            // What lies above the bins in question, exactly; where those are many and full, down to their middle too, which halves them.
+            const bool halve = within > (unsigned)SF_LIST && to - from > SF_BINS / 4;
+            const int middle = from + (to - from) / 2;
+            unsigned long long above = 0, down = 0;
+            r.each(fmaxf(sf_floor(cut), bins.floor(halve ? middle : from - 1)), [&](int i, float v) {
+                const unsigned key = sf_key(v);
+                if (!sf_left(cut, key, r.first + i)) return;
+                const int b = bins.of(v, key);
+                if (b < 0 || b > (halve ? middle : from - 1)) return;
+                const unsigned long long w = sf_fixed(r.weight(v));
+                if (b < from) above += w; else down += w;
+            });
+            sf_sum(cluster, s, above, down);
+            weight_above += above;
+            if (halve) {
+                if (sf_reached(weight_above + down, top_p, all)) to = middle;
+                else { from = middle + 1; weight_above += down; }
+            }
+        }
+        if (within <= (unsigned)SF_LIST) {
+            sf_gather(cluster, s, r, bins, cut, from, to);
             if (cluster.block_rank() == 0) {
-                const int n = f.in_bin;
+                const int n = (int)within;
                 sf_sort(s.list, n);
                 int last;                                // the last entry that is left
-                if (by_weight) last = sf_kept_by_weight(s, r, n, f.weight_above, top_p, f.weight_all) - 1;
+                if (by_weight) last = sf_kept_by_weight(s, r, n, weight_above, top_p, all) - 1;
                 else last = min(n - 1, max(0, (int)(want - f.above) - 1));
                 if (threadIdx.x == 0) {
                     SfCut c;
@@ -464,14 +571,14 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
         if (cluster.block_rank() == 0 && threadIdx.x == 0) { s.lo_key = 0xffffffffu; s.hi_key = 0u; }
         cluster.sync();
         unsigned lo = 0xffffffffu, hi = 0u;
-        for (int i = threadIdx.x; i < r.n; i += SF_THREADS) {
-            const float v = r.at(i);
-            if (!(v > -INFINITY)) continue;
+        r.each(fmaxf(sf_floor(cut), bins.floor(to)), [&](int i, float v) {
             const unsigned key = sf_key(v);
-            if (!sf_left(cut, key, r.first + i) || bins.of(v, key) != f.bin) continue;
+            if (!sf_left(cut, key, r.first + i)) return;
+            const int b = bins.of(v, key);
+            if (b < from || b > to) return;
             lo = min(lo, key);
             hi = max(hi, key);
-        }
+        });
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
         if ((threadIdx.x & 31) == 0 && lo <= hi) { atomicMin(&home->lo_key, lo); atomicMax(&home->hi_key, hi); }
@@ -479,23 +586,23 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
         lo = home->lo_key;
         hi = home->hi_key;
         cluster.sync();
-        if (lo == hi) {                                  // more equal tokens than the list holds
+        if (lo >= hi) {                                  // more equal tokens than the list holds
             SfCut c;
             c.key = lo;
             c.index = 0x7fffffff;
             if (by_weight) {
-                // The first `keep` of them: the smallest number that reaches top_p. The bin holds it, so it is one at least.
+                // The first `keep` of them: the smallest number that reaches top_p, one at least.
                 const unsigned long long e = sf_fixed(r.weight(sf_value(lo)));
-                int keep = f.in_bin;
+                const int tied = (int)within;            // (of a halved level fewer may be there: the count below stops at the last)
+                int keep = tied;
                 if (e > 0) {
-                    const double some = ceil((top_p * (double)f.weight_all - (double)f.weight_above) / (double)e);
-                    keep = (int)fmin(fmax(some, 1.0), (double)f.in_bin);
-                    while (keep > 1 && sf_reached(f.weight_above + (unsigned long long)(keep - 1) * e, top_p, f.weight_all)) --keep;
-                    while (keep < f.in_bin && !sf_reached(f.weight_above + (unsigned long long)keep * e, top_p, f.weight_all)) ++keep;
+                    const double some = ceil((top_p * (double)all - (double)weight_above) / (double)e);
+                    keep = (int)fmin(fmax(some, 1.0), (double)tied);
+                    while (keep > 1 && sf_reached(weight_above + (unsigned long long)(keep - 1) * e, top_p, all)) --keep;
+                    while (keep < tied && !sf_reached(weight_above + (unsigned long long)keep * e, top_p, all)) ++keep;
                 }
-                const int at = sf_locate(cluster, s, r, [&](int i) {
-                    const float v = r.at(i);
-                    return v > -INFINITY && sf_key(v) == lo && sf_left(cut, lo, r.first + i) ? 1.0 : 0.0;
+                const int at = sf_locate(cluster, s, r, fmaxf(SF_LOWEST, sf_value(lo)), [&](int i, float v) {
+                    return sf_key(v) == lo && sf_left(cut, lo, r.first + i) ? 1.0 : 0.0;
                 }, [&](double) { return (double)keep - 0.5; });
                 if (at >= 0)
                     for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->cut = SfCut{lo, r.first + at};
@@ -510,14 +617,21 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
         bins.hi = hi;
         bins.shift = 0;
         while (((hi - lo) >> bins.shift) >= (unsigned)SF_BINS) ++bins.shift;
-        sf_histogram(cluster, s, r, bins, cut, by_weight, want, top_p, f.above, f.weight_above, f.weight_all);
+        sf_clear(s);
+        r.each(fmaxf(SF_LOWEST, sf_value(lo)), [&](int i, float v) {
+            const unsigned key = sf_key(v);
+            if (!sf_left(cut, key, r.first + i)) return;
+            const int b = bins.of(v, key);
+            if (b >= 0) atomicAdd(&s.counts[b], 1u);
+        });
+        sf_find(cluster, s, r, bins, want, top_p, f.above, weight_above, all);
     }
 }
 
 __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const SfParams p) {
     extern __shared__ __align__(16) unsigned char sf_smem[];
     SfShared& s = *reinterpret_cast<SfShared*>(sf_smem);
-    float* cache = reinterpret_cast<float*>(sf_smem + sizeof(SfShared));
+    float* cache = reinterpret_cast<float*>(sf_smem + (sizeof(SfShared) + 15) / 16 * 16);
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int row = blockIdx.x / blocks;
@@ -528,80 +642,153 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
     r.n = min(p.vocab - r.first, p.share);
     r.cached = min(r.n, p.cached);
     r.row = p.logits + (size_t)row * p.vocab + r.first;
+    const int ahead = (int)(((uintptr_t)r.row >> 2) & 3);
+    cache += ahead;
     r.cache = cache;
-    Best mine;
-    mine.v = 0.f; mine.i = -1;
-    bool nan = false;
-#pragma unroll 8
-    for (int i = tid; i < r.n; i += SF_THREADS) {
-        const float v = r.row[i];
-        if (i < r.cached) cache[i] = v;
-        if (v != v) { nan = true; continue; }
-        Best c;
-        c.v = v; c.i = r.first + i;
-        mine = better(mine, c);
-    }
-    nan = __syncthreads_or(nan);
-    mine = block_best(mine, s.best);
-    cluster.barrier_wait();
-    if (tid < blocks) {
-        SfTop t;
-        t.best = mine; t.nan = nan ? 1 : 0; t.unused = 0;
-        cluster.map_shared_rank(&s, tid)->tops[rank] = t;
-    }
-    cluster.sync();
-    Best top;
-    top.v = 0.f; top.i = -1;
-    for (int b = 0; b < blocks; ++b) {
-        top = better(top, s.tops[b].best);
-        nan = nan || s.tops[b].nan != 0;
-    }
+    if (tid < 32) s.powers[tid] = exp2((double)tid / 32.0);          // before the barriers below
     const double temperature = p.temperature[row];
     const double top_p = p.top_p[row], min_p = p.min_p[row];
     const int top_k = p.top_k[row] > 0 && p.top_k[row] < p.vocab ? p.top_k[row] : 0;
     const double u = p.uniform[row];
+    // The share, 16 bytes at a time where both the row and its place in shared memory allow (the cache begins as far behind a multiple of
+    // 16 bytes as the share does). fmaxf passes over a NaN.
+    float most = -INFINITY;
+    bool nan = false;
+    {
+        const int head = min(r.n, (4 - ahead) & 3), fours = r.cached == r.n ? (r.n - head) / 4 : 0;
+        const float4* src = reinterpret_cast<const float4*>(r.row + head);
+        float4* dst = reinterpret_cast<float4*>(cache + head);
+        constexpr int DEEP = 8;
+        for (int base = 0; base < fours; base += DEEP * SF_THREADS) {
+            float4 x[DEEP];
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) {
+                const int i = base + k * SF_THREADS + tid;
+                x[k] = i < fours ? __ldcs(src + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            }
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) {
+                const int i = base + k * SF_THREADS + tid;
+                if (i < fours) dst[i] = x[k];
+                most = fmaxf(fmaxf(fmaxf(most, x[k].x), fmaxf(x[k].y, x[k].z)), x[k].w);
+                nan = nan || x[k].x != x[k].x || x[k].y != x[k].y || x[k].z != x[k].z || x[k].w != x[k].w;
+            }
+        }
+        auto one = [&](int i) {
+            const float v = r.row[i];
+            if (i < r.cached) cache[i] = v;
+            most = fmaxf(most, v);
+            nan = nan || v != v;
+        };
+        if (tid < head) one(tid);
+        for (int i = head + 4 * fours + tid; i < r.n; i += SF_THREADS) one(i);
+    }
+    const float own = most;                              // this thread's largest
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((tid & 31) == 0) s.warp_max[tid >> 5] = most;
+    nan = __syncthreads_or(nan);
+    most = s.warp_max[tid & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    cluster.barrier_wait();
+    if (tid < blocks) cluster.map_shared_rank(&s, tid)->tops[rank] = SfTop{most, nan ? 1 : 0};
+    cluster.sync();
+    for (int b = 0; b < blocks; ++b) {
+        most = fmaxf(most, s.tops[b].v);
+        nan = nan || s.tops[b].nan != 0;
+    }
     // Certain choices: greedy; a temperature that is no number leaves token 0, as a top_p that keeps nothing does; with a NaN among the
     // logits, an infinite one, or none above -inf the probabilities are none and the first largest stands.
     const bool greedy = temperature <= 0.0;
-    if (greedy || !(temperature > 0.0) || top_p <= 0.0 || min_p > 1.0 || nan || top.i < 0 || isinf(top.v)) {
-        const bool none = !greedy && (!(temperature > 0.0) || top_p <= 0.0 || (min_p > 1.0 && !nan && !isinf(top.v)));
-        if (rank == 0 && tid == 0) p.tokens[row] = none || top.i < 0 ? 0 : top.i;
+    if (greedy || !(temperature > 0.0) || top_p <= 0.0 || min_p > 1.0 || nan || isinf(most)) {
+        const bool none = !greedy && (!(temperature > 0.0) || top_p <= 0.0 || (min_p > 1.0 && !nan && !isinf(most)));
+        SfShared* home = cluster.map_shared_rank(&s, 0);
+        if (rank == 0 && tid == 0) s.owner = 0x7fffffff;
+        cluster.sync();
+        int first = 0x7fffffff;
+        for (int i = tid; i < r.n; i += SF_THREADS)
+            if (r.at(i) == most) { first = r.first + i; break; }
+        first = __reduce_min_sync(0xffffffffu, first);
+        if ((tid & 31) == 0 && first != 0x7fffffff) atomicMin(&home->owner, first);
+        cluster.sync();
+        if (rank == 0 && tid == 0) p.tokens[row] = none || s.owner == 0x7fffffff ? 0 : s.owner;
         return;
     }
-    r.largest = top.v;
-    r.inv = isinf(temperature) ? 0.0 : fmin(1.0 / temperature, 1e300);
+    r.scale(most, temperature, s.powers);
     SfCut cut;
     cut.key = 0u; cut.index = 0x7fffffff;
     SfBins bins;
     bins.by_key = false;
-    bins.largest = top.v;
+    bins.largest = most;
     bins.step = (float)((SF_BINS - 1) * r.inv / SF_SPAN);
     bins.lo = 0u; bins.hi = 0xffffffffu; bins.shift = 0;
-    bool by_k = top_k > 0, by_p = top_p < 1.0;
-    while (by_k || by_p) {
-        const bool by_weight = !by_k;
-        sf_histogram(cluster, s, r, bins, cut, by_weight, (unsigned)top_k, top_p, 0u, 0ull, 0ull);
-        const SfFound f = s.found;
-        if (f.upto <= (unsigned)SF_LIST) {
-            sf_gather(cluster, s, r, bins, cut, 0, f.bin);
+    const bool by_p = top_p < 1.0;
+    if (top_k > 0) {
+        if (top_k <= SF_LIST / 2) {
+            sf_clear(s);
+            if (own > -INFINITY) atomicAdd(&s.counts[bins.of(own, sf_key(own))], 1u);
+            sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull);
+            if (s.found.upto >= (unsigned)top_k) {
+                const int down = s.found.to;
+                sf_gather(cluster, s, r, bins, cut, 0, down);
+                const int listed = cluster.map_shared_rank(&s, 0)->listed;
+                if (listed <= SF_LIST) {
+                    cluster.sync();                      // the first block's count has been read
+                    if (rank == 0) {
+                        const int token = sf_draw_from_list(s, r, listed, top_k, by_p ? top_p : 1.0, min_p, u, 0ull);
+                        if (tid == 0) p.tokens[row] = token;
+                    }
+                    return;
+                }
+            }
+        }
+        sf_clear(s);
+        r.each(SF_LOWEST, [&](int, float v) { atomicAdd(&s.counts[bins.of(v, 0u)], 1u); });
+        sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull);
+        if (s.found.upto <= (unsigned)SF_LIST) {
+            const int n = (int)(s.found.upto);
+            sf_gather(cluster, s, r, bins, cut, 0, s.found.to);
             if (rank == 0) {
-                const int token = sf_draw_from_list(s, r, (int)f.upto, by_k ? top_k : 0, by_p ? top_p : 1.0, min_p, u, f.weight_all);
+                const int token = sf_draw_from_list(s, r, n, top_k, by_p ? top_p : 1.0, min_p, u, 0ull);
                 if (tid == 0) p.tokens[row] = token;
             }
             return;
         }
-        sf_refine(cluster, s, r, bins, cut, by_weight, (unsigned)top_k, top_p);
+        sf_refine(cluster, s, r, bins, cut, (unsigned)top_k, 0.0, 0ull, 0ull);
         cut = s.cut;
-        if (by_k) by_k = false; else by_p = false;
+    }
+    if (by_p) {
+        sf_clear(s);
+        unsigned long long all = 0, unused = 0;
+        r.each(sf_floor(cut), [&](int i, float v) {
+            const unsigned key = sf_key(v);
+            if (!sf_left(cut, key, r.first + i)) return;
+            atomicAdd(&s.counts[bins.of(v, key)], 1u);
+            all += sf_fixed(r.weight(v));
+        });
+        sf_sum(cluster, s, all, unused);
+        sf_find(cluster, s, r, bins, 0u, top_p, 0u, 0ull, all);
+        if (s.found.upto <= (unsigned)SF_LIST) {
+            const int n = (int)(s.found.upto);
+            sf_gather(cluster, s, r, bins, cut, 0, s.found.to);
+            if (rank == 0) {
+                const int token = sf_draw_from_list(s, r, n, 0, top_p, min_p, u, all);
+                if (tid == 0) p.tokens[row] = token;
+            }
+            return;
+        }
+        sf_refine(cluster, s, r, bins, cut, 0u, top_p, 0ull, all);
+        cut = s.cut;
     }
     // Below this a weight is under min_p for sure: no exponential.
-    const double floor = min_p > 0.0 ? (double)top.v + log(min_p) / r.inv : -INFINITY;
-    const float floor_v = min_p > 0.0 ? (float)(floor - 1e-5 * (fabs(floor) + fabs((double)top.v)) - 1e-30) : -INFINITY;
-    const int at = sf_locate(cluster, s, r, [&](int i) {
-        const float v = r.at(i);
-        if (!(v > -INFINITY) || v < floor_v || !sf_left(cut, sf_key(v), r.first + i)) return 0.0;
+    const double floor = min_p > 0.0 ? (double)most + log(min_p) / r.inv : -INFINITY;
+    const float floor_v = min_p > 0.0 ? (float)(floor - 1e-5 * (fabs(floor) + fabs((double)most)) - 1e-30) : -INFINITY;
+    const float sure_v = min_p > 0.0 ? (float)(floor + 1e-5 * (fabs(floor) + fabs((double)most)) + 1e-30) : -INFINITY;       // above this it is not, for sure
+    const int at = sf_locate(cluster, s, r, fmaxf(sf_floor(cut), floor_v), [&](int i, float v) {
+        if (!sf_left(cut, sf_key(v), r.first + i)) return 0.0;
         const double e = r.weight(v);
-        return e < min_p ? 0.0 : e;
+        return v < sure_v && e < min_p ? 0.0 : e;
     }, [&](double total) { return u * total; });
     if (at >= 0) p.tokens[row] = r.first + at;
     cluster.sync();                                      // nobody leaves while another may still write to it
@@ -629,9 +816,9 @@ extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double
     p.share = (vocab + blocks - 1) / blocks;
     constexpr int MOST = 232448 - 1024;
     static_assert(sizeof(SfShared) + 65536 <= MOST, "the histogram and the list leave no room for a share");
-    p.cached = (int)(((size_t)MOST - sizeof(SfShared)) / 4);
+    p.cached = (int)(((size_t)MOST - sizeof(SfShared) - 32) / 4);
     if (p.cached > p.share) p.cached = p.share;
-    const size_t smem = sizeof(SfShared) + (size_t)p.cached * 4;
+    const size_t smem = (sizeof(SfShared) + 15) / 16 * 16 + 16 + (size_t)p.cached * 4;
     const cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
     KB_REQUIRE(e == cudaSuccess, "sample_filtered: cannot have %d bytes of shared memory: %s", MOST, cudaGetErrorString(e));
     cudaLaunchConfig_t cfg = {};
