@@ -158,90 +158,104 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
                 if (at + 2 < p.dv) piece[at + 2] = acc[c].z;
                 if (at + 3 < p.dv) piece[at + 3] = acc[c].w;
             }
-            if (sub == 0) { piece[p.dv] = m; piece[p.dv + 1] = l; }
+            if (sub == 0) { piece[(p.dv + 3) / 4 * 4] = m; piece[(p.dv + 3) / 4 * 4 + 1] = l; }
         }
     }
 }
 
-// Joins a (row, head) pair's pieces: its tile's, worker by worker, then its own. A block a pair: the pieces' references and sums all at once, then
-// LANES threads a piece, four components each, several pieces side by side; their sums in the order of the threads' groups.
-constexpr int SJ_THREADS = 256, SJ_PIECES = 512;
+// Joins a (row, head) pair's pieces: its tile's, worker by worker, then its own. A warp a pair: 32 pieces' references and sums at once, a lane each,
+// then four (or eight) components a lane over the pieces in their order.
+constexpr int SJ_WARPS = 4;
 template <typename T>
-__global__ void __launch_bounds__(SJ_THREADS) shared_combine_kernel(const SharedParams p, int tile_pairs) {
-    __shared__ float weight[SJ_PIECES];
-    __shared__ float scratch[32];
-    __shared__ float4 part[SJ_THREADS];
-    const int r = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+__global__ void __launch_bounds__(SJ_WARPS * 32) shared_combine_kernel(const SharedParams p, int tile_pairs) {
+    const int pair = blockIdx.x * SJ_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (pair >= p.rows * p.hq) return;
+    const int r = pair / p.hq, head = pair % p.hq;
     const int group = p.hq / p.hkv, kvh = head / group, width = SH_PIECE(p.dv);
-    const int t = p.cut[SH_CUT_ROW_TILE + r], tiles = p.cut[SH_CUT_COUNTS];
-    const int row_units = p.cut[SH_CUT_ROW_UNITS + r + 1] - p.cut[SH_CUT_ROW_UNITS + r];
+    const int t = p.cut[SH_CUT_ROW_TILE + r], tiles = p.cut[SH_CUT_COUNTS], row_at = p.cut[SH_CUT_ROW_UNITS + r];
+    const int row_units = p.cut[SH_CUT_ROW_UNITS + r + 1] - row_at;
+    const int all_tiles = p.cut[SH_CUT_TILE_UNITS + tiles], all_rows = p.cut[SH_CUT_ROW_UNITS + p.rows];
+    const int tile_workers = p.cut[SH_CUT_COUNTS + 1], row_workers = p.cut[SH_CUT_COUNTS + 2];
+    const float sink = p.sinks ? p.sinks[head] : -INFINITY;
     const float* piece[2] = {nullptr, nullptr};          // the first of the tile's and of the row's, and the floats from one to the next
     int count[2] = {0, 0};
     const size_t step[2] = {(size_t)tile_pairs * width, (size_t)group * width};
-    const int tile_units = t < 0 ? 0 : p.cut[SH_CUT_TILE_UNITS + t + 1] - p.cut[SH_CUT_TILE_UNITS + t];
-    if (tile_units > 0) {
+    if (t >= 0) {
+        const int at = p.cut[SH_CUT_TILE_UNITS + t], units = p.cut[SH_CUT_TILE_UNITS + t + 1] - at;
         const int* tile = p.cut + SH_CUT_TILES + 3 * t;
-        const long long u = (long long)p.cut[SH_CUT_TILE_UNITS + t] * p.hkv + (long long)kvh * tile_units, all = (long long)p.cut[SH_CUT_TILE_UNITS + tiles] * p.hkv;
-        const int workers = p.cut[SH_CUT_COUNTS + 1], first = shared_worker_of(u, all, workers);
-        count[0] = shared_worker_of(u + tile_units - 1, all, workers) - first + 1;
-        piece[0] = p.tile_pieces + (shared_tile_place(p, tile[2], tile[1], kvh, first, tile_pairs) + (r - tile[0]) * group + head % group) * width;
+        const int row0 = tile[0], n = tile[1], before = tile[2];
+        if (units > 0) {
+            const long long u = (long long)at * p.hkv + (long long)kvh * units, all = (long long)all_tiles * p.hkv;
+            const int first = shared_worker_of(u, all, tile_workers);
+            count[0] = shared_worker_of(u + units - 1, all, tile_workers) - first + 1;
+            piece[0] = p.tile_pieces + (shared_tile_place(p, before, n, kvh, first, tile_pairs) + (r - row0) * group + head % group) * width;
+        }
     }
     if (row_units > 0) {
-        const long long u = (long long)p.cut[SH_CUT_ROW_UNITS + r] * p.hkv + (long long)kvh * row_units, all = (long long)p.cut[SH_CUT_ROW_UNITS + p.rows] * p.hkv;
-        const int workers = p.cut[SH_CUT_COUNTS + 2], first = shared_worker_of(u, all, workers);
-        count[1] = shared_worker_of(u + row_units - 1, all, workers) - first + 1;
+        const long long u = (long long)row_at * p.hkv + (long long)kvh * row_units, all = (long long)all_rows * p.hkv;
+        const int first = shared_worker_of(u, all, row_workers);
+        count[1] = shared_worker_of(u + row_units - 1, all, row_workers) - first + 1;
         piece[1] = p.row_pieces + (shared_row_place(p, r, kvh, first) + head % group) * width;
     }
     const int n = count[0] + count[1];
     auto at = [&](int b) { return b < count[0] ? piece[0] + b * step[0] : piece[1] + (b - count[0]) * step[1]; };
-    const int lanes = (p.dv + 3) / 4, groups = SJ_THREADS / lanes, mine = tid / lanes, c = tid % lanes * 4;
-    const float sink = p.sinks ? p.sinks[head] : -INFINITY;
-    float m = sink, total = 0.f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int base = 0; base < n; base += SJ_PIECES) {    // (one turn but for very many workers)
-        const int here = min(SJ_PIECES, n - base);
-        float most = -INFINITY;
-        for (int b = tid; b < here; b += SJ_THREADS) most = fmaxf(most, at(base + b)[p.dv]);
-        most = fmaxf(block_max(most, scratch), m);
-        const float fade = most == -INFINITY ? 1.f : expf(m - most);
-        m = most;
-        sum.x *= fade; sum.y *= fade; sum.z *= fade; sum.w *= fade;
-        float l = 0.f;
-        for (int b = tid; b < here; b += SJ_THREADS) {
-            const float* x = at(base + b);
-            const float w = x[p.dv] == -INFINITY ? 0.f : expf(x[p.dv] - m);          // a range of which the row sees nothing
-            weight[b] = w;
-            l = w > 0.f ? fmaf(w, x[p.dv + 1], l) : l;
+    float m = sink;
+    for (int b = lane; b < n; b += 32) m = fmaxf(m, at(b)[(p.dv + 3) / 4 * 4]);
+    m = warp_max(m);
+    const int quads = (p.dv + 3) / 4;                    // of components: lane's, and from 128 components on 32 + lane's
+    float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    float l = 0.f;
+    for (int base = 0; base < n; base += 32) {
+        float mine = 0.f;
+        if (base + lane < n) {
+            const float2 x = *reinterpret_cast<const float2*>(at(base + lane) + (p.dv + 3) / 4 * 4);
+            mine = x.x == -INFINITY ? 0.f : expf(x.x - m);           // a range of which the row sees nothing
+            l = mine > 0.f ? fmaf(mine, x.y, l) : l;
         }
-        total = total * (base ? fade : 0.f) + block_sum(l, scratch);     // its barriers show the weights to all
-        if (mine < groups) {
-#pragma unroll 4
-            for (int b = mine; b < here; b += groups) {
-                const float w = weight[b];
-                if (w == 0.f) continue;
-                const float4 x = *reinterpret_cast<const float4*>(at(base + b) + c);
-                sum.x = fmaf(w, x.x, sum.x);
-                sum.y = fmaf(w, x.y, sum.y);
-                sum.z = fmaf(w, x.z, sum.z);
-                sum.w = fmaf(w, x.w, sum.w);
+        const int here = min(32, n - base);
+        constexpr int DEEP = 8;                          // pieces asked for before the first is used
+        for (int b0 = 0; b0 < here; b0 += DEEP) {
+            float4 v[DEEP][2];
+#pragma unroll
+            for (int b = 0; b < DEEP; ++b) {
+                const float4* x = reinterpret_cast<const float4*>(at(base + min(b0 + b, here - 1)));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) v[b][k] = lane + 32 * k < quads ? x[lane + 32 * k] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int b = 0; b < DEEP; ++b) {
+                const float w = __shfl_sync(0xffffffffu, mine, min(b0 + b, 31));
+                if (w == 0.f || b0 + b >= here) continue;            // (a piece without weight may be anything)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    sum[k].x = fmaf(w, v[b][k].x, sum[k].x);
+                    sum[k].y = fmaf(w, v[b][k].y, sum[k].y);
+                    sum[k].z = fmaf(w, v[b][k].z, sum[k].z);
+                    sum[k].w = fmaf(w, v[b][k].w, sum[k].w);
+                }
             }
         }
-        __syncthreads();
     }
+    float total = warp_sum(l);
     if (p.sinks && m != -INFINITY) total += expf(sink - m);
-    part[tid] = sum;
-    __syncthreads();
-    if (tid >= lanes) return;
-    for (int k = 1; k < groups; ++k) {
-        const float4 x = part[k * lanes + tid];
-        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-    }
     const float inv = total > 0.f ? 1.f / total : 0.f;
-    T* out = static_cast<T*>(p.out) + ((size_t)r * p.hq + head) * p.dv;
-    const float v[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+    T* out = static_cast<T*>(p.out) + (size_t)pair * p.dv;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < p.dv) Elem<T>::store(out + c + j, v[j]);
+    for (int k = 0; k < 2; ++k) {
+        const int c = 4 * (lane + 32 * k);
+        const float v[4] = {sum[k].x * inv, sum[k].y * inv, sum[k].z * inv, sum[k].w * inv};
+        if (c + 3 < p.dv && p.dv % 4 == 0) {
+            store_four(out + c, make_float4(v[0], v[1], v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < p.dv) Elem<T>::store(out + c + j, v[j]);
+        }
+    }
+}
+template <typename T> static int launch_combine(const SharedParams& p, int tile_pairs, cudaStream_t s) {
+    shared_combine_kernel<T><<<(p.rows * p.hq + SJ_WARPS - 1) / SJ_WARPS, SJ_WARPS * 32, 0, s>>>(p, tile_pairs);
+    return check_launch("shared_attention");
 }
 
 template <typename T> static int launch_shared_rows(const SharedParams& p, int blocks, cudaStream_t s) {
@@ -250,8 +264,7 @@ template <typename T> static int launch_shared_rows(const SharedParams& p, int b
     KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
     shared_rows_kernel<T><<<blocks, SR_THREADS, smem, s>>>(p);
     if (int err = check_launch("shared_attention")) return err;
-    shared_combine_kernel<T><<<dim3(p.rows, p.hq), SJ_THREADS, 0, s>>>(p, SR_PAIRS);
-    return check_launch("shared_attention");
+    return launch_combine<T>(p, SR_PAIRS, s);
 }
 
 }  // namespace kb
@@ -314,9 +327,11 @@ extern "C" int kb_shared_attention(void* out, const void* q, const void* k_table
         if (int e = encode_map_bf16(&mk, k_table, lines, d, d, 16)) return e;
         if (int e = encode_map_bf16(&mv, v_table, lines, d, d, 16)) return e;
         if (int e = launch_shared_tiles(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
-        if (int e = launch_shared_own(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
-        shared_combine_kernel<__nv_bfloat16><<<dim3(rows, hq), SJ_THREADS, 0, (cudaStream_t)stream>>>(p, 128);
-        return check_launch("shared_attention");
+        CUtensorMap ok, ov;                              // the same in boxes of all of a line's chunks
+        if (int e = encode_map_bf16_chunks(&ok, k_table, lines, d, 16)) return e;
+        if (int e = encode_map_bf16_chunks(&ov, v_table, lines, d, 16)) return e;
+        if (int e = launch_shared_own(p, ok, ov, blocks, (cudaStream_t)stream)) return e;
+        return launch_combine<__nv_bfloat16>(p, 128, (cudaStream_t)stream);
     }
     return dtype == KB_DT_F32 ? launch_shared_rows<float>(p, blocks, (cudaStream_t)stream) : launch_shared_rows<__nv_bfloat16>(p, blocks, (cudaStream_t)stream);
 }

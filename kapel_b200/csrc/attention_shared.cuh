@@ -22,7 +22,7 @@
 namespace kb {
 
 constexpr int SH_ROWS = 512;                 // requests of one call
-__host__ __device__ constexpr int SH_PIECE(int dv) { return (dv + 3) / 4 * 4 + 4; }      // floats of a piece: dv, then m and the sum of weights; rows of 16 bytes
+__host__ __device__ constexpr int SH_PIECE(int dv) { return (dv + 3) / 4 * 4 + 4; }      // floats of a piece: dv (up to a multiple of four), then m and the sum of weights
 
 struct SharedParams {
     const void* q;             // [rows, hq, d]

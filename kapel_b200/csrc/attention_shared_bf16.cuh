@@ -81,15 +81,17 @@ __device__ __forceinline__ unsigned long long sh_fma2(unsigned long long a, unsi
 template <int N> __device__ __forceinline__ float sh_scores(uint32_t (&x)[N], const SharedScore& score) {
     const float first = score.cap ? score.u : score.in;
     const unsigned long long in = sh_pair(first, first);
-    float top = -INFINITY, far = 0.f;
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, fars[4] = {0.f, 0.f, 0.f, 0.f};        // four chains side by side
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
         sh_split(sh_mul2(sh_pair(x[j], x[j + 1]), in), x[j], x[j + 1]);
-        top = fmaxf(fmaxf(top, __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
+        tops[(j >> 1) & 3] = fmaxf(fmaxf(tops[(j >> 1) & 3], __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
     }
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     if (!score.cap) return top;
 #pragma unroll
-    for (int j = 0; j < N; j += 2) far = fmaxf(fmaxf(far, fabsf(__uint_as_float(x[j]))), fabsf(__uint_as_float(x[j + 1])));
+    for (int j = 0; j < N; j += 2) fars[(j >> 1) & 3] = fmaxf(fmaxf(fars[(j >> 1) & 3], fabsf(__uint_as_float(x[j]))), fabsf(__uint_as_float(x[j + 1])));
+    const float far = fmaxf(fmaxf(fars[0], fars[1]), fmaxf(fars[2], fars[3]));
     // (a NaN is passed over by fmaxf and goes through the polynomial as well as through the other)
     if (!__all_sync(0xffffffffu, far <= 0.75f)) {
 #pragma unroll

@@ -1,7 +1,8 @@
 // What each request reads by itself behind the pages it shares (bfloat16; see attention_shared.cuh for the cut): every warp a worker.
 //
-// The units are 16 positions of one kv head, which lie in one page: TMA brings their keys and values as D / 64 boxes of 16 x 64 elements each
-// (128-byte swizzle) into a pipeline that is the warp's own. A warp walks its units whatever items they belong to, requests
+// The units are 16 positions of one kv head, which lie in one page: TMA brings their keys and their values as one box each of D / 64 x 16 x 64
+// elements (128-byte swizzle) into a pipeline that is the warp's own (a request a lane: as eight boxes of 16 x 64 they took 1,100 clocks of the
+// 2,400 that a unit of 256 components took). A warp walks its units whatever items they belong to, requests
 // for the next item's keys go out while it still computes on the one before, and nothing in the loop waits for another warp: short answers of many
 // requests stream like one long one. The products have the keys as the MMAs' M (S^T = K Q^T, O^T = V^T P^T), the query
 // heads of the kv head as their N, eight a block, NB blocks; P^T comes out of S^T's registers by movmatrix. Scores, softmax and sums are 32-bit; the
@@ -77,9 +78,8 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
             const int row = (page * p.hkv + a_kvh) * p.page_size + (a_j + 16 * a_in) % p.page_size;
             if (lane == 0) at_mbar_expect_tx(bars + stage, C::STAGE);
             __syncwarp();
-            const uint32_t dst = at_saddr(pipe + stage * C::STAGE) + lane * 2048u;
-            if (lane < C::BOXES) at_tma_box(dst, &map_k, lane * 64, row, bars + stage);
-            else if (lane < 2 * C::BOXES) at_tma_box(dst, &map_v, (lane - C::BOXES) * 64, row, bars + stage);
+            const uint32_t dst = at_saddr(pipe + stage * C::STAGE) + lane * (C::STAGE / 2);
+            if (lane < 2) at_tma_page(dst, lane == 0 ? &map_k : &map_v, row, bars + stage);
             absent &= ~(1u << stage);
         } else {
             if (lane == 0) at_mbar_arrive(bars + stage);     // nothing to wait for

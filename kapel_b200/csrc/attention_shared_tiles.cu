@@ -46,6 +46,20 @@ __device__ __forceinline__ TilePart st_part(const SharedParams& p, const SharedT
     return w;
 }
 
+// Lane i's word j becomes lane j's word i.
+__device__ __forceinline__ void st_transpose(uint32_t (&x)[32], int lane) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        const bool up = (lane & s) != 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (j & s) continue;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? x[j] : x[j + s], s);
+            if (up) x[j] = got; else x[j + s] = got;
+        }
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(ST_THREADS, 1)
 shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -210,12 +224,26 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
         const bf16* q = static_cast<const bf16*>(p.q);
         // A part's queries, K-major under the swizzle: chunk c of pair r at c 16 KB + r 128, its 16-byte pieces exchanged by r mod 8. Eight
         // neighbouring threads bring a pair's 128 bytes. Pairs that are none keep what is there: nobody reads their results.
+        const uint32_t by_group = (65536u + (uint32_t)group - 1u) / (uint32_t)group;          // r / group = r by_group >> 16 for r < 128
         auto lay_queries = [&](const TilePart& w) {
             const int pairs = w.n * group;
-            for (int i = st; i < pairs * CH * 8; i += 256) {
-                const int j = i & 7, ch = (i >> 3) % CH, r = (i >> 3) / CH;
-                const uint4 x = *reinterpret_cast<const uint4*>(q + ((size_t)(w.row0 + r / group) * p.hq + w.kvh * group + r % group) * D + ch * 64 + j * 8);
-                *reinterpret_cast<uint4*>(q_smem + (size_t)ch * (ST_PAIRS * 128) + (size_t)r * 128 + ((j ^ (r & 7)) << 4)) = x;
+            constexpr int ITER = ST_PAIRS * CH * 8 / 256, DEEP = ITER < 8 ? ITER : 8;          // pieces a thread; asked for eight at a time
+            const int j = st & 7, ch = (st >> 3) % CH, r0 = (st >> 3) / CH;
+            const bf16* src = q + ((size_t)w.row0 * p.hq + w.kvh * group) * D + ch * 64 + j * 8;
+            unsigned char* dst = q_smem + ch * (ST_PAIRS * 128);
+            for (int base = 0; base < ITER; base += DEEP) {
+                uint4 x[DEEP];
+#pragma unroll
+                for (int k = 0; k < DEEP; ++k) {
+                    const int r = r0 + (base + k) * (32 / CH);
+                    const uint32_t row = (uint32_t)r * by_group >> 16;
+                    x[k] = r < pairs ? *reinterpret_cast<const uint4*>(src + (size_t)(row * p.hq + (r - row * group)) * D) : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int k = 0; k < DEEP; ++k) {
+                    const int r = r0 + (base + k) * (32 / CH);
+                    if (r < pairs) *reinterpret_cast<uint4*>(dst + (size_t)r * 128 + ((j ^ (r & 7)) << 4)) = x[k];
+                }
             }
             at_fence_async_smem();
             __syncwarp();
@@ -285,7 +313,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                     }
                     const float base = ref == -INFINITY ? 0.f : ref;
                     const unsigned long long less = sh_pair(-base, -base);
-                    unsigned long long sums = 0ull;
+                    unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};
                     uint32_t pr[HALF / 2];
 #pragma unroll
                     for (int k = 0; k < HALF / 32; ++k)
@@ -294,11 +322,11 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                             uint32_t a, c2;
                             sh_split(sh_add2(sh_pair(x[k][j], x[k][j + 1]), less), a, c2);
                             const uint32_t two = at_pack(at_exp2(__uint_as_float(a)), at_exp2(__uint_as_float(c2)));
-                            sums = sh_add2(sums, sh_pair(two << 16, two & 0xffff0000u));
+                            sums[(j >> 1) & 3] = sh_add2(sums[(j >> 1) & 3], sh_pair(two << 16, two & 0xffff0000u));
                             pr[k * 16 + (j >> 1)] = two;
                         }
                     uint32_t la, lb;
-                    sh_split(sums, la, lb);
+                    sh_split(sh_add2(sh_add2(sums[0], sums[1]), sh_add2(sums[2], sums[3])), la, lb);
                     l += __uint_as_float(la) + __uint_as_float(lb);
                     if constexpr (HALF == 64) at_st32(lanes + (uint32_t)(C::COL_S + b * KEYS + half * 32), pr);
                     else at_st16(lanes + (uint32_t)(C::COL_S + b * KEYS + half * 16), pr);
@@ -325,22 +353,21 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
             if (!failed && !__all_sync(0xffffffffu, at_mbar_wait(o_full, (uint32_t)part & 1u))) failed = true;
             if (!failed && !idle) {
                 at_fence_after();
-                float* piece = p.tile_pieces + (mine.place + pair) * SH_PIECE(D);
+                // 32 pairs x 32 components a time, turned around in registers: a pair's components leave side by side, a line a store.
+                float* pieces = p.tile_pieces + (mine.place + quarter * 32) * SH_PIECE(D);
+                const int here = min(32, mine.n * group - quarter * 32);
                 for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
                     uint32_t o[32];
                     __syncwarp();
                     at_ld32(lanes + (uint32_t)c0, o);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (!own) continue;
+                    st_transpose(o, lane);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(piece + c0 + j) =
-                            make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+                    for (int j = 0; j < 32; ++j)
+                        if (j < here) pieces[(size_t)j * SH_PIECE(D) + c0 + lane] = __uint_as_float(o[j]);
                 }
-                if (own && half == 0) {
-                    piece[D] = ref == -INFINITY ? -INFINITY : ref * 0.6931471805599453f;
-                    piece[D + 1] = l;
-                }
+                if (own && half == 0)
+                    *reinterpret_cast<float2*>(pieces + (size_t)lane * SH_PIECE(D) + D) = make_float2(ref == -INFINITY ? -INFINITY : ref * 0.6931471805599453f, l);
             }
             at_fence_before();
         }
