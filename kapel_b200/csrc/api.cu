@@ -23,8 +23,9 @@ static unsigned long long g_launches = 0;
 static unsigned long long g_dependent_launches = 0;
 static bool g_pdl = false;
 static thread_local int g_pass_rows = 0;
+bool may_chain(bool dependent) { return dependent && g_pdl && g_pass_rows <= DEPENDENT_ROWS; }
 bool chains(bool dependent) {
-    if (!dependent || !g_pdl || g_pass_rows > DEPENDENT_ROWS) return false;
+    if (!may_chain(dependent)) return false;
     ++g_dependent_launches;
     return true;
 }

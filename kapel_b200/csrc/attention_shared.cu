@@ -7,10 +7,12 @@
 // positions end there) what a row does not see is left out of its sum, not multiplied by zero: it may be anything.
 #include "attention_shared_bf16.cuh"
 #include "tensor_map.cuh"
+#include <cstdlib>
 
 namespace kb {
 
 constexpr int SR_PAIRS = 32, SR_KEYS = 32, SR_THREADS = 256, SR_DIM = 256;
+static_assert(SR_PAIRS == SR_KEYS, "queries are laid out as lines are");
 
 template <typename T> struct SharedRowsSmem {
     float q[SR_PAIRS][SR_DIM + 4];
@@ -18,8 +20,36 @@ template <typename T> struct SharedRowsSmem {
     float v[SR_KEYS][SR_DIM];
     long long line[SR_KEYS];               // a position's line of this kv head in the tables, -1 for none
     SharedTiles tiles;
-    int upto[SH_ROWS + 1];                 // units before a row
+    int upto[SH_ROWS + 1], lo[SH_ROWS], hi[SH_ROWS];       // units before a row, the positions it reads by itself
 };
+
+// SR_KEYS lines of `size` components into shared memory in 32 bits, zeros where a line is none and up to a multiple of four components.
+template <typename T, int STRIDE> __device__ __forceinline__ void sr_lines(float* to, const T* table, const long long* lines, int size, bool fours) {
+    constexpr int WARPS = SR_THREADS / 32, ROWS = SR_KEYS / WARPS, QUADS = SR_DIM / 128;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (fours) {
+        float4 x[ROWS][QUADS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int k = 0; k < QUADS; ++k) {
+                const long long line = lines[warp + i * WARPS];
+                const int c = 4 * (lane + 32 * k);
+                x[i][k] = line >= 0 && c < size ? load_four(table + line * size + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int k = 0; k < QUADS; ++k) {
+                const int c = 4 * (lane + 32 * k);
+                if (c < size) *reinterpret_cast<float4*>(to + (warp + i * WARPS) * STRIDE + c) = x[i][k];
+            }
+    } else {
+        for (int r = warp; r < SR_KEYS; r += WARPS)
+            for (int c = lane; c < (size + 3) / 4 * 4; c += 32)
+                to[r * STRIDE + c] = c < size && lines[r] >= 0 ? Elem<T>::load(table + lines[r] * size + c) : 0.f;
+    }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedParams p) {
@@ -31,7 +61,7 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
     const T* kt = static_cast<const T*>(p.k_table);
     const T* vt = static_cast<const T*>(p.v_table);
     shared_cut_tiles(p, s.tiles, rows_a_tile, SR_KEYS);
-    shared_cut_rows(p, s.upto, SR_KEYS);
+    shared_cut_rows(p, s.upto, s.lo, s.hi, SR_KEYS);
     const SharedRange over[2] = {shared_range(blockIdx.x, gridDim.x, s.tiles.upto[s.tiles.tiles], p.hkv), shared_range(blockIdx.x, gridDim.x, s.upto[p.rows], p.hkv)};
     if (blockIdx.x == 0) {
         shared_leave_tiles(p, s.tiles, over[0].workers);
@@ -53,7 +83,7 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
             pieces = p.tile_pieces + shared_tile_place(p, s.tiles.before[item], w.n, w.kvh, blockIdx.x, SR_PAIRS) * SH_PIECE(p.dv);
         } else {
             w.row0 = w.looks = item; w.n = 1;
-            shared_own(p, item, SR_KEYS, w.lo, w.hi);
+            w.lo = s.lo[item]; w.hi = s.hi[item];
             pieces = p.row_pieces + shared_row_place(p, item, w.kvh, blockIdx.x) * SH_PIECE(p.dv);
         }
         u += w.n_units;
@@ -61,10 +91,9 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
         const int row = w.row0 + pair / group;
         const bool own = pair < pairs;
         __syncthreads();                                 // the part before is done with the queries
-        for (int i = tid; i < pairs * d4 * 4; i += SR_THREADS) {
-            const int r = i / (d4 * 4), c = i % (d4 * 4);
-            s.q[r][c] = c < p.d ? Elem<T>::load(q + ((size_t)(w.row0 + r / group) * p.hq + w.kvh * group + r % group) * p.d + c) : 0.f;
-        }
+        if (tid < SR_KEYS) s.line[tid] = tid < pairs ? (long long)(w.row0 + tid / group) * p.hq + w.kvh * group + tid % group : -1;
+        __syncthreads();
+        sr_lines<T, SR_DIM + 4>(&s.q[0][0], q, s.line, p.d, p.d % 4 == 0);
         const int count = own ? min(p.row_count[row], w.hi) : 0;
         const int first = own ? max(shared_first(p, p.row_count[row]), w.lo) : 0;
         float m = -INFINITY, l = 0.f;
@@ -84,14 +113,9 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
                 s.line[tid] = line;
             }
             __syncthreads();
-            for (int i = tid; i < SR_KEYS * d4 * 4; i += SR_THREADS) {
-                const int r = i / (d4 * 4), c = i % (d4 * 4);
-                s.k[r][c] = c < p.d && s.line[r] >= 0 ? Elem<T>::load(kt + s.line[r] * p.d + c) : 0.f;
-            }
-            for (int i = tid; i < SR_KEYS * p.dv; i += SR_THREADS) {
-                const int r = i / p.dv, c = i % p.dv;
-                s.v[r][c] = s.line[r] >= 0 ? Elem<T>::load(vt + s.line[r] * p.dv + c) : 0.f;
-            }
+            // A warp four lines, four components a lane and load (eight loads of keys, then eight of values, before the first is laid down).
+            sr_lines<T, SR_DIM + 4>(&s.k[0][0], kt, s.line, p.d, p.d % 4 == 0);
+            sr_lines<T, SR_DIM>(&s.v[0][0], vt, s.line, p.dv, p.dv % 4 == 0);
             __syncthreads();
             float x[SR_KEYS / 8];
             float top = -INFINITY;
@@ -168,6 +192,8 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
 constexpr int SJ_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(SJ_WARPS * 32) shared_combine_kernel(const SharedParams p, int tile_pairs) {
+    dependent_wait();
+    dependent_trigger();
     const int pair = blockIdx.x * SJ_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (pair >= p.rows * p.hq) return;
     const int r = pair / p.hq, head = pair % p.hq;
@@ -254,7 +280,7 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_combine_kernel(const Sha
     }
 }
 template <typename T> static int launch_combine(const SharedParams& p, int tile_pairs, cudaStream_t s) {
-    shared_combine_kernel<T><<<(p.rows * p.hq + SJ_WARPS - 1) / SJ_WARPS, SJ_WARPS * 32, 0, s>>>(p, tile_pairs);
+    launch_dependent_if(p.rows <= DEPENDENT_ROWS, shared_combine_kernel<T>, dim3((p.rows * p.hq + SJ_WARPS - 1) / SJ_WARPS), dim3(SJ_WARPS * 32), 0, s, p, tile_pairs);
     return check_launch("shared_attention");
 }
 
@@ -283,6 +309,12 @@ static SharedScratch shared_scratch(int rows, int hq, int hkv, int d) {         
     const int blocks = shared_blocks();
     return SharedScratch{shared_tile_places(rows, hq, blocks, 128), shared_row_places(rows, hq, hkv, blocks * shared_own_workers(d))};
 }
+// What a unit of a tile costs a multiprocessor, counted in units of 16 positions of a row.
+static float shared_tile_cost(int d) {
+    if (getenv("KB_SH_COST")) return (float)atof(getenv("KB_SH_COST"));
+    return d == 256 ? 14.f : 20.f;
+}
+
 // Floats of scratch memory: the tiles' pieces, the rows' pieces, then the cut.
 extern "C" long long kb_shared_attention_scratch_floats(int rows, int hq, int hkv, int d, int dv) {
     if (rows <= 0 || rows > SH_ROWS || hq <= 0 || hkv <= 0 || hq % hkv || dv <= 0) return 0;
@@ -319,13 +351,16 @@ extern "C" int kb_shared_attention(void* out, const void* q, const void* k_table
     p.tile_pieces = scratch;
     p.row_pieces = scratch + x.tile_places * SH_PIECE(dv);
     p.cut = reinterpret_cast<int*>(p.row_pieces + x.row_places * SH_PIECE(dv));
+    KB_REQUIRE((((uintptr_t)q | (uintptr_t)k_table | (uintptr_t)v_table | (uintptr_t)out) & 15) == 0, "shared_attention: operands must be 16-byte aligned");
     if (shared_on_tensor_cores(dtype, hq, hkv, d, dv, page_size)) {
-        KB_REQUIRE((((uintptr_t)q | (uintptr_t)k_table | (uintptr_t)v_table) & 15) == 0, "shared_attention: operands must be 16-byte aligned");
         const unsigned long long lines = (unsigned long long)n_pages * hkv * page_size;
         KB_REQUIRE(lines <= 0x7fffffffull, "shared_attention: tables of %llu lines", lines);
         CUtensorMap mk, mv;
         if (int e = encode_map_bf16(&mk, k_table, lines, d, d, 16)) return e;
         if (int e = encode_map_bf16(&mv, v_table, lines, d, d, 16)) return e;
+        // In a step of few rows the kernel over rows starts while the one over tiles runs, and takes the multiprocessors that one leaves.
+        const bool side = may_chain(p.rows <= DEPENDENT_ROWS);
+        p.tile_cost = side ? shared_tile_cost(d) : 0.f;
         if (int e = launch_shared_tiles(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
         CUtensorMap ok, ov;                              // the same in boxes of all of a line's chunks
         if (int e = encode_map_bf16_chunks(&ok, k_table, lines, d, 16)) return e;

@@ -39,6 +39,7 @@ struct SharedParams {
     int* cut;                  // what the kernels leave for the one that joins: see SH_CUT_*
     int rows, hq, hkv, d, dv, page_size, table_width, n_pages, window;
     float scale, cap;
+    float tile_cost;           // > 0: the kernels over tiles and over rows run side by side; what a tile's unit costs, counted in a row's units
 };
 
 // The cut as the joining kernel reads it, in p.cut: the tile of each row (-1: none), for each tile {first row, rows, rows in tiles before}, and for tiles
@@ -49,7 +50,7 @@ constexpr int SH_CUT_INTS = SH_CUT_COUNTS + 3;
 
 // A block's copy of the cut into tiles.
 struct SharedTiles {
-    int tiles;
+    int tiles, row_units;                    // tiles, and units of 16 positions that the rows read by themselves
     int row_tile[SH_ROWS];                   // a row's tile, -1 where it shares nothing
     int length[SH_ROWS], id[SH_ROWS], first[SH_ROWS];    // by row: positions it shares, with whom, the first it sees
     int row0[SH_ROWS], n[SH_ROWS], before[SH_ROWS + 1];      // by tile
@@ -119,11 +120,15 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
             tiles += __popc(opened);
             if (who) run = base + 31 - __clz(who);
         }
-        if (lane == 0) c.tiles = tiles;
+        if (lane == 0) { c.tiles = tiles; c.row_units = 0; }
     }
     __syncthreads();
     for (int r = tid; r < p.rows; r += nt) {
         const int t = c.row_tile[r];
+        if (p.tile_cost > 0.f) {
+            int lo, hi;
+            atomicAdd(&c.row_units, shared_own(p, r, 16, lo, hi));
+        }
         if (t < 0) continue;
         atomicMin(&c.row0[t], r);
         atomicAdd(&c.before[t], 1);
@@ -149,15 +154,35 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
     __syncthreads();
 }
 
-// The cut into rows: upto[r] = units before row r. By the whole block.
-__device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int keys) {
-    for (int r = threadIdx.x; r < p.rows; r += blockDim.x) {
-        int lo, hi;
-        upto[r] = shared_own(p, r, keys, lo, hi);
-    }
+// The cut into rows: upto[r] = units before row r, which reads positions [lo[r], hi[r]) by itself. By the whole block.
+__device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int* lo, int* hi, int keys) {
+    for (int r = threadIdx.x; r < p.rows; r += blockDim.x) upto[r] = shared_own(p, r, keys, lo[r], hi[r]);
     __syncthreads();
     if (threadIdx.x < 32) shared_totals(upto, p.rows);
     __syncthreads();
+}
+
+// The units of all tiles of one kv head as a rule that both kernels can follow has them: a tile's opening row stands for the tile. By one warp.
+__device__ __forceinline__ int shared_tile_units(const SharedParams& p, const int* length, const int* id, int rows_a_tile, int keys) {
+    const int lane = threadIdx.x & 31;
+    int run = 0, units = 0;
+    for (int base = 0; base < p.rows; base += 32) {
+        const int r = base + lane, n = r < p.rows ? length[r] : 0;
+        const bool starts = r < p.rows && (r == 0 || n == 0 || length[r - 1] != n || id[r - 1] != id[r]);
+        const unsigned who = __ballot_sync(0xffffffffu, starts), mine = who & (0xffffffffu >> (31 - lane));
+        const int begins = mine ? base + 31 - __clz(mine) : run;
+        if (n > 0 && (r - begins) % rows_a_tile == 0) units += max(0, n - shared_first(p, p.row_count[r]) + keys - 1) / keys;
+        if (who) run = base + 31 - __clz(who);
+    }
+    return __reduce_add_sync(0xffffffffu, units);
+}
+
+// Blocks over tiles where both kernels run side by side, of `blocks` in all: as many as the tiles' share of the work, and of the rest the rows get
+// one at least. `tile_units` and `row_units` of one kv head.
+__device__ __forceinline__ int shared_tile_blocks(const SharedParams& p, int tile_units, int row_units, int blocks) {
+    if (p.tile_cost <= 0.f || row_units == 0) return blocks;
+    const float tiles = p.tile_cost * (float)tile_units, all = tiles + (float)row_units;
+    return tile_units == 0 ? 0 : min(max((int)(tiles / all * (float)blocks + 0.5f), 1), blocks - 1);
 }
 
 // A worker's units, the items' one after the other and each item's kv head by kv head.

@@ -50,6 +50,19 @@ struct SharedScore {
 };
 
 int shared_own_workers(int d);                               // warps a block
+// Tensor memory, 32 lanes x 16 or 32 words; and out of 16 or 8.
+__device__ __forceinline__ void sh_ld(uint32_t taddr, uint32_t (&r)[32]) { at_ld32(taddr, r); }
+__device__ __forceinline__ void sh_ld(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void sh_st(uint32_t taddr, const uint32_t (&r)[16]) { at_st16(taddr, r); }
+__device__ __forceinline__ void sh_st(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
 // Two 32-bit values at a time.
 __device__ __forceinline__ unsigned long long sh_pair(uint32_t a, uint32_t b) {
     unsigned long long d;
@@ -74,40 +87,52 @@ __device__ __forceinline__ unsigned long long sh_fma2(unsigned long long a, unsi
     return d;
 }
 
-// Scores of a thread's N products in place, none of them masked, and their largest. Without a cap x scale; with one, where every product of the warp is
-// below 3/4 of it, cap tanh(x) by an odd polynomial of degree 9 fitted to tanh x / x on [0, 9/16] of x^2 (6e-7 of the value), two
-// values an instruction: the hardware's exponential, reciprocal and exponential again for each score are three of sixteen a clock and bound the
-// kernel; this leaves one.
-template <int N> __device__ __forceinline__ float sh_scores(uint32_t (&x)[N], const SharedScore& score) {
+__device__ __forceinline__ float sh_max_abs(float a, float b, float c) {
+    float d;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// A thread's N products divided by the cap (without one: as scores), in place; returns the largest magnitude.
+template <int N> __device__ __forceinline__ float sh_scale(uint32_t (&x)[N], const SharedScore& score) {
     const float first = score.cap ? score.u : score.in;
     const unsigned long long in = sh_pair(first, first);
-    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, fars[4] = {0.f, 0.f, 0.f, 0.f};        // four chains side by side
+    float far[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
         sh_split(sh_mul2(sh_pair(x[j], x[j + 1]), in), x[j], x[j + 1]);
-        tops[(j >> 1) & 3] = fmaxf(fmaxf(tops[(j >> 1) & 3], __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
+        far[(j >> 1) & 1] = sh_max_abs(far[(j >> 1) & 1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
     }
-    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    if (!score.cap) return top;
-#pragma unroll
-    for (int j = 0; j < N; j += 2) fars[(j >> 1) & 3] = fmaxf(fmaxf(fars[(j >> 1) & 3], fabsf(__uint_as_float(x[j]))), fabsf(__uint_as_float(x[j + 1])));
-    const float far = fmaxf(fmaxf(fars[0], fars[1]), fmaxf(fars[2], fars[3]));
-    // (a NaN is passed over by fmaxf and goes through the polynomial as well as through the other)
-    if (!__all_sync(0xffffffffu, far <= 0.75f)) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = __float_as_uint(score.of_u(__uint_as_float(x[j])));
-        return score.of_u(top);
-    }
-    constexpr float C0 = 0.999999463558197f, C1 = -0.3332834839820862f, C2 = 0.13259831070899963f, C3 = -0.05008019134402275f, C4 = 0.012950727716088295f;
-    const float o = score.out;
-    const unsigned long long c0 = sh_pair(C0 * o, C0 * o), c1 = sh_pair(C1 * o, C1 * o), c2 = sh_pair(C2 * o, C2 * o), c3 = sh_pair(C3 * o, C3 * o), c4 = sh_pair(C4 * o, C4 * o);
+    return fmaxf(far[0], far[1]);
+}
+// The weights 2^(score - base) of what `sh_scale` left, rounded, two to a word; returns the sum of the rounded ones. `SMOOTH`: every product is
+// below SH_NEAR of the cap, and cap tanh(x) is an odd polynomial of degree 7 fitted to tanh x / x (1.2e-6 of the value), two values an
+// instruction. The hardware makes four exponentials or reciprocals a clock and scheduler: with the polynomial a weight takes one, not three, and
+// the polynomial's products run beside it.
+constexpr float SH_NEAR = 0.55f;
+template <int N, typename F> __device__ __forceinline__ float sh_weights(const uint32_t (&x)[N], uint32_t (&out)[N / 2], float base, F score_of) {
+    const unsigned long long less = sh_pair(-base, -base);
+    unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-        const unsigned long long u = sh_pair(x[j], x[j + 1]), z = sh_mul2(u, u);
-        sh_split(sh_mul2(u, sh_fma2(sh_fma2(sh_fma2(sh_fma2(c4, z, c3), z, c2), z, c1), z, c0)), x[j], x[j + 1]);
+        uint32_t a, b;
+        sh_split(score_of(sh_pair(x[j], x[j + 1]), less), a, b);
+        const uint32_t two = at_pack(at_exp2(__uint_as_float(a)), at_exp2(__uint_as_float(b)));
+        sums[(j >> 1) & 1] = sh_add2(sums[(j >> 1) & 1], sh_pair(two << 16, two & 0xffff0000u));
+        out[j >> 1] = two;
     }
-    const float z = top * top;
-    return top * fmaf(fmaf(fmaf(fmaf(C4 * o, z, C3 * o), z, C2 * o), z, C1 * o), z, C0 * o);
+    uint32_t la, lb;
+    sh_split(sh_add2(sums[0], sums[1]), la, lb);
+    return __uint_as_float(la) + __uint_as_float(lb);
+}
+template <int N> __device__ __forceinline__ float sh_weights_near(const uint32_t (&x)[N], uint32_t (&out)[N / 2], float base, const SharedScore& score) {
+    constexpr float C0 = 0.999998927116394f, C1 = -0.33321505784988403f, C2 = 0.13132257759571075f, C3 = -0.042718496173620224f;
+    const float o = score.out;
+    const unsigned long long c0 = sh_pair(C0 * o, C0 * o), c1 = sh_pair(C1 * o, C1 * o), c2 = sh_pair(C2 * o, C2 * o), c3 = sh_pair(C3 * o, C3 * o);
+    return sh_weights(x, out, base, [&](unsigned long long u, unsigned long long less) {
+        const unsigned long long z = sh_mul2(u, u);
+        return sh_fma2(u, sh_fma2(sh_fma2(sh_fma2(c3, z, c2), z, c1), z, c0), less);
+    });
 }
 
 int launch_shared_tiles(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s);

@@ -20,7 +20,7 @@ template <int D> struct OwnCfg {
     static constexpr int BOXES = D / 64;
     static constexpr int STAGE = 2 * BOXES * 2048;                       // bytes: keys, then values
     static constexpr int PIPES = WARPS * STAGES * STAGE;
-    static constexpr int SMEM = 1024 + PIPES + WARPS * STAGES * 8 + (SH_ROWS + 1) * 4;
+    static constexpr int SMEM = 1024 + PIPES + WARPS * STAGES * 8 + (5 * SH_ROWS + 4) * 4;
     static_assert(SMEM <= 232448, "more shared memory than a block can have");
 };
 
@@ -33,6 +33,11 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)so_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* all_bars = reinterpret_cast<uint64_t*>(smem + C::PIPES);
     int* upto = reinterpret_cast<int*>(all_bars + C::WARPS * C::STAGES);
+    int* row_lo = upto + SH_ROWS + 1;
+    int* row_hi = row_lo + SH_ROWS;
+    int* length = row_hi + SH_ROWS;                          // what rows share, and with whom
+    int* id = length + SH_ROWS;
+    int* tile_units = id + SH_ROWS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* pipe = smem + warp * C::STAGES * C::STAGE;
     uint64_t* bars = all_bars + warp * C::STAGES;
@@ -40,9 +45,19 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
         for (int s = 0; s < C::STAGES; ++s) at_mbar_init(bars + s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    shared_cut_rows(p, upto, 16);                            // ends with a barrier
     const int group = p.hq / p.hkv;
-    const SharedRange range = shared_range(blockIdx.x * C::WARPS + warp, gridDim.x * C::WARPS, upto[p.rows], p.hkv);
+    int blocks = gridDim.x;
+    if (p.tile_cost > 0.f) {
+        for (int r = threadIdx.x; r < p.rows; r += blockDim.x) { length[r] = shared_length(p, r); id[r] = p.share_id[r]; }
+    }
+    shared_cut_rows(p, upto, row_lo, row_hi, 16);            // ends with a barrier
+    if (p.tile_cost > 0.f) {                                 // the tiles' kernel runs beside this one and has its share of the multiprocessors
+        if (warp == 0) *tile_units = shared_tile_units(p, length, id, 128 / group, D == 256 ? 64 : 128);
+        __syncthreads();
+        const int theirs = shared_tile_blocks(p, *tile_units, upto[p.rows], gridDim.x);
+        if (theirs < blocks) blocks -= theirs;
+    }
+    const SharedRange range = shared_range(blockIdx.x * C::WARPS + warp, blocks * C::WARPS, upto[p.rows], p.hkv);
     if (blockIdx.x == 0) shared_leave_rows(p, upto, range.workers);
     const bf16* q = static_cast<const bf16*>(p.q);
 
@@ -59,8 +74,7 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
             const int in = ask - upto[a_row] * p.hkv;
             a_kvh = in / a_units;
             a_in = in % a_units;
-            int hi;
-            shared_own(p, a_row, 16, a_lo, hi);
+            a_lo = row_lo[a_row];
             a_j = a_lo / 16 * 16;
             fresh = true;
         }
@@ -88,6 +102,11 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
         ++ask;
         ++a_in;
     };
+    if (range.begin < range.end) {                           // the first item's queries are on their way before its keys crowd the memory
+        const int r = shared_item(upto, p.rows, p.hkv, range.begin), kvh = (range.begin - upto[r] * p.hkv) / (upto[r + 1] - upto[r]);
+        const bf16* first = q + ((size_t)r * p.hq + kvh * group) * D;
+        for (int i = lane * 64; i < group * D; i += 32 * 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(first + i));
+    }
     for (int s = 0; s < C::STAGES; ++s) next_unit(s);
 
     const SharedScore score(p.scale, p.cap);
@@ -97,8 +116,7 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
         const int r = shared_item(upto, p.rows, p.hkv, u);
         const int units = upto[r + 1] - upto[r], in = u - upto[r] * p.hkv;
         const int kvh = in / units, first = in % units, n = min(units - first, range.end - u);
-        int lo, hi;
-        shared_own(p, r, 16, lo, hi);
+        const int lo = row_lo[r], hi = row_hi[r];
         u += n;
         uint32_t bq[KK][NB][2];
 #pragma unroll
@@ -227,6 +245,7 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
                 if (g == 0) { piece[D] = m[nb][h] * 0.6931471805599453f; piece[D + 1] = l[nb][h]; }
             }
     }
+    dependent_wait();                                        // this grid ends behind the tiles' kernel: whoever waits for it has both
     if (failed) {
         if (lane == 0) atomicExch(&g_shared_attention_error, 1);
         // what was asked for may still come (a wait that ran out is not repeated for ever)
@@ -237,7 +256,7 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
 template <int D, int NB> static int launch_own(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(shared_own_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnCfg<D>::SMEM);
     KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", OwnCfg<D>::SMEM, cudaGetErrorString(e));
-    shared_own_kernel<D, NB><<<blocks, OwnCfg<D>::WARPS * 32, OwnCfg<D>::SMEM, s>>>(p, mk, mv);
+    launch_dependent_if(p.tile_cost > 0.f, shared_own_kernel<D, NB>, dim3(blocks), dim3(OwnCfg<D>::WARPS * 32), OwnCfg<D>::SMEM, s, p, mk, mv);
     return check_launch("shared_attention");
 }
 

@@ -4,21 +4,26 @@
 // belong to:
 //   S = Q K^T   tcgen05.mma, Q [128 x D] and the keys [KEYS x D] K-major in shared memory (128-byte swizzle), S float32 in one of three
 //               TMEM buffers;
-//   P = 2^(score - m) by eight warps, two to each quarter of the pairs, half of the unit's positions each; written over S as bfloat16;
+//   P = 2^(score - m) by sixteen warps, four to each quarter of the pairs, a quarter of the unit's positions each (with eight warps the
+//               multiprocessor issued 1.7 instructions a clock); written over S as bfloat16;
 //   O += P V    tcgen05.mma, P from TMEM, the values [KEYS x D] an MN-major operand; O float32 stays in TMEM until the block's part of
 //               the tile ends, when it goes out as a piece.
-// m is a pair's largest score so far; where a unit raises it the quarter's warps wait for the product before, scale O in TMEM and go on. The
+// m is a score of the pair that none seen so far passes by more than 2^ST_LAG; where a unit does, the quarter's warps wait for the product before,
+// scale O in TMEM and go on. (With m the largest so far some of a warp's 32 pairs raise it in nearly every unit of the first thousands of
+// positions, and scaling O of 256 components takes longer than all the rest of a unit. The weights are rounded relative to themselves, so
+// larger ones lose nothing; only the largest of a pair, no longer exactly 1, is rounded as well.) The
 // next tile's queries are laid out as soon as the last score product of this one is complete, so its products run while this one's O is read out.
 //
-// Warp 0 brings keys, 11 values (TMA, 16 positions x 64 elements a box, a box a lane); 1 allocates TMEM and issues the score products, 10
-// the others; 2 to 9 are the softmax's. Every wait gives up after about a second, raises a flag and the block still frees its TMEM.
+// Warp 0 brings keys, 19 values (TMA, 16 positions x 64 elements a box, a box a lane); 1 allocates TMEM and issues the score products, 18
+// the others; 2 to 17 are the softmax's. Every wait gives up after about a second, raises a flag and the block still frees its TMEM.
 #include "attention_shared_bf16.cuh"
 #include "tensor_map.cuh"
 
 namespace kb {
 
-constexpr int ST_PAIRS = 128, ST_THREADS = 384, ST_S = 3;
-constexpr int ST_WARP_PV = 10, ST_WARP_V = 11;
+constexpr int ST_PAIRS = 128, ST_SOFT = 16, ST_THREADS = (ST_SOFT + 4) * 32, ST_S = 3;
+constexpr int ST_WARP_PV = ST_SOFT + 2, ST_WARP_V = ST_SOFT + 3;
+constexpr float ST_LAG = 8.f;
 
 template <int D> struct TilesCfg {
     static constexpr int KEYS = D == 256 ? 64 : 128;
@@ -27,7 +32,7 @@ template <int D> struct TilesCfg {
     static constexpr int RING = D == 64 ? 4 : 2;             // units of keys, and of values
     static constexpr int COL_S = D, TMEM_COLS = 512;
     static constexpr int BARS = 4 * RING + 3 * ST_S + 2;
-    static constexpr int SMEM = 1024 + Q_BYTES + 2 * RING * KV_BYTES + BARS * 8 + 8 + 2 * 2 * ST_PAIRS * 4 + (int)sizeof(SharedTiles);
+    static constexpr int SMEM = 1024 + Q_BYTES + 2 * RING * KV_BYTES + BARS * 8 + 8 + 2 * 4 * ST_PAIRS * 4 + (int)sizeof(SharedTiles);
     static_assert(D + ST_S * KEYS <= TMEM_COLS, "O and the S buffers outgrew TMEM");
     static_assert(SMEM <= 232448, "more shared memory than a block can have");
 };
@@ -64,7 +69,7 @@ template <int D>
 __global__ void __launch_bounds__(ST_THREADS, 1)
 shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using C = TilesCfg<D>;
-    constexpr int KEYS = C::KEYS, CH = C::CH, RING = C::RING, HALF = KEYS / 2, SB = ST_S;
+    constexpr int KEYS = C::KEYS, CH = C::CH, RING = C::RING, PART = KEYS / 4, SB = ST_S;
     extern __shared__ unsigned char st_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)st_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* q_smem = smem;                                // [chunk][128 pairs][128 bytes]
@@ -75,24 +80,26 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
     uint64_t* v_full = k_empty + RING;
     uint64_t* v_empty = v_full + RING;
     uint64_t* s_full = v_empty + RING;                           // [SB] S complete
-    uint64_t* p_full = s_full + SB;                              // [SB] P written, eight warps arrive
+    uint64_t* p_full = s_full + SB;                              // [SB] P written, the softmax's warps arrive
     uint64_t* s_free = p_full + SB;                              // [SB] the product that read P is complete
-    uint64_t* q_full = s_free + SB;                              // a part's queries are laid out, eight warps arrive
+    uint64_t* q_full = s_free + SB;                              // a part's queries are laid out, the softmax's warps arrive
     uint64_t* o_full = q_full + 1;                               // a part's products are complete
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
-    float* exchange = reinterpret_cast<float*>(tmem_slot + 2);   // [2][2][128]: a unit's maxima by (turn, half, pair)
-    SharedTiles& cut = *reinterpret_cast<SharedTiles*>(exchange + 2 * 2 * ST_PAIRS);
+    float* exchange = reinterpret_cast<float*>(tmem_slot + 2);   // [2][4][128]: a unit's maxima by (turn, quarter of its positions, pair)
+    SharedTiles& cut = *reinterpret_cast<SharedTiles*>(exchange + 2 * 4 * ST_PAIRS);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = p.hq / p.hkv;
+    dependent_wait();                                            // queries, keys and counts may be the work of the kernel before
+    dependent_trigger();                                         // the kernel over rows may begin: it waits for nothing else
     shared_cut_tiles(p, cut, ST_PAIRS / group, KEYS);            // ends with a barrier
-    const SharedRange range = shared_range(blockIdx.x, gridDim.x, cut.upto[cut.tiles], p.hkv);
+    const SharedRange range = shared_range(blockIdx.x, shared_tile_blocks(p, cut.upto[cut.tiles], cut.row_units, gridDim.x), cut.upto[cut.tiles], p.hkv);
     if (blockIdx.x == 0) shared_leave_tiles(p, cut, range.workers);
     if (range.begin == range.end) return;                        // nothing for this block: before anything is allocated
     if (tid == 0) {
         for (int s = 0; s < RING; ++s) { at_mbar_init(k_full + s, 1); at_mbar_init(k_empty + s, 1); at_mbar_init(v_full + s, 1); at_mbar_init(v_empty + s, 1); }
-        for (int b = 0; b < SB; ++b) { at_mbar_init(s_full + b, 1); at_mbar_init(p_full + b, 8); at_mbar_init(s_free + b, 1); }
-        at_mbar_init(q_full, 8);
+        for (int b = 0; b < SB; ++b) { at_mbar_init(s_full + b, 1); at_mbar_init(p_full + b, ST_SOFT); at_mbar_init(s_free + b, 1); }
+        at_mbar_init(q_full, ST_SOFT);
         at_mbar_init(o_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -217,8 +224,8 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
             if (!failed && one) at_commit(o_full);
         }
     } else {
-        // ---------------------------------------------------------------- queries, softmax and pieces, half a pair's positions a thread
-        const int quarter = warp & 3, half = (warp - 2) >> 2, pair = quarter * 32 + lane, st = tid - 64;
+        // ---------------------------------------------------------------- queries, softmax and pieces, a quarter of a pair's positions a thread
+        const int quarter = warp & 3, share = (warp - 2) >> 2, pair = quarter * 32 + lane, st = tid - 64;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const SharedScore score(p.scale, p.cap);
         const bf16* q = static_cast<const bf16*>(p.q);
@@ -227,7 +234,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
         const uint32_t by_group = (65536u + (uint32_t)group - 1u) / (uint32_t)group;          // r / group = r by_group >> 16 for r < 128
         auto lay_queries = [&](const TilePart& w) {
             const int pairs = w.n * group;
-            constexpr int ITER = ST_PAIRS * CH * 8 / 256, DEEP = ITER < 8 ? ITER : 8;          // pieces a thread; asked for eight at a time
+            constexpr int ITER = ST_PAIRS * CH * 8 / (ST_SOFT * 32), DEEP = ITER < 8 ? ITER : 8;          // pieces a thread; asked for eight at a time
             const int j = st & 7, ch = (st >> 3) % CH, r0 = (st >> 3) / CH;
             const bf16* src = q + ((size_t)w.row0 * p.hq + w.kvh * group) * D + ch * 64 + j * 8;
             unsigned char* dst = q_smem + ch * (ST_PAIRS * 128);
@@ -235,13 +242,13 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                 uint4 x[DEEP];
 #pragma unroll
                 for (int k = 0; k < DEEP; ++k) {
-                    const int r = r0 + (base + k) * (32 / CH);
+                    const int r = r0 + (base + k) * (ST_SOFT * 4 / CH);
                     const uint32_t row = (uint32_t)r * by_group >> 16;
                     x[k] = r < pairs ? *reinterpret_cast<const uint4*>(src + (size_t)(row * p.hq + (r - row * group)) * D) : make_uint4(0u, 0u, 0u, 0u);
                 }
 #pragma unroll
                 for (int k = 0; k < DEEP; ++k) {
-                    const int r = r0 + (base + k) * (32 / CH);
+                    const int r = r0 + (base + k) * (ST_SOFT * 4 / CH);
                     if (r < pairs) *reinterpret_cast<uint4*>(dst + (size_t)r * 128 + ((j ^ (r & 7)) << 4)) = x[k];
                 }
             }
@@ -249,7 +256,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
             __syncwarp();
             if (lane == 0) at_mbar_arrive(q_full);
         };
-        int c = 0, part = 0;
+        int c = 0, part = 0, turns = 0;
         TilePart w = st_part(p, cut, range.begin, range.end);
         lay_queries(w);
         for (int u = range.begin; u < range.end; ++part) {
@@ -261,46 +268,57 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
             const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
             float ref = -INFINITY, l = 0.f;
             for (int i = 0; i < w.units; ++i, ++c) {
-                const int b = c % SB, j0 = (w.lo / KEYS + w.first + i) * KEYS + half * HALF;
+                const int b = c % SB, j0 = (w.lo / KEYS + w.first + i) * KEYS + share * PART;
                 // a wait that ran out is not repeated, but the walk goes on: the quarter's warps meet at every unit's barrier
                 if (!failed && !__all_sync(0xffffffffu, at_mbar_wait(s_full + b, (uint32_t)(c / SB) & 1u))) failed = true;
                 at_fence_after();
                 if (!idle) {
-                    uint32_t x[HALF / 32][32];
-#pragma unroll
-                    for (int k = 0; k < HALF / 32; ++k) at_ld32(lanes + (uint32_t)(C::COL_S + b * KEYS + half * HALF + k * 32), x[k]);
+                    uint32_t x[PART];
+                    sh_ld(lanes + (uint32_t)(C::COL_S + b * KEYS + share * PART), x);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    float top = -INFINITY;
-                    if (j0 < lo_max || j0 + HALF > hi_min) {     // some pair does not see all of it: the same for the whole warp
+                    const bool edge = j0 < lo_max || j0 + PART > hi_min;         // some pair does not see all of it: the same for the whole warp
+                    float top = -INFINITY, far = 0.f;
+                    if (edge) {
 #pragma unroll
-                        for (int k = 0; k < HALF / 32; ++k)
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                float v = score(__uint_as_float(x[k][j]));
-                                if (j0 + k * 32 + j < lo || j0 + k * 32 + j >= hi) v = -INFINITY;
-                                x[k][j] = __float_as_uint(v);
-                                top = fmaxf(top, v);
-                            }
+                        for (int j = 0; j < PART; ++j) {
+                            float v = score(__uint_as_float(x[j]));
+                            if (j0 + j < lo || j0 + j >= hi) v = -INFINITY;
+                            x[j] = __float_as_uint(v);
+                            top = fmaxf(top, v);
+                        }
                     } else {
-#pragma unroll
-                        for (int k = 0; k < HALF / 32; ++k) top = fmaxf(top, sh_scores(x[k], score));
+                        far = sh_scale(x, score);
+                        top = score.cap ? score.of_u(far) : far;     // no less than the largest score
                     }
-                    // The quarter's two warps tell each other their halves' maxima; behind this barrier both have their scores in registers,
-                    // so P may be written over them. Two sets of places in turn.
-                    float* turn = exchange + (c & 1) * 2 * ST_PAIRS;
-                    turn[half * ST_PAIRS + pair] = top;
-                    asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
-                    top = fmaxf(top, turn[(half ^ 1) * ST_PAIRS + pair]);
-                    const bool moves = top > ref;
+                    // The quarter's four warps tell each other their largest scores, or bounds of them; behind this barrier all have their scores in
+                    // registers, so P may be written over them. Sets of places in turn. Only where a bound passes m by too much the scores
+                    // themselves are looked through: the same for the four warps.
+                    float* turn = exchange + (turns++ & 1) * 4 * ST_PAIRS + pair;
+                    turn[share * ST_PAIRS] = top;
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + quarter) : "memory");
+                    float most = fmaxf(fmaxf(turn[0], turn[ST_PAIRS]), fmaxf(turn[2 * ST_PAIRS], turn[3 * ST_PAIRS]));
+                    if (__any_sync(0xffffffffu, most > ref + ST_LAG)) {
+                        if (!edge) {
+                            top = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < PART; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+                            if (score.cap) top = score.of_u(top);
+                        }
+                        turn = exchange + (turns++ & 1) * 4 * ST_PAIRS + pair;
+                        turn[share * ST_PAIRS] = top;
+                        asm volatile("bar.sync %0, 128;" ::"r"(2 + quarter) : "memory");
+                        most = fmaxf(fmaxf(turn[0], turn[ST_PAIRS]), fmaxf(turn[2 * ST_PAIRS], turn[3 * ST_PAIRS]));
+                    }
+                    const bool moves = most > ref + ST_LAG;          // (anything above -inf, to begin with)
                     const float was = ref;
-                    if (moves) ref = top;
+                    if (moves) ref = most;
                     const float fade = moves ? (was == -INFINITY ? 0.f : at_exp2(was - ref)) : 1.f;
                     l *= fade;
                     if (i > 0 && __any_sync(0xffffffffu, moves && was != -INFINITY)) {
                         const int before = c - 1;
                         if (!failed && !__all_sync(0xffffffffu, at_mbar_wait(s_free + before % SB, (uint32_t)(before / SB) & 1u))) failed = true;
                         at_fence_after();
-                        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
+                        for (int c0 = share * 32; c0 < D; c0 += 128) {
                             uint32_t o[32];
                             __syncwarp();
                             at_ld32(lanes + (uint32_t)c0, o);
@@ -312,24 +330,17 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
                     const float base = ref == -INFINITY ? 0.f : ref;
-                    const unsigned long long less = sh_pair(-base, -base);
-                    unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};
-                    uint32_t pr[HALF / 2];
+                    uint32_t pr[PART / 2];
+                    if (!edge && score.cap && __all_sync(0xffffffffu, far <= SH_NEAR)) {
+                        l += sh_weights_near(x, pr, base, score);
+                    } else {
+                        if (!edge && score.cap) {
 #pragma unroll
-                    for (int k = 0; k < HALF / 32; ++k)
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            uint32_t a, c2;
-                            sh_split(sh_add2(sh_pair(x[k][j], x[k][j + 1]), less), a, c2);
-                            const uint32_t two = at_pack(at_exp2(__uint_as_float(a)), at_exp2(__uint_as_float(c2)));
-                            sums[(j >> 1) & 3] = sh_add2(sums[(j >> 1) & 3], sh_pair(two << 16, two & 0xffff0000u));
-                            pr[k * 16 + (j >> 1)] = two;
+                            for (int j = 0; j < PART; ++j) x[j] = __float_as_uint(score.of_u(__uint_as_float(x[j])));
                         }
-                    uint32_t la, lb;
-                    sh_split(sh_add2(sh_add2(sums[0], sums[1]), sh_add2(sums[2], sums[3])), la, lb);
-                    l += __uint_as_float(la) + __uint_as_float(lb);
-                    if constexpr (HALF == 64) at_st32(lanes + (uint32_t)(C::COL_S + b * KEYS + half * 32), pr);
-                    else at_st16(lanes + (uint32_t)(C::COL_S + b * KEYS + half * 16), pr);
+                        l += sh_weights(x, pr, base, [](unsigned long long v, unsigned long long less) { return sh_add2(v, less); });
+                    }
+                    sh_st(lanes + (uint32_t)(C::COL_S + b * KEYS + share * (PART / 2)), pr);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 at_fence_before();
@@ -343,12 +354,12 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                 lay_queries(w);
             }
             if (!idle) {
-                // the pair's sum over both halves, through shared memory
-                float* turn = exchange + (c & 1) * 2 * ST_PAIRS;
-                turn[half * ST_PAIRS + pair] = l;
-                asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
-                l += turn[(half ^ 1) * ST_PAIRS + pair];
-                asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
+                // the pair's sum over its four shares, through shared memory
+                float* turn = exchange + (turns++ & 1) * 4 * ST_PAIRS + pair;
+                turn[share * ST_PAIRS] = l;
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + quarter) : "memory");
+                l = (turn[0] + turn[ST_PAIRS]) + (turn[2 * ST_PAIRS] + turn[3 * ST_PAIRS]);
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + quarter) : "memory");
             }
             if (!failed && !__all_sync(0xffffffffu, at_mbar_wait(o_full, (uint32_t)part & 1u))) failed = true;
             if (!failed && !idle) {
@@ -356,7 +367,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                 // 32 pairs x 32 components a time, turned around in registers: a pair's components leave side by side, a line a store.
                 float* pieces = p.tile_pieces + (mine.place + quarter * 32) * SH_PIECE(D);
                 const int here = min(32, mine.n * group - quarter * 32);
-                for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
+                for (int c0 = share * 32; c0 < D; c0 += 128) {
                     uint32_t o[32];
                     __syncwarp();
                     at_ld32(lanes + (uint32_t)c0, o);
@@ -366,7 +377,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                     for (int j = 0; j < 32; ++j)
                         if (j < here) pieces[(size_t)j * SH_PIECE(D) + c0 + lane] = __uint_as_float(o[j]);
                 }
-                if (own && half == 0)
+                if (own && share == 0)
                     *reinterpret_cast<float2*>(pieces + (size_t)lane * SH_PIECE(D) + D) = make_float2(ref == -INFINITY ? -INFINITY : ref * 0.6931471805599453f, l);
             }
             at_fence_before();
@@ -384,7 +395,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
 template <int D> static int launch_tiles(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(shared_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesCfg<D>::SMEM);
     KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", TilesCfg<D>::SMEM, cudaGetErrorString(e));
-    shared_tiles_kernel<D><<<blocks, ST_THREADS, TilesCfg<D>::SMEM, s>>>(p, mk, mv);
+    launch_dependent_if(p.rows <= DEPENDENT_ROWS, shared_tiles_kernel<D>, dim3(blocks), dim3(ST_THREADS), TilesCfg<D>::SMEM, s, p, mk, mv);
     return check_launch("shared_attention");
 }
 

@@ -35,6 +35,7 @@ int multiprocessors();                   // the current device's (148 where ther
 // overlap with one another and with no kernel of a prompt.
 constexpr int DEPENDENT_ROWS = 64;
 bool chains(bool dependent);             // whether a launch that may be a dependent is one (and counts it)
+bool may_chain(bool dependent);          // the same without counting
 template <typename... KArgs, typename... Args>
 inline void launch_dependent_if(bool dependent, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
