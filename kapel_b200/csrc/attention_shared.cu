@@ -1,7 +1,7 @@
 // Attention of single tokens over shared and own pages (see attention_shared.cuh for the cut), for any element type and head size up
 // to 256; and the kernel that joins the pieces.
 //
-// A block of 256 threads walks its units of 32 positions. Eight threads have one (row, head) pair of the 32 that a tile takes: each
+// A block of 256 threads walks its units of 32 positions, lines padded with zeros to 64, 128 or 256 components. Eight threads have one (row, head) pair of the 32 that a tile takes: each
 // computes every eighth position's score out of keys and queries in shared memory, and keeps every eighth group of four components of the
 // sum in registers. All arithmetic is 32-bit. Where some row of the tile does not see all of a unit (its window begins there, its
 // positions end there) what a row does not see is left out of its sum, not multiplied by zero: it may be anything.
@@ -14,18 +14,18 @@ namespace kb {
 constexpr int SR_PAIRS = 32, SR_KEYS = 32, SR_THREADS = 256, SR_DIM = 256;
 static_assert(SR_PAIRS == SR_KEYS, "queries are laid out as lines are");
 
-template <typename T> struct SharedRowsSmem {
-    float q[SR_PAIRS][SR_DIM + 4];
-    float k[SR_KEYS][SR_DIM + 4];
-    float v[SR_KEYS][SR_DIM];
+template <int DIM> struct SharedRowsSmem {
+    float q[SR_PAIRS][DIM + 4];
+    float k[SR_KEYS][DIM + 4];
+    float v[SR_KEYS][DIM];
     long long line[SR_KEYS];               // a position's line of this kv head in the tables, -1 for none
     SharedTiles tiles;
     int upto[SH_ROWS + 1], lo[SH_ROWS], hi[SH_ROWS];       // units before a row, the positions it reads by itself
 };
 
-// SR_KEYS lines of `size` components into shared memory in 32 bits, zeros where a line is none and up to a multiple of four components.
-template <typename T, int STRIDE> __device__ __forceinline__ void sr_lines(float* to, const T* table, const long long* lines, int size, bool fours) {
-    constexpr int WARPS = SR_THREADS / 32, ROWS = SR_KEYS / WARPS, QUADS = SR_DIM / 128;
+// SR_KEYS lines of `size` components into shared memory in 32 bits, zeros where a line is none and from its last component up to DIM.
+template <typename T, int DIM, int STRIDE> __device__ __forceinline__ void sr_lines(float* to, const T* table, const long long* lines, int size, bool fours) {
+    constexpr int WARPS = SR_THREADS / 32, ROWS = SR_KEYS / WARPS, QUADS = (DIM + 127) / 128;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (fours) {
         float4 x[ROWS][QUADS];
@@ -42,19 +42,19 @@ template <typename T, int STRIDE> __device__ __forceinline__ void sr_lines(float
 #pragma unroll
             for (int k = 0; k < QUADS; ++k) {
                 const int c = 4 * (lane + 32 * k);
-                if (c < size) *reinterpret_cast<float4*>(to + (warp + i * WARPS) * STRIDE + c) = x[i][k];
+                if (c < DIM) *reinterpret_cast<float4*>(to + (warp + i * WARPS) * STRIDE + c) = x[i][k];
             }
     } else {
         for (int r = warp; r < SR_KEYS; r += WARPS)
-            for (int c = lane; c < (size + 3) / 4 * 4; c += 32)
+            for (int c = lane; c < DIM; c += 32)
                 to[r * STRIDE + c] = c < size && lines[r] >= 0 ? Elem<T>::load(table + lines[r] * size + c) : 0.f;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedParams p) {
+template <typename T, int DIM>
+__global__ void __launch_bounds__(SR_THREADS, 1) shared_rows_kernel(const SharedParams p) {
     extern __shared__ __align__(16) unsigned char sr_raw[];
-    SharedRowsSmem<T>& s = *reinterpret_cast<SharedRowsSmem<T>*>(sr_raw);
+    SharedRowsSmem<DIM>& s = *reinterpret_cast<SharedRowsSmem<DIM>*>(sr_raw);
     const int tid = threadIdx.x, pair = tid >> 3, sub = tid & 7, lane = tid & 31;
     const int group = p.hq / p.hkv, rows_a_tile = SR_PAIRS / group;
     const T* q = static_cast<const T*>(p.q);
@@ -67,7 +67,6 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
         shared_leave_tiles(p, s.tiles, over[0].workers);
         shared_leave_rows(p, s.upto, over[1].workers);
     }
-    const int d4 = (p.d + 3) / 4;
     for (int kind = 0; kind < 2; ++kind)                     // what is shared, then what each row reads by itself
     for (int u = over[kind].begin; u < over[kind].end;) {
         struct { int row0, n, looks, kvh, lo, hi, first_unit, n_units; } w;
@@ -93,13 +92,13 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
         __syncthreads();                                 // the part before is done with the queries
         if (tid < SR_KEYS) s.line[tid] = tid < pairs ? (long long)(w.row0 + tid / group) * p.hq + w.kvh * group + tid % group : -1;
         __syncthreads();
-        sr_lines<T, SR_DIM + 4>(&s.q[0][0], q, s.line, p.d, p.d % 4 == 0);
+        sr_lines<T, DIM, DIM + 4>(&s.q[0][0], q, s.line, p.d, p.d % 4 == 0);
         const int count = own ? min(p.row_count[row], w.hi) : 0;
         const int first = own ? max(shared_first(p, p.row_count[row]), w.lo) : 0;
         float m = -INFINITY, l = 0.f;
-        float4 acc[SR_DIM / 32];
+        float4 acc[DIM / 32];
 #pragma unroll
-        for (int j = 0; j < SR_DIM / 32; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < DIM / 32; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int t = 0; t < w.n_units; ++t) {
             const int j0 = (w.lo / SR_KEYS + w.first_unit + t) * SR_KEYS;
             __syncthreads();                             // the unit before is done with keys and values
@@ -114,22 +113,29 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
             }
             __syncthreads();
             // A warp four lines, four components a lane and load (eight loads of keys, then eight of values, before the first is laid down).
-            sr_lines<T, SR_DIM + 4>(&s.k[0][0], kt, s.line, p.d, p.d % 4 == 0);
-            sr_lines<T, SR_DIM>(&s.v[0][0], vt, s.line, p.dv, p.dv % 4 == 0);
+            sr_lines<T, DIM, DIM + 4>(&s.k[0][0], kt, s.line, p.d, p.d % 4 == 0);
+            sr_lines<T, DIM, DIM>(&s.v[0][0], vt, s.line, p.dv, p.dv % 4 == 0);
             __syncthreads();
             float x[SR_KEYS / 8];
             float top = -INFINITY;
             bool all = true;
 #pragma unroll
+            for (int i = 0; i < SR_KEYS / 8; ++i) x[i] = 0.f;
+            if (own) {
+#pragma unroll 8
+                for (int c = 0; c < DIM / 4; ++c) {
+                    const float4 a = *reinterpret_cast<const float4*>(&s.q[pair][4 * c]);
+#pragma unroll
+                    for (int i = 0; i < SR_KEYS / 8; ++i) {
+                        const float4 b = *reinterpret_cast<const float4*>(&s.k[sub + 8 * i][4 * c]);
+                        x[i] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, x[i]))));
+                    }
+                }
+            }
+#pragma unroll
             for (int i = 0; i < SR_KEYS / 8; ++i) {
                 const int j = sub + 8 * i;
-                float dot = 0.f;
-                if (own)
-                    for (int c = 0; c < d4; ++c) {
-                        const float4 a = *reinterpret_cast<const float4*>(&s.q[pair][4 * c]), b = *reinterpret_cast<const float4*>(&s.k[j][4 * c]);
-                        dot = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, dot))));
-                    }
-                dot *= p.scale;
+                float dot = x[i] * p.scale;
                 if (p.cap > 0.f) dot = p.cap * tanhf(dot / p.cap);
                 const bool sees = j0 + j >= first && j0 + j < count && s.line[j] >= 0;
                 all = all && sees;
@@ -151,31 +157,30 @@ __global__ void __launch_bounds__(SR_THREADS) shared_rows_kernel(const SharedPar
             for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l = l * fade + sum;
 #pragma unroll
-            for (int j = 0; j < SR_DIM / 32; ++j) { acc[j].x *= fade; acc[j].y *= fade; acc[j].z *= fade; acc[j].w *= fade; }
+            for (int j = 0; j < DIM / 32; ++j) { acc[j].x *= fade; acc[j].y *= fade; acc[j].z *= fade; acc[j].w *= fade; }
             const bool whole = __all_sync(0xffffffffu, all || !own);
 #pragma unroll
             for (int i = 0; i < SR_KEYS / 8; ++i)
 #pragma unroll
                 for (int b = 0; b < 8; ++b) {
                     const float e = __shfl_sync(0xffffffffu, x[i], (lane & 24) + b);
-                    const int j = 8 * i + b;
-                    if (!own || (!whole && e == 0.f)) continue;
+                    const float* v = &s.v[8 * i + b][4 * sub];
+                    if (whole || e != 0.f) {
 #pragma unroll
-                    for (int c = 0; c < SR_DIM / 32; ++c) {
-                        const int at = 32 * c + 4 * sub;
-                        if (at >= p.dv) break;
-                        const float4 v = *reinterpret_cast<const float4*>(&s.v[j][at]);
-                        acc[c].x = fmaf(e, v.x, acc[c].x);
-                        acc[c].y = fmaf(e, v.y, acc[c].y);
-                        acc[c].z = fmaf(e, v.z, acc[c].z);
-                        acc[c].w = fmaf(e, v.w, acc[c].w);
+                        for (int c = 0; c < DIM / 32; ++c) {
+                            const float4 y = *reinterpret_cast<const float4*>(v + 32 * c);
+                            acc[c].x = fmaf(e, y.x, acc[c].x);
+                            acc[c].y = fmaf(e, y.y, acc[c].y);
+                            acc[c].z = fmaf(e, y.z, acc[c].z);
+                            acc[c].w = fmaf(e, y.w, acc[c].w);
+                        }
                     }
                 }
         }
         if (own) {
             float* piece = pieces + (size_t)pair * SH_PIECE(p.dv);
 #pragma unroll
-            for (int c = 0; c < SR_DIM / 32; ++c) {
+            for (int c = 0; c < DIM / 32; ++c) {
                 const int at = 32 * c + 4 * sub;
                 if (at < p.dv) piece[at] = acc[c].x;
                 if (at + 1 < p.dv) piece[at + 1] = acc[c].y;
@@ -284,13 +289,17 @@ template <typename T> static int launch_combine(const SharedParams& p, int tile_
     return check_launch("shared_attention");
 }
 
-template <typename T> static int launch_shared_rows(const SharedParams& p, int blocks, cudaStream_t s) {
-    const int smem = (int)sizeof(SharedRowsSmem<T>);
-    const cudaError_t e = cudaFuncSetAttribute(shared_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    shared_rows_kernel<T><<<blocks, SR_THREADS, smem, s>>>(p);
+template <typename T, int DIM> static int launch_shared_rows(const SharedParams& p, int blocks, cudaStream_t s) {
+    const int smem = (int)sizeof(SharedRowsSmem<DIM>);
+    static unsigned long long done = 0;
+    if (int e = allow_shared_memory((const void*)shared_rows_kernel<T, DIM>, smem, &done)) return e;
+    shared_rows_kernel<T, DIM><<<blocks, SR_THREADS, smem, s>>>(p);
     if (int err = check_launch("shared_attention")) return err;
     return launch_combine<T>(p, SR_PAIRS, s);
+}
+template <typename T> static int launch_shared_rows(const SharedParams& p, int blocks, cudaStream_t s) {
+    const int most = p.d > p.dv ? p.d : p.dv;
+    return most <= 64 ? launch_shared_rows<T, 64>(p, blocks, s) : most <= 128 ? launch_shared_rows<T, 128>(p, blocks, s) : launch_shared_rows<T, 256>(p, blocks, s);
 }
 
 }  // namespace kb

@@ -254,8 +254,8 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
 }
 
 template <int D, int NB> static int launch_own(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(shared_own_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnCfg<D>::SMEM);
-    KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", OwnCfg<D>::SMEM, cudaGetErrorString(e));
+    static unsigned long long done = 0;
+    if (int e = allow_shared_memory((const void*)shared_own_kernel<D, NB>, OwnCfg<D>::SMEM, &done)) return e;
     launch_dependent_if(p.tile_cost > 0.f, shared_own_kernel<D, NB>, dim3(blocks), dim3(OwnCfg<D>::WARPS * 32), OwnCfg<D>::SMEM, s, p, mk, mv);
     return check_launch("shared_attention");
 }

@@ -393,8 +393,8 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
 }
 
 template <int D> static int launch_tiles(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(shared_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesCfg<D>::SMEM);
-    KB_REQUIRE(e == cudaSuccess, "shared_attention: cannot have %d bytes of shared memory: %s", TilesCfg<D>::SMEM, cudaGetErrorString(e));
+    static unsigned long long done = 0;
+    if (int e = allow_shared_memory((const void*)shared_tiles_kernel<D>, TilesCfg<D>::SMEM, &done)) return e;
     launch_dependent_if(p.rows <= DEPENDENT_ROWS, shared_tiles_kernel<D>, dim3(blocks), dim3(ST_THREADS), TilesCfg<D>::SMEM, s, p, mk, mv);
     return check_launch("shared_attention");
 }

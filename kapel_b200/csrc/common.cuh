@@ -59,6 +59,18 @@ __device__ __forceinline__ void dependent_wait() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void dependent_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
 
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once a device (`done`: one word a kernel, a bit a device); 0 or the error.
+inline int allow_shared_memory(const void* kernel, int bytes, unsigned long long* done) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return fail("no current CUDA device");
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (__atomic_load_n(done, __ATOMIC_RELAXED) & bit) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail("a kernel cannot have %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    __atomic_fetch_or(done, bit, __ATOMIC_RELAXED);
+    return 0;
+}
+
 #define KB_REQUIRE(cond, ...)                 \
     do {                                      \
         if (!(cond)) return kb::fail(__VA_ARGS__); \

@@ -234,7 +234,7 @@ __device__ void sf_sort(unsigned long long* list, int n) {
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             if (t < size / 2) {
-                const int i = (t / j) * 2 * j + t % j;
+                const int i = 2 * (t & ~(j - 1)) + (t & (j - 1));
                 const unsigned long long a = list[i], b = list[i + j];
                 if (((i & k) == 0) ? a < b : a > b) { list[i] = b; list[i + j] = a; }
             }
@@ -344,19 +344,29 @@ __device__ void sf_sum(cg::cluster_group& cluster, SfShared& s, unsigned long lo
     for (unsigned k = 0; k < cluster.num_blocks(); ++k) { a += s.fixed_sums[k][0]; b += s.fixed_sums[k][1]; }
 }
 
-// What is left in the bins from `from` to `to` into the first block's list.
+// What is left in the bins from `from` to `to` into the first block's list (`listed` of them there, of which SF_LIST are kept): every block lists its
+// own, then asks the first for room once.
 __device__ void sf_gather(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, const SfCut& cut, int from, int to) {
-    SfShared* home = cluster.map_shared_rank(&s, 0);
-    if (cluster.block_rank() == 0 && threadIdx.x == 0) s.listed = 0;
-    cluster.sync();
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
     r.each(fmaxf(sf_floor(cut), bins.floor(to)), [&](int i, float v) {
         const unsigned key = sf_key(v);
         if (!sf_left(cut, key, r.first + i)) return;
         const int b = bins.of(v, key);
         if (b < from || b > to) return;
-        const int at = atomicAdd(&home->listed, 1);
-        if (at < SF_LIST) home->list[at] = ((unsigned long long)key << 32) | (unsigned)~(r.first + i);
+        const int at = atomicAdd(&s.listed, 1);
+        if (at < SF_LIST) s.list[at] = ((unsigned long long)key << 32) | (unsigned)~(r.first + i);
     });
+    cluster.sync();
+    if (cluster.block_rank() != 0) {
+        SfShared* home = cluster.map_shared_rank(&s, 0);
+        const int mine = s.listed;
+        if (threadIdx.x == 0 && mine > 0) s.kept = atomicAdd(&home->listed, mine);
+        __syncthreads();
+        const int at = mine > 0 ? s.kept : 0;
+        for (int i = threadIdx.x; i < min(mine, SF_LIST); i += SF_THREADS)
+            if (at + i < SF_LIST) home->list[at + i] = s.list[i];
+    }
     cluster.sync();
 }
 
@@ -819,8 +829,8 @@ extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double
     p.cached = (int)(((size_t)MOST - sizeof(SfShared) - 32) / 4);
     if (p.cached > p.share) p.cached = p.share;
     const size_t smem = (sizeof(SfShared) + 15) / 16 * 16 + 16 + (size_t)p.cached * 4;
-    const cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
-    KB_REQUIRE(e == cudaSuccess, "sample_filtered: cannot have %d bytes of shared memory: %s", MOST, cudaGetErrorString(e));
+    static unsigned long long done = 0;
+    if (int e = allow_shared_memory((const void*)sample_filtered_kernel, MOST, &done)) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * blocks));
     cfg.blockDim = dim3(SF_THREADS);

@@ -183,9 +183,9 @@ def _need(t: torch.Tensor, what: str, dtype=None, shape=None) -> torch.Tensor:
 
 def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """Launches go to the current device's stream: every tensor has to be there."""
-    here = torch.cuda.current_device()
+    here = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
             raise KernelError(f"{what}: a tensor on {t.device} while device {here} is the current one")
 
 
@@ -1041,6 +1041,7 @@ def paged_attention_mma(q, k_table, v_table, block_table, row_count, tiles, page
 
 
 SHARED_PREFIX_ROWS = 512                # the most requests one call of `shared_prefix_attention` takes
+_SHARED_SCRATCH = {}                    # floats of scratch memory by sizes and device
 
 
 def shared_prefix_takes(dtype, hq: int, hkv: int, d: int, dv: int, page_size: int) -> bool:
@@ -1078,7 +1079,10 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
         raise KernelError(f"shared attention: a window of {window}")
     out = _fresh((rows, hq, dv), q.dtype, q.device)
     lib = library()
-    need = int(lib.kb_shared_attention_scratch_floats(rows, hq, hkv, d, dv))
+    sizes = (rows, hq, hkv, d, dv, q.get_device())
+    need = _SHARED_SCRATCH.get(sizes)
+    if need is None:
+        need = _SHARED_SCRATCH[sizes] = int(lib.kb_shared_attention_scratch_floats(rows, hq, hkv, d, dv))
     scratch = _fresh((need,), torch.float32, q.device) if need else None
     _check(lib.kb_shared_attention(_ptr(out), _ptr(q), _ptr(k_table), _ptr(v_table), dt, _ptr(block_table), _ptr(row_count), _ptr(share_id),
                                    _ptr(share_len), rows, hq, hkv, d, dv, int(page_size), int(block_table.shape[1]), int(n_pages),
