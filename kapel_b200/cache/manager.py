@@ -110,6 +110,8 @@ class Plan:
     committed: bool = False
     native: object = None        # the manager's own: the entries as the host library takes them
     share: object = None         # (ids, positions) by row where single tokens share pages (`CacheManager.shared_runs`), else None
+    line_bytes: int = 0          # bytes of a position's keys and values in the group that holds most of them, and of one component
+    item_bytes: int = 2
     added: List[Hashable] = field(default_factory=list)   # the step function's: sequences it added for this step
 
     @property
@@ -203,6 +205,7 @@ class CacheManager:
         self._info_ptr = self._info.ctypes.data
         self._family: Dict[Hashable, Tuple[int, int]] = {}       # sequence -> (family, positions its members share, whole pages)
         self._families = 0
+        self.line_bytes, self.item_bytes = 0, 2
         self._names = 0                                          # counts the sequences that have come or gone
         if allocate is not None:
             self.allocate_tables(allocate, dtype)
@@ -229,6 +232,8 @@ class CacheManager:
             for layer in g.layers:
                 g.keys[layer] = allocate(shape, dtype)
                 g.values[layer] = g.keys[layer] if g.needs.shared_values else allocate(v_shape, dtype)
+                self.item_bytes = getattr(getattr(g.keys[layer], "dtype", None), "itemsize", 2)
+                self.line_bytes = max(self.line_bytes, g.needs.kv_heads * (shape[3] + v_shape[3]) * self.item_bytes)
         for layer, spec in self.state_specs.items():
             self.states[layer] = allocate((self.max_sequences + 1, *spec.shape), spec.dtype)
 
@@ -425,6 +430,7 @@ class CacheManager:
         plan.native = (self._names, sc, n)
         if n_rows == n:
             plan.share = self.shared_runs([s for s, _ in entries])
+            plan.line_bytes, plan.item_bytes = self.line_bytes, self.item_bytes
         return plan
 
     def _entries_arrays(self, entries):

@@ -7,7 +7,6 @@
 // positions end there) what a row does not see is left out of its sum, not multiplied by zero: it may be anything.
 #include "attention_shared_bf16.cuh"
 #include "tensor_map.cuh"
-#include <cstdlib>
 
 namespace kb {
 
@@ -51,11 +50,79 @@ template <typename T, int DIM, int STRIDE> __device__ __forceinline__ void sr_li
     }
 }
 
+// A unit's NI groups of eight positions from group i0 on for eight threads' pair (row `pair` of the queries): scores, the running maximum and sum, the
+// weighted values.
+template <int NI, int DIM>
+__device__ __forceinline__ void sr_unit(const SharedRowsSmem<DIM>& s, const SharedParams& p, int pair, bool own, int i0, int j0, int first, int count, float& m, float& l,
+                                        float4 (&acc)[DIM / 32]) {
+    const int lane = threadIdx.x & 31, sub = threadIdx.x & 7;
+    float x[NI];
+    float top = -INFINITY;
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) x[i] = 0.f;
+    if (own) {
+#pragma unroll 8
+        for (int c = 0; c < DIM / 4; ++c) {
+            const float4 a = *reinterpret_cast<const float4*>(&s.q[pair][4 * c]);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const float4 b = *reinterpret_cast<const float4*>(&s.k[sub + 8 * (i0 + i)][4 * c]);
+                x[i] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, x[i]))));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int j = sub + 8 * (i0 + i);
+        float dot = x[i] * p.scale;
+        if (p.cap > 0.f) dot = p.cap * tanhf(dot / p.cap);
+        const bool sees = j0 + j >= first && j0 + j < count && s.line[j] >= 0;
+        all = all && sees;
+        x[i] = sees ? dot : -INFINITY;
+        top = fmaxf(top, x[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float next = fmaxf(m, top);
+    const float fade = next == -INFINITY ? 1.f : expf(m - next);           // e^-inf = 0 where nothing was seen before
+    m = next;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        x[i] = x[i] == -INFINITY ? 0.f : expf(x[i] - m);
+        sum += x[i];
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = l * fade + sum;
+#pragma unroll
+    for (int j = 0; j < DIM / 32; ++j) { acc[j].x *= fade; acc[j].y *= fade; acc[j].z *= fade; acc[j].w *= fade; }
+    const bool whole = __all_sync(0xffffffffu, all || !own);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const float e = __shfl_sync(0xffffffffu, x[i], (lane & 24) + b);
+            const float* v = &s.v[8 * (i0 + i) + b][4 * sub];
+            if (whole || e != 0.f) {
+#pragma unroll
+                for (int c = 0; c < DIM / 32; ++c) {
+                    const float4 y = *reinterpret_cast<const float4*>(v + 32 * c);
+                    acc[c].x = fmaf(e, y.x, acc[c].x);
+                    acc[c].y = fmaf(e, y.y, acc[c].y);
+                    acc[c].z = fmaf(e, y.z, acc[c].z);
+                    acc[c].w = fmaf(e, y.w, acc[c].w);
+                }
+            }
+        }
+}
+
 template <typename T, int DIM>
 __global__ void __launch_bounds__(SR_THREADS, 1) shared_rows_kernel(const SharedParams p) {
     extern __shared__ __align__(16) unsigned char sr_raw[];
     SharedRowsSmem<DIM>& s = *reinterpret_cast<SharedRowsSmem<DIM>*>(sr_raw);
-    const int tid = threadIdx.x, pair = tid >> 3, sub = tid & 7, lane = tid & 31;
+    const int tid = threadIdx.x, slot = tid >> 3, sub = tid & 7;
     const int group = p.hq / p.hkv, rows_a_tile = SR_PAIRS / group;
     const T* q = static_cast<const T*>(p.q);
     const T* kt = static_cast<const T*>(p.k_table);
@@ -87,6 +154,9 @@ __global__ void __launch_bounds__(SR_THREADS, 1) shared_rows_kernel(const Shared
         }
         u += w.n_units;
         const int pairs = w.n * group;
+        // Of few pairs each has two or four of the 32 places, each with its share of a unit's positions.
+        const int places = pairs <= 8 ? 8 : pairs <= 16 ? 16 : 32, shares = SR_PAIRS / places;
+        const int pair = slot & (places - 1), share = slot / places;
         const int row = w.row0 + pair / group;
         const bool own = pair < pairs;
         __syncthreads();                                 // the part before is done with the queries
@@ -116,66 +186,39 @@ __global__ void __launch_bounds__(SR_THREADS, 1) shared_rows_kernel(const Shared
             sr_lines<T, DIM, DIM + 4>(&s.k[0][0], kt, s.line, p.d, p.d % 4 == 0);
             sr_lines<T, DIM, DIM>(&s.v[0][0], vt, s.line, p.dv, p.dv % 4 == 0);
             __syncthreads();
-            float x[SR_KEYS / 8];
-            float top = -INFINITY;
-            bool all = true;
+            if (shares == 1) sr_unit<4, DIM>(s, p, pair, own, 0, j0, first, count, m, l, acc);
+            else if (shares == 2) sr_unit<2, DIM>(s, p, pair, own, 2 * share, j0, first, count, m, l, acc);
+            else sr_unit<1, DIM>(s, p, pair, own, share, j0, first, count, m, l, acc);
+        }
+        if (shares > 1) {
+            // The shares' sums, through the keys' and values' places, added up in the order of the shares.
+            __syncthreads();
+            float* sums = &s.k[slot][0];
+            float* states = &s.v[0][0];
 #pragma unroll
-            for (int i = 0; i < SR_KEYS / 8; ++i) x[i] = 0.f;
-            if (own) {
-#pragma unroll 8
-                for (int c = 0; c < DIM / 4; ++c) {
-                    const float4 a = *reinterpret_cast<const float4*>(&s.q[pair][4 * c]);
+            for (int c = 0; c < DIM / 32; ++c) *reinterpret_cast<float4*>(sums + 32 * c + 4 * sub) = acc[c];
+            if (sub == 0) { states[2 * slot] = m; states[2 * slot + 1] = l; }
+            __syncthreads();
+            if (share > 0) continue;
+            for (int k = 1; k < shares; ++k) m = fmaxf(m, states[2 * (slot + k * places)]);
+            const float base = m == -INFINITY ? 0.f : m, mine = states[2 * slot] == -INFINITY ? 0.f : expf(states[2 * slot] - base);
+            l *= mine;
 #pragma unroll
-                    for (int i = 0; i < SR_KEYS / 8; ++i) {
-                        const float4 b = *reinterpret_cast<const float4*>(&s.k[sub + 8 * i][4 * c]);
-                        x[i] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, x[i]))));
-                    }
+            for (int c = 0; c < DIM / 32; ++c) { acc[c].x *= mine; acc[c].y *= mine; acc[c].z *= mine; acc[c].w *= mine; }
+            for (int k = 1; k < shares; ++k) {
+                const int other = slot + k * places;
+                if (states[2 * other] == -INFINITY) continue;
+                const float theirs = expf(states[2 * other] - base);
+                l = fmaf(theirs, states[2 * other + 1], l);
+#pragma unroll
+                for (int c = 0; c < DIM / 32; ++c) {
+                    const float4 y = *reinterpret_cast<const float4*>(&s.k[other][32 * c + 4 * sub]);
+                    acc[c].x = fmaf(theirs, y.x, acc[c].x);
+                    acc[c].y = fmaf(theirs, y.y, acc[c].y);
+                    acc[c].z = fmaf(theirs, y.z, acc[c].z);
+                    acc[c].w = fmaf(theirs, y.w, acc[c].w);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < SR_KEYS / 8; ++i) {
-                const int j = sub + 8 * i;
-                float dot = x[i] * p.scale;
-                if (p.cap > 0.f) dot = p.cap * tanhf(dot / p.cap);
-                const bool sees = j0 + j >= first && j0 + j < count && s.line[j] >= 0;
-                all = all && sees;
-                x[i] = sees ? dot : -INFINITY;
-                top = fmaxf(top, x[i]);
-            }
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float next = fmaxf(m, top);
-            const float fade = next == -INFINITY ? 1.f : expf(m - next);       // e^-inf = 0 where nothing was seen before
-            m = next;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < SR_KEYS / 8; ++i) {
-                x[i] = x[i] == -INFINITY ? 0.f : expf(x[i] - m);
-                sum += x[i];
-            }
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l = l * fade + sum;
-#pragma unroll
-            for (int j = 0; j < DIM / 32; ++j) { acc[j].x *= fade; acc[j].y *= fade; acc[j].z *= fade; acc[j].w *= fade; }
-            const bool whole = __all_sync(0xffffffffu, all || !own);
-#pragma unroll
-            for (int i = 0; i < SR_KEYS / 8; ++i)
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    const float e = __shfl_sync(0xffffffffu, x[i], (lane & 24) + b);
-                    const float* v = &s.v[8 * i + b][4 * sub];
-                    if (whole || e != 0.f) {
-#pragma unroll
-                        for (int c = 0; c < DIM / 32; ++c) {
-                            const float4 y = *reinterpret_cast<const float4*>(v + 32 * c);
-                            acc[c].x = fmaf(e, y.x, acc[c].x);
-                            acc[c].y = fmaf(e, y.y, acc[c].y);
-                            acc[c].z = fmaf(e, y.z, acc[c].z);
-                            acc[c].w = fmaf(e, y.w, acc[c].w);
-                        }
-                    }
-                }
         }
         if (own) {
             float* piece = pieces + (size_t)pair * SH_PIECE(p.dv);
@@ -318,11 +361,10 @@ static SharedScratch shared_scratch(int rows, int hq, int hkv, int d) {         
     const int blocks = shared_blocks();
     return SharedScratch{shared_tile_places(rows, hq, blocks, 128), shared_row_places(rows, hq, hkv, blocks * shared_own_workers(d))};
 }
-// What a unit of a tile costs a multiprocessor, counted in units of 16 positions of a row.
-static float shared_tile_cost(int d) {
-    if (getenv("KB_SH_COST")) return (float)atof(getenv("KB_SH_COST"));
-    return d == 256 ? 14.f : 20.f;
-}
+// What a unit of a tile costs a multiprocessor, counted in units of 16 positions of a row; more than its bytes say, since a block over tiles takes
+// some 15 us to begin and to leave its pieces. As measured at 8, 12, 16, 24: 64 answers to 2,048 tokens, 16 heads over 8 of 256, 61, 58, 53, 54 us; 8
+// to 6,144, 8 over 4 of 256, 31, 27, 31, 36; two prompts and 34 requests, 32 over 16 of 128, 84, 76, 70, 68.
+static float shared_tile_cost(int d) { return d == 256 ? 14.f : 20.f; }
 
 // Floats of scratch memory: the tiles' pieces, the rows' pieces, then the cut.
 extern "C" long long kb_shared_attention_scratch_floats(int rows, int hq, int hkv, int d, int dv) {

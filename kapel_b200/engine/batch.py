@@ -57,8 +57,16 @@ def decode_split(pairs: int, longest: int, sms: int, window: Optional[int] = Non
     return split, max(1, -(-(span if relative else longest) // split))
 
 
-# Positions that need not be read again from which a step of single tokens goes by `kernels.shared_prefix_attention`.
-SHARED_POSITIONS = 512
+# When a step of single tokens goes by `kernels.shared_prefix_attention`. In bfloat16: from so many bytes of a layer's keys and values on that need not be
+# read again. Its three kernels take 19 us where the decode kernel takes 7 at the least; as measured (us, shared and row by row, each request with
+# 100 positions of its own): 8 heads over 4 of 256, 8 requests sharing 4,096 positions (117 MB) 29 and 29, 16 sharing 1,024 (63 MB) 22 and 18,
+# 32 sharing 1,024 (130 MB) 22 and 29, 64 sharing 4,096 (1.1 GB) 33 and 189; 16 over 8 of 256, 16 sharing 1,024 (126 MB) 22 and 28; 32 over 16 of 128,
+# 8 sharing 1,024 (59 MB) 26 and 19, 64 sharing 256 (132 MB) 32 and 38.
+SHARED_BYTES = 110_000_000
+# In 32-bit, where the kernel takes longer than the row-wise one over what requests have of their own: from so many positions a request (on average),
+# for each request of the step, on. 8 over 4 of 256: 2 requests sharing 64 positions 20 and 30, 16 sharing 256 36 and 46, 64 sharing 256 64 and 55; 32 over 16
+# of 128: 32 sharing 256 73 and 53, sharing 1,024 116 and 132.
+SHARED_POSITIONS_32 = 16
 
 
 def sharing_of(plan):
@@ -69,7 +77,9 @@ def sharing_of(plan):
     ids, lengths = share
     begins = np.ones(len(ids), bool)
     begins[1:] = (ids[1:] != ids[:-1]) | (lengths[1:] == 0)
-    return share if int(lengths[~begins].sum()) >= SHARED_POSITIONS else None
+    saved = int(lengths[~begins].sum())
+    pays = saved >= SHARED_POSITIONS_32 * plan.rows ** 2 if plan.item_bytes == 4 else saved * plan.line_bytes >= SHARED_BYTES
+    return share if saved and pays else None
 
 
 # Latent attention: a request's rows from which its keys and values are made for every head: that costs about 6 ns a position (16 heads of

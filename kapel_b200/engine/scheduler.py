@@ -24,8 +24,8 @@ never met, and one long request cannot end the others.
 Several answers to one prompt (`add_samples`; Kapel's engine shares prompt beginnings through its cache,
 crates/kapel-models/src/cache.rs:74-124) are one request until all but the last of the prompt's tokens are in
 the cache: there it is forked, and every answer feeds the last token by itself, over pages they hold
-together. An answer that then finds no slot or no page waits like any other request and computes its
-prompt when its turn comes, as one that was suspended does.
+together. Answers that then find no slot or no page wait, ahead of everybody, as a group of their own that
+computes the prompt again when its turn comes; one that was suspended computes its own.
 
 The scheduler needs of its engine only `cache` (a CacheManager), `step(entries)`, `end(id)` and
 `vocab_size` (and uses `max_positions`, `new_request_ids()` and `fork(id, new_ids)` where they exist), so its
@@ -152,7 +152,7 @@ class Scheduler:
 
     def add_samples(self, request: Request, n: int) -> List[int]:
         """`n` answers to one prompt, each a request of its own from here on (its events, its cancellation); the i-th draws
-        with the request's seed + i. The prompt is computed once."""
+        with the request's seed + i. The prompt is computed once for all that find room together."""
         if n < 1:
             raise ValueError(f"{n} answers to a prompt")
         if getattr(self.engine, "fork", None) is None or len(request.prompt) < 2:
@@ -173,10 +173,7 @@ class Scheduler:
         if entry is None:
             return
         others = self.answers.pop(rid, None)
-        if others:                                          # the next answer takes the prompt over
-            self.waiting.appendleft(others[0])
-            if others[1:]:
-                self.answers[others[0]] = others[1:]
+        self._wait_together(others or [])                   # the next answer takes the prompt over
         for first, rest in list(self.answers.items()):
             if rid in rest:
                 rest.remove(rid)
@@ -261,7 +258,7 @@ class Scheduler:
 
     def _fork(self) -> None:
         """Answers whose prompt is in the cache but for its last token go on from there, beside the request that computed it, as far
-        as there are slots and pages for them; the others wait, ahead of everybody, as requests of their own."""
+        as there are slots and pages for them; the others wait, ahead of everybody, the first of them to compute the prompt for all."""
         for first in [rid for rid in self.answers if self.entries[rid].running and self._cached(rid) == self.entries[rid].prompt_len - 1]:
             others = self.answers.pop(first)
             promised = [0] * len(self.cache.groups)
@@ -277,7 +274,7 @@ class Scheduler:
                 try:
                     self.engine.fork(first, go)
                 except Exception as e:
-                    self.waiting.extendleft(reversed(others))
+                    self._wait_together(others)
                     if not isinstance(e, CacheFull):
                         raise
                     continue
@@ -285,7 +282,13 @@ class Scheduler:
                 self.running[at:at] = go
                 for rid in go:
                     self.entries[rid].running = True
-            self.waiting.extendleft(reversed(wait))
+            self._wait_together(wait)
+
+    def _wait_together(self, answers: List[int]) -> None:
+        if answers:
+            self.waiting.appendleft(answers[0])
+            if answers[1:]:
+                self.answers[answers[0]] = answers[1:]
 
     def _suspend_last(self) -> None:
         rid = self.running.pop()

@@ -240,6 +240,18 @@ def main(argv=None) -> int:
     decode_fused_case(None)
     decode_fused_case(args.window)
 
+    if want("shared prefix") and B > 1 and ctx > 272:
+        # the batch as answers to one prompt: all but 256 positions of each request's history are the first one's pages
+        shared = (ctx - 256) // page * page
+        one = bt.clone()
+        one[:, : shared // page] = bt[:1, : shared // page]
+        q = torch.randn(B, Hq, D, device=dev).to(bf)
+        rc = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+        ids, lens = torch.zeros(B, dtype=torch.int32, device=dev), torch.full((B,), shared, dtype=torch.int32, device=dev)
+        us = _time(lambda i: K.shared_prefix_attention(q, tables[i % 2][0], tables[i % 2][1], one, rc, ids, lens, page, None, scale, cap), args.iters)
+        report(f"shared prefix [{B} requests, {shared} of {ctx} positions]", us, (shared + B * (ctx - shared)) * Hkv * D * 4 + 4 * B * Hq * D,
+               4.0 * B * ctx * Hq * D)
+
     def prompt_case(window):
         name = f"attention prompt window={window}"
         if not want(name):
@@ -304,6 +316,14 @@ def main(argv=None) -> int:
             temps = torch.full((B,), 0.8, device=dev) if sampled else None
             us_ = torch.rand(B, device=dev) if sampled else None
             us = _time(lambda i: K.sample(logits[i % c], temps, us_), args.iters)
+            report(f"{name} [{B}x{V}]", us, B * V * 4)
+    for name, k, p in (("sample top_k 50 top_p 0.95", 50, 0.95), ("sample top_p 0.95", 0, 0.95)):
+        if want(name):
+            c = min(copies(B * V * 4), 16)
+            logits = [2.0 * torch.randn(B, V, device=dev) for _ in range(c)]
+            f64 = lambda v: torch.full((B,), v, dtype=torch.float64, device=dev)
+            settings = (f64(0.8), torch.full((B,), k, dtype=torch.int32, device=dev), f64(p), f64(0.0), torch.rand(B, dtype=torch.float64, device=dev))
+            us = _time(lambda i: K.sample_filtered(logits[i % c], *settings), args.iters)
             report(f"{name} [{B}x{V}]", us, B * V * 4)
     return 0
 

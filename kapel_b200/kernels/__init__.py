@@ -69,6 +69,10 @@ def library():
                     getattr(lib, name).restype = ctypes.c_longlong
                 lib.kb_launch_count.restype = ctypes.c_ulonglong
                 lib.kb_dependent_launch_count.restype = ctypes.c_ulonglong
+                # Functions of many arguments take plain numbers: with their types known a call makes no object for each.
+                vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+                lib.kb_shared_attention.argtypes = [vp] * 4 + [i32] + [vp] * 4 + [i32] * 9 + [f32, f32, vp, vp, i64, vp]
+                lib.kb_sample_filtered.argtypes = [vp] * 7 + [i32, i32, vp]
                 lib.kb_set_pdl(1 if PDL else 0)
                 if _os.environ.get("KAPEL_B200_DELTA_COLUMNS"):      # 1, 2 or 4 columns a warp in the delta scan instead of the launcher's choice
                     lib.kb_delta_columns_per_warp(int(_os.environ["KAPEL_B200_DELTA_COLUMNS"]))
@@ -1084,9 +1088,10 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
     if need is None:
         need = _SHARED_SCRATCH[sizes] = int(lib.kb_shared_attention_scratch_floats(rows, hq, hkv, d, dv))
     scratch = _fresh((need,), torch.float32, q.device) if need else None
-    _check(lib.kb_shared_attention(_ptr(out), _ptr(q), _ptr(k_table), _ptr(v_table), dt, _ptr(block_table), _ptr(row_count), _ptr(share_id),
-                                   _ptr(share_len), rows, hq, hkv, d, dv, int(page_size), int(block_table.shape[1]), int(n_pages),
-                                   int(window or 0), _f(scale), _f(softcap or 0.0), _ptr(sinks), _ptr(scratch), ctypes.c_longlong(need), _stream()))
+    _check(lib.kb_shared_attention(out.data_ptr(), q.data_ptr(), k_table.data_ptr(), v_table.data_ptr(), dt, block_table.data_ptr(), row_count.data_ptr(),
+                                   share_id.data_ptr(), share_len.data_ptr(), rows, hq, hkv, d, dv, int(page_size), block_table.shape[1], n_pages,
+                                   int(window or 0), float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
+                                   None if scratch is None else scratch.data_ptr(), need, _stream()))
     return out
 
 
@@ -2126,8 +2131,8 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     _need(top_k, "sample_filtered top_k", torch.int32, (rows,))
     _on_current_device("sample_filtered", logits, temperature, top_k, top_p, min_p, uniform)
     out = _fresh((rows,), torch.int32, logits.device)
-    _check(library().kb_sample_filtered(_ptr(out), _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform),
-                                        int(rows), int(vocab), _stream()))
+    _check(library().kb_sample_filtered(out.data_ptr(), logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
+                                        uniform.data_ptr(), rows, vocab, _stream()))
     return out
 
 # ------------------------------------------------------------------------------------------

@@ -191,7 +191,8 @@ class Model:
                          seed: Optional[int] = None, stop: Optional[Sequence] = None, ignore_eos: bool = False,
                          max_sequences: Optional[int] = None):
         """`n` answers to one prompt (token ids in, lists of token ids out; text in, texts out); answer i draws with seed + i. The
-        prompt is computed once and its pages are held together; a step reads them once for all answers that run."""
+        prompt is computed once for all answers that run together (up to `max_sequences`), and they hold its pages together; a step reads
+        those once for all of them where that pays."""
         as_text = isinstance(prompt, str)
         ids = self.tokenize(prompt) if as_text else [int(t) for t in prompt]
         request = self._request(ids, max_tokens, temperature, top_k, top_p, min_p, repetition_penalty, seed, stop, ignore_eos)

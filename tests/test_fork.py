@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from kapel_b200.cache import CacheFull, CacheManager, CacheNeeds, PagedKV, StateSpec
-from kapel_b200.engine.batch import SHARED_POSITIONS, sharing_of
+from kapel_b200.engine.batch import SHARED_BYTES, SHARED_POSITIONS_32, sharing_of
 from kapel_b200.engine.scheduler import EngineOptions, Request, Scheduler
 from kapel_b200.sampling import Sampling
 from test_scheduler import FakeEngine, StagingEngine
@@ -122,14 +122,20 @@ def test_rows_that_share_are_told():
     assert lengths.tolist() == [0, 0, 32, 32]
     p = m.plan([(s, 1) for s in "abc"])
     assert p.share is not None and p.share[1].tolist() == [32, 32, 32]
-    assert sharing_of(p) is None                             # 64 positions less to read
+    p.line_bytes = SHARED_BYTES // 64                        # the three rows need 64 positions less
+    assert sharing_of(p) is p.share
+    p.line_bytes = SHARED_BYTES // 64 - 1
+    assert sharing_of(p) is None
+    p.item_bytes = 4
+    assert (sharing_of(p) is not None) == (64 >= SHARED_POSITIONS_32 * 9)
     m.abort(p)
     assert m.plan([("a", 2), ("b", 1)]).share is None        # not a step of single tokens
     m2 = manager(pages=200, max_sequences=8)
     m2.add_sequence("a")
-    feed(m2, "a", SHARED_POSITIONS + 5)
+    feed(m2, "a", 4 * SHARED_POSITIONS_32 + 5)
     m2.fork("a", "b")
     p = m2.plan([("a", 1), ("b", 1)])
+    p.item_bytes = 4
     assert sharing_of(p) is p.share
     m2.abort(p)
     m2.remove_sequence("a")
@@ -246,6 +252,8 @@ def test_answers_beyond_the_slots_and_pages_wait_and_come():
         out = run(sched)
         assert all(out[r] == alone(prompt, 25) for r in ids)
         assert eng.cache.free_pages() == eng.cache.total_pages()
+        if pages == 60:                                      # three at a time: the prompt for each group once
+            assert sum(c for p in eng.passes for r, c in p) == 3 * 39 + 7 * 25
 
 
 def test_an_engine_without_fork_computes_each():

@@ -40,7 +40,7 @@ def test_forked_requests_go_on_as_if_alone(family, name, shared, graphs, prompt_
     """32-bit: logits of three forked requests beside one of its own against the same tokens computed without a fork."""
     from kapel_b200.engine import batch
 
-    monkeypatch.setattr(batch, "SHARED_POSITIONS", 1 if shared else 1 << 30)
+    monkeypatch.setattr(batch, "SHARED_POSITIONS_32", 0 if shared else 1 << 30)
     eng = engine_of(config_of(family, name), "float32", graphs=graphs)
     rng = np.random.default_rng(1)
     prompt = random_tokens(rng, prompt_len, eng.vocab_size)
@@ -67,7 +67,8 @@ def test_forked_requests_go_on_as_if_alone(family, name, shared, graphs, prompt_
 def test_forked_requests_in_bfloat16(family, name, monkeypatch):
     from kapel_b200.engine import batch
 
-    monkeypatch.setattr(batch, "SHARED_POSITIONS", 1)
+    monkeypatch.setattr(batch, "SHARED_BYTES", 1)
+    monkeypatch.setattr(batch, "SHARED_POSITIONS_32", 0)
     eng = engine_of(config_of(family, name), "bfloat16")
     rng = np.random.default_rng(2)
     prompt = random_tokens(rng, 50, eng.vocab_size)
@@ -122,7 +123,8 @@ def test_greedy_answers_are_the_one_answer(family, name, monkeypatch):
     from kapel_b200 import Model
     from kapel_b200.engine import batch
 
-    monkeypatch.setattr(batch, "SHARED_POSITIONS", 1)
+    monkeypatch.setattr(batch, "SHARED_BYTES", 1)
+    monkeypatch.setattr(batch, "SHARED_POSITIONS_32", 0)
     model = Model(None, dtype="f32", max_sequences=12, _engine=engine_of(config_of(family, name), "float32"))
     prompt = random_tokens(np.random.default_rng(3), 37, model.engine.vocab_size)
     want = model.generate(prompt, max_tokens=16, temperature=0.0, ignore_eos=True)
@@ -136,7 +138,8 @@ def test_drawn_answers_are_those_of_their_seeds(monkeypatch):
     from kapel_b200 import Model
     from kapel_b200.engine import batch
 
-    monkeypatch.setattr(batch, "SHARED_POSITIONS", 1)
+    monkeypatch.setattr(batch, "SHARED_BYTES", 1)
+    monkeypatch.setattr(batch, "SHARED_POSITIONS_32", 0)
     model = Model(None, dtype="f32", max_sequences=12, _engine=engine_of(config_of("gemma2", "A"), "float32"))
     prompt = random_tokens(np.random.default_rng(4), 50, model.engine.vocab_size)
     kw = dict(max_tokens=24, temperature=1.1, top_k=60, top_p=0.95, ignore_eos=True)
@@ -152,7 +155,8 @@ def test_shared_steps_are_recorded_and_run_ahead(monkeypatch):
     from kapel_b200 import Model
     from kapel_b200.engine import batch
 
-    monkeypatch.setattr(batch, "SHARED_POSITIONS", 1)
+    monkeypatch.setattr(batch, "SHARED_BYTES", 1)
+    monkeypatch.setattr(batch, "SHARED_POSITIONS_32", 0)
     eng = engine_of(config_of("gemma2", "A"), "bfloat16")
     model = Model(None, dtype="bf16", max_sequences=12, _engine=eng)
     model.generate_samples([3, 4, 5] * 12, 4, max_tokens=40, temperature=0.9, top_p=0.9, ignore_eos=True)
