@@ -356,6 +356,13 @@ static bool shared_on_tensor_cores(int dtype, int hq, int hkv, int d, int dv, in
     return dtype == KB_DT_BF16 && d == dv && (d == 64 || d == 128 || d == 256) && page_size % 16 == 0 && hq / hkv <= 16;
 }
 
+// Where all rows' block tables together hold no more keys and values than this, every row reads what it sees by itself: the shared part comes out of
+// the second-level cache for all but the first, and the kernel over tiles, some 10 us before its first product, is not launched. As measured
+// (us, with tiles and without): 8 heads over 4 of 256, 2 rows sharing 64 positions (1 MB) 19 and 9, 16 sharing 1,024 (75 MB) 22 and 19, 8 sharing
+// 4,096 (138 MB) 30 and 26, 32 sharing 1,024 (153 MB) 22 and 26, 16 sharing 4,096 (277 MB) 29 and 38; 32 over 16 of 128, 8 sharing 1,024 (74 MB) 27 and
+// 17, 64 sharing 64 (126 MB) 46 and 22, 16 sharing 1,024 (151 MB) 26 and 25, 8 sharing 4,096 (276 MB) 30 and 37.
+constexpr long long SHARED_ALONE_BYTES = 144000000;
+
 struct SharedScratch { long long tile_places, row_places; };
 static SharedScratch shared_scratch(int rows, int hq, int hkv, int d) {          // what either path needs at most
     const int blocks = shared_blocks();
@@ -406,13 +413,16 @@ extern "C" int kb_shared_attention(void* out, const void* q, const void* k_table
     if (shared_on_tensor_cores(dtype, hq, hkv, d, dv, page_size)) {
         const unsigned long long lines = (unsigned long long)n_pages * hkv * page_size;
         KB_REQUIRE(lines <= 0x7fffffffull, "shared_attention: tables of %llu lines", lines);
+        p.alone = (long long)rows * table_width * page_size * hkv * d * 4 <= SHARED_ALONE_BYTES;
         CUtensorMap mk, mv;
-        if (int e = encode_map_bf16(&mk, k_table, lines, d, d, 16)) return e;
-        if (int e = encode_map_bf16(&mv, v_table, lines, d, d, 16)) return e;
         // In a step of few rows the kernel over rows starts while the one over tiles runs, and takes the multiprocessors that one leaves.
-        const bool side = may_chain(p.rows <= DEPENDENT_ROWS);
-        p.tile_cost = side ? shared_tile_cost(d) : 0.f;
-        if (int e = launch_shared_tiles(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
+        if (!p.alone) {
+            const bool side = may_chain(p.rows <= DEPENDENT_ROWS);
+            p.tile_cost = side ? shared_tile_cost(d) : 0.f;
+            if (int e = encode_map_bf16(&mk, k_table, lines, d, d, 16)) return e;
+            if (int e = encode_map_bf16(&mv, v_table, lines, d, d, 16)) return e;
+            if (int e = launch_shared_tiles(p, mk, mv, blocks, (cudaStream_t)stream)) return e;
+        }
         CUtensorMap ok, ov;                              // the same in boxes of all of a line's chunks
         if (int e = encode_map_bf16_chunks(&ok, k_table, lines, d, 16)) return e;
         if (int e = encode_map_bf16_chunks(&ov, v_table, lines, d, 16)) return e;

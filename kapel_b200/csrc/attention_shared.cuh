@@ -39,6 +39,7 @@ struct SharedParams {
     int* cut;                  // what the kernels leave for the one that joins: see SH_CUT_*
     int rows, hq, hkv, d, dv, page_size, table_width, n_pages, window;
     float scale, cap;
+    int alone;                 // every row reads all it sees by itself (there is little to read)
     float tile_cost;           // > 0: the kernels over tiles and over rows run side by side; what a tile's unit costs, counted in a row's units
 };
 
@@ -64,6 +65,7 @@ __device__ __forceinline__ int shared_first(const SharedParams& p, int count) { 
 }
 // What a row shares, as the launcher's limits let it stand: whole pages, no more than its block table holds and than it has seen.
 __device__ __forceinline__ int shared_length(const SharedParams& p, int r) {
+    if (p.alone) return 0;
     const int n = min(min(p.share_len[r], p.row_count[r]), p.table_width * p.page_size);
     return n > 0 ? n / p.page_size * p.page_size : 0;
 }
@@ -75,9 +77,10 @@ __device__ __forceinline__ int shared_own(const SharedParams& p, int r, int keys
 }
 
 // upto[0 .. n] holds n numbers and becomes their running totals (what lies before each, then all), by one warp. No barrier.
-__device__ __forceinline__ void shared_totals(int* upto, int n) {
+static __device__ __noinline__ void shared_totals(int* upto, int n) {
     const int lane = threadIdx.x & 31;
     int total = 0;
+#pragma unroll 1
     for (int base = 0; base < n; base += 32) {
         const int i = base + lane;
         const int mine = i < n ? upto[i] : 0;
@@ -96,6 +99,7 @@ __device__ __forceinline__ void shared_totals(int* upto, int n) {
 // The cut into tiles, by the whole block; `rows_a_tile` requests to a tile, `keys` positions to a unit.
 __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, int rows_a_tile, int keys) {
     const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x;
+#pragma unroll 1
     for (int i = tid; i < p.rows; i += nt) {
         c.klo[i] = 0x7fffffff; c.khi[i] = 0; c.before[i] = 0; c.row0[i] = 0x7fffffff; c.looks[i] = 0x7fffffff;
         c.length[i] = shared_length(p, i);               // every load of the cut is asked for here, all rows at once
@@ -106,6 +110,7 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
     if (tid < 32) {
         // Where each row's run begins, and with it the row's place in the run: rows_a_tile of them to a tile.
         int run = 0, tiles = 0;
+#pragma unroll 1
         for (int base = 0; base < p.rows; base += 32) {
             const int r = base + lane;
             const bool in = r < p.rows;
@@ -123,6 +128,7 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
         if (lane == 0) { c.tiles = tiles; c.row_units = 0; }
     }
     __syncthreads();
+#pragma unroll 1
     for (int r = tid; r < p.rows; r += nt) {
         const int t = c.row_tile[r];
         if (p.tile_cost > 0.f) {
@@ -138,10 +144,12 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
         }
     }
     __syncthreads();
+#pragma unroll 1
     for (int r = tid; r < p.rows; r += nt) {
         const int t = c.row_tile[r];
         if (t >= 0 && c.first[r] <= c.klo[t]) atomicMin(&c.looks[t], r);
     }
+#pragma unroll 1
     for (int i = tid; i < c.tiles; i += nt) {
         c.n[i] = c.before[i];
         c.upto[i] = c.klo[i] < c.khi[i] ? (c.khi[i] - c.klo[i] / keys * keys + keys - 1) / keys : 0;
@@ -156,6 +164,7 @@ __device__ inline void shared_cut_tiles(const SharedParams& p, SharedTiles& c, i
 
 // The cut into rows: upto[r] = units before row r, which reads positions [lo[r], hi[r]) by itself. By the whole block.
 __device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int* lo, int* hi, int keys) {
+#pragma unroll 1
     for (int r = threadIdx.x; r < p.rows; r += blockDim.x) upto[r] = shared_own(p, r, keys, lo[r], hi[r]);
     __syncthreads();
     if (threadIdx.x < 32) shared_totals(upto, p.rows);
@@ -166,6 +175,7 @@ __device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int* lo
 __device__ __forceinline__ int shared_tile_units(const SharedParams& p, const int* length, const int* id, int rows_a_tile, int keys) {
     const int lane = threadIdx.x & 31;
     int run = 0, units = 0;
+#pragma unroll 1
     for (int base = 0; base < p.rows; base += 32) {
         const int r = base + lane, n = r < p.rows ? length[r] : 0;
         const bool starts = r < p.rows && (r == 0 || n == 0 || length[r - 1] != n || id[r - 1] != id[r]);

@@ -47,6 +47,10 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
     }
     const int group = p.hq / p.hkv;
     int blocks = gridDim.x;
+    if (p.alone) {                                           // no kernel over tiles has waited for the one before
+        dependent_wait();
+        dependent_trigger();
+    }
     if (p.tile_cost > 0.f) {
         for (int r = threadIdx.x; r < p.rows; r += blockDim.x) { length[r] = shared_length(p, r); id[r] = p.share_id[r]; }
     }
@@ -58,7 +62,13 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
         if (theirs < blocks) blocks -= theirs;
     }
     const SharedRange range = shared_range(blockIdx.x * C::WARPS + warp, blocks * C::WARPS, upto[p.rows], p.hkv);
-    if (blockIdx.x == 0) shared_leave_rows(p, upto, range.workers);
+    if (blockIdx.x == 0) {
+        shared_leave_rows(p, upto, range.workers);
+        if (p.alone) {                                       // no tiles
+            for (int i = threadIdx.x; i < p.rows; i += blockDim.x) p.cut[SH_CUT_ROW_TILE + i] = -1;
+            if (threadIdx.x == 0) p.cut[SH_CUT_COUNTS] = p.cut[SH_CUT_COUNTS + 1] = p.cut[SH_CUT_TILE_UNITS] = 0;
+        }
+    }
     const bf16* q = static_cast<const bf16*>(p.q);
 
     // What is asked for: unit `ask` of the worker's, the `a_in`-th of `a_units` of a request and kv head. The pages of the next
@@ -256,7 +266,7 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
 template <int D, int NB> static int launch_own(const SharedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t s) {
     static unsigned long long done = 0;
     if (int e = allow_shared_memory((const void*)shared_own_kernel<D, NB>, OwnCfg<D>::SMEM, &done)) return e;
-    launch_dependent_if(p.tile_cost > 0.f, shared_own_kernel<D, NB>, dim3(blocks), dim3(OwnCfg<D>::WARPS * 32), OwnCfg<D>::SMEM, s, p, mk, mv);
+    launch_dependent_if(p.alone ? p.rows <= DEPENDENT_ROWS : p.tile_cost > 0.f, shared_own_kernel<D, NB>, dim3(blocks), dim3(OwnCfg<D>::WARPS * 32), OwnCfg<D>::SMEM, s, p, mk, mv);
     return check_launch("shared_attention");
 }
 

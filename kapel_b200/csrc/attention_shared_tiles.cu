@@ -51,6 +51,33 @@ __device__ __forceinline__ TilePart st_part(const SharedParams& p, const SharedT
     return w;
 }
 
+// A part's queries by the softmax's warps, K-major under the swizzle: chunk c of pair r at c 16 KB + r 128, its 16-byte pieces exchanged by r mod 8.
+// Eight neighbouring threads bring a pair's 128 bytes, up to eight pieces each asked for at a time. Pairs that are none keep what is there: nobody
+// reads their results.
+template <int D> __device__ __forceinline__ void st_queries(const SharedParams& p, const TilePart& w, unsigned char* q_smem, uint64_t* q_full) {
+    constexpr int CH = TilesCfg<D>::CH, ITER = ST_PAIRS * CH * 8 / (ST_SOFT * 32), STEP = ST_SOFT * 4 / CH;
+    const int st = threadIdx.x - 64, j = st & 7, ch = (st >> 3) % CH, r0 = (st >> 3) / CH;
+    const int group = p.hq / p.hkv, pairs = w.n * group;
+    const uint32_t by_group = (65536u + (uint32_t)group - 1u) / (uint32_t)group;          // r / group = r by_group >> 16 for r < 128
+    const bf16* src = static_cast<const bf16*>(p.q) + ((size_t)w.row0 * p.hq + w.kvh * group) * D + ch * 64 + j * 8;
+    unsigned char* dst = q_smem + ch * (ST_PAIRS * 128);
+    uint4 x[ITER];
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+        const int r = r0 + k * STEP;
+        const uint32_t row = (uint32_t)r * by_group >> 16;
+        x[k] = r < pairs ? *reinterpret_cast<const uint4*>(src + (size_t)(row * p.hq + (r - row * group)) * D) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+        const int r = r0 + k * STEP;
+        if (r < pairs) *reinterpret_cast<uint4*>(dst + (size_t)r * 128 + ((j ^ (r & 7)) << 4)) = x[k];
+    }
+    at_fence_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) at_mbar_arrive(q_full);
+}
+
 // Lane i's word j becomes lane j's word i.
 __device__ __forceinline__ void st_transpose(uint32_t (&x)[32], int lane) {
 #pragma unroll
@@ -225,37 +252,10 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
         }
     } else {
         // ---------------------------------------------------------------- queries, softmax and pieces, a quarter of a pair's positions a thread
-        const int quarter = warp & 3, share = (warp - 2) >> 2, pair = quarter * 32 + lane, st = tid - 64;
+        const int quarter = warp & 3, share = (warp - 2) >> 2, pair = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const SharedScore score(p.scale, p.cap);
-        const bf16* q = static_cast<const bf16*>(p.q);
-        // A part's queries, K-major under the swizzle: chunk c of pair r at c 16 KB + r 128, its 16-byte pieces exchanged by r mod 8. Eight
-        // neighbouring threads bring a pair's 128 bytes. Pairs that are none keep what is there: nobody reads their results.
-        const uint32_t by_group = (65536u + (uint32_t)group - 1u) / (uint32_t)group;          // r / group = r by_group >> 16 for r < 128
-        auto lay_queries = [&](const TilePart& w) {
-            const int pairs = w.n * group;
-            constexpr int ITER = ST_PAIRS * CH * 8 / (ST_SOFT * 32), DEEP = ITER < 8 ? ITER : 8;          // pieces a thread; asked for eight at a time
-            const int j = st & 7, ch = (st >> 3) % CH, r0 = (st >> 3) / CH;
-            const bf16* src = q + ((size_t)w.row0 * p.hq + w.kvh * group) * D + ch * 64 + j * 8;
-            unsigned char* dst = q_smem + ch * (ST_PAIRS * 128);
-            for (int base = 0; base < ITER; base += DEEP) {
-                uint4 x[DEEP];
-#pragma unroll
-                for (int k = 0; k < DEEP; ++k) {
-                    const int r = r0 + (base + k) * (ST_SOFT * 4 / CH);
-                    const uint32_t row = (uint32_t)r * by_group >> 16;
-                    x[k] = r < pairs ? *reinterpret_cast<const uint4*>(src + (size_t)(row * p.hq + (r - row * group)) * D) : make_uint4(0u, 0u, 0u, 0u);
-                }
-#pragma unroll
-                for (int k = 0; k < DEEP; ++k) {
-                    const int r = r0 + (base + k) * (ST_SOFT * 4 / CH);
-                    if (r < pairs) *reinterpret_cast<uint4*>(dst + (size_t)r * 128 + ((j ^ (r & 7)) << 4)) = x[k];
-                }
-            }
-            at_fence_async_smem();
-            __syncwarp();
-            if (lane == 0) at_mbar_arrive(q_full);
-        };
+        auto lay_queries = [&](const TilePart& w) { st_queries<D>(p, w, q_smem, q_full); };
         int c = 0, part = 0, turns = 0;
         TilePart w = st_part(p, cut, range.begin, range.end);
         lay_queries(w);

@@ -6,6 +6,15 @@ import pytest
 import torch
 
 PAGE = 16
+WIDE = False
+
+
+@pytest.fixture(autouse=True, params=["narrow", "wide"])
+def tables(request):
+    """Every test twice: with block tables as wide as the requests are long, of which a small call reads every row by itself, and in bfloat16 with
+    tables wide enough that what rows share is read once on the tensor cores."""
+    global WIDE
+    WIDE = request.param == "wide"
 
 
 def make(runs, hq, hkv, d, dv=None, dtype=torch.bfloat16, seed=0, page=PAGE, sinks=False, spread=1.0, extra_width=0):
@@ -14,6 +23,8 @@ def make(runs, hq, hkv, d, dv=None, dtype=torch.bfloat16, seed=0, page=PAGE, sin
     rng = np.random.default_rng(seed)
     counts = [c for cs, _ in runs for c in cs]
     width = max(1, -(-max(counts) // page)) + extra_width
+    if WIDE and dtype == torch.bfloat16:
+        width += -(-150_000_000 // (len(counts) * page * hkv * d * 4))
     table = np.full((len(counts), width), -1, np.int32)
     total = sum(shared // page + sum(max(0, -(-(c - shared) // page)) for c in cs) for cs, shared in runs) + 3
     pages = rng.permutation(total).astype(np.int32).tolist()
@@ -264,6 +275,14 @@ def test_what_is_refused():
             K.shared_prefix_attention(**{**good, **bad})
     e = K.shared_prefix_attention(**{**good, "q": c["q"][:0], "row_count": c["count"][:0], "share_id": c["share_id"][:0], "share_len": c["share_len"][:0]})
     assert e.shape == (0, 8, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [None, 1500])
+@pytest.mark.parametrize("rows", [40, 70])                   # a step of few rows runs its two kernels side by side, a larger one does not
+@pytest.mark.parametrize("hq,hkv,d", [(8, 4, 256), (16, 4, 128), (4, 2, 64)])
+def test_many_units_a_block(hq, hkv, d, rows, window):
+    check(make([([2400 + 1 + 13 * i % 200 for i in range(rows - 3)], 2400), ([800, 790], 752), ([1300], 0)], hq, hkv, d, seed=rows, spread=2.0), window=window, softcap=50.0)
 
 
 @pytest.mark.gpu
