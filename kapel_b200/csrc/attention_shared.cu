@@ -5,6 +5,9 @@
 // computes every eighth position's score out of keys and queries in shared memory, and keeps every eighth group of four components of the
 // sum in registers. All arithmetic is 32-bit. Where some row of the tile does not see all of a unit (its window begins there, its
 // positions end there) what a row does not see is left out of its sum, not multiplied by zero: it may be anything.
+//
+// What bounds it: the multiply-adds and what they read of shared memory; a unit's loads are not asked for ahead of the one before. 8 requests behind
+// 1,024 positions with some 70 of their own, 8 heads over 4 of 256 in 32 bits: 28 us, the joining of the pieces among them.
 #include "attention_shared_bf16.cuh"
 #include "tensor_map.cuh"
 

@@ -8,6 +8,9 @@
 // heads of the kv head as their N, eight a block, NB blocks; P^T comes out of S^T's registers by movmatrix. Scores, softmax and sums are 32-bit; the
 // weights are rounded to bfloat16 for the second product, and the sum of the weights adds up the rounded ones.
 //
+// What bounds it: memory, at the copy's rate once under way (3 x 16 KB a warp in flight). Before that the cut is made, the block tables are read and
+// the first keys and queries come, some 7 us. 64 requests of some 330 positions each, 8 kv heads of 256 (175 MB): 42 us, 4.2 TB/s.
+//
 // Positions of a unit that the request does not see get the weight 0, and their values are cleared in shared memory first: what another request
 // left in the page may be anything.
 #include "attention_shared_bf16.cuh"

@@ -23,6 +23,11 @@
 // few units of the 13th digit. It is made of 2^(n / 32) = 2^k T[n mod 32], n an integer within a roundoff of the nearest to 32 x / ln 2 (found in 32 bits), and a
 // polynomial of degree 5 for what is left (the series' next term is below 3e-15): nine 64-bit operations, of which a multiprocessor does some 37 a
 // clock. Two entries of T share a bank, so a warp's loads take two turns at most.
+//
+// What bounds it, over 256,000 tokens: one row alone takes 15 us under top_k 50, of which the row's load is 3 and the rest some eight cluster
+// barriers and what lies between them. 64 rows: 67 us under top_k 50 (1.0 TB/s), 110 without filters, 130 under a nucleus of 0.95 (the exponentials of
+// all tokens and the histogram's atomics), 215 under 0.99, whose cut lies among so many tokens of nearly one weight that the bins are divided
+// again. A multiprocessor holds one block, so 16 to 18 rows are under way at a time, and none while the last of them end.
 #include <cooperative_groups.h>
 #include <cfloat>
 #include "common.cuh"

@@ -1060,7 +1060,8 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
     same `share_id` and `share_len` (int32 [rows]) have the same pages for their first share_len positions, and what they share is read
     once for all of them, out of the block table of the one that sees furthest back. share_len is taken down to whole pages and to the row's
     count; 0 shares nothing. Up to SHARED_PREFIX_ROWS rows. Window, soft cap and `sinks` as for `paged_attention_mma`; a row that
-    sees nothing gives zeros. With a window, shared values that only some rows of a group still see have to be finite in bfloat16."""
+    sees nothing gives zeros. Every page with a position that a row sees has to be in its table; what lies in it behind the row's count, or before its
+    window, may be anything, but that with a window shared values which only some rows of a group still see have to be finite in bfloat16."""
     _need(q, "shared attention q")
     if q.dim() != 3:
         raise KernelError(f"shared attention: q {tuple(q.shape)} is not [rows, heads, head size]")
@@ -2119,7 +2120,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     """One token a row of float32 logits [rows, vocab], by the host sampler's rules (`sampling.Sampler`) and in 64 bits as there: the
     first largest where the row's temperature is 0 or less; else logits / temperature, top_k (0 or less: none; what ties with the
     k-th stays), top_p (1 or more: none; the lower index first among equals), min_p (0 or less: none), and the first index
-    whose running total exceeds `uniform` times what is left. `temperature`, `top_p`, `min_p` and `uniform` are float64 [rows], `top_k`
+    whose running total exceeds `uniform`, in [0, 1), times what is left. `temperature`, `top_p`, `min_p` and `uniform` are float64 [rows], `top_k`
     int32 [rows], all on the logits' device, which has to be the current one. Nothing left (a top_p of 0 or less, a min_p above 1) gives
     token 0; logits with a NaN or an infinity among them their first largest."""
     _need(logits, "sample_filtered logits", torch.float32)

@@ -186,6 +186,30 @@ def test_a_recorded_choice_and_another_stream():
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    from kapel_b200 import kernels as K
+
+    rng = np.random.default_rng(9)
+    f = lambda a: torch.tensor(a, dtype=torch.float64, device="cuda")
+    cases = []
+    for rows, vocab in ((24, 256000), (5, 3001)):
+        cases.append((torch.from_numpy(rng.normal(0.0, 2.0, (rows, vocab)).astype(np.float32)).cuda(), f([0.9] * rows), torch.tensor([i % 3 * 40 for i in range(rows)], dtype=torch.int32, device="cuda"),
+                      f([0.95] * rows), f([0.01] * rows), f(rng.random(rows))))
+    want = [K.sample_filtered(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(K.sample_filtered(*cases[j]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for x in got[j]:
+            assert torch.equal(x, want[j])
+
+
+@pytest.mark.gpu
 def test_no_rows():
     from kapel_b200 import kernels as K
 

@@ -286,6 +286,62 @@ def test_many_units_a_block(hq, hkv, d, rows, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shared_lengths_that_are_no_whole_pages(dtype):
+    """Taken down to whole pages, to what the row has seen and to its block table; below a page, or negative, nothing is shared."""
+    for shared, whole in ((175, 160), (15, 0), (-1, 0), (-2 ** 31, 0), (2 ** 31 - 1, None)):
+        c = make([([200, 161, 177], 160), ([40], 0)], 8, 4, 128, dtype=dtype, seed=4)
+        if whole is None:                                    # three rows with the same history, all of it shared
+            c["count"][:3], c["counts"][:3] = 176, [176] * 3
+            c["table"][:3] = c["table"][0].clone()
+        c["share_len"][:3] = shared
+        check(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 4, 256), (16, 4, 128), (6, 2, 20)])
+def test_own_pages_that_are_none_are_not_seen(dtype, hq, hkv, d):
+    c = make([([200, 161, 177], 160), ([90], 0)], hq, hkv, d, dtype=dtype, seed=5)
+    c["table"][0, 11] = -1
+    c["table"][3, 1:3] = -7
+    want, size = plain(c)
+    c["table"][0, 11] = c["k"].shape[0]                      # beyond the tables
+    c["table"][3, 2] = 2 ** 31 - 1
+    got = run(c).double().cpu().numpy()
+    bound = 2e-5 * (size + 1e-3) if dtype == torch.float32 else 2.0 ** -8 * size + 2.0 ** -8 * np.abs(want) + 1e-5
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.gpu
+def test_one_page_many_times():
+    """The same page at several places of a table, and in tables that share nothing."""
+    c = make([([200, 161, 177], 160), ([90, 80], 0)], 8, 4, 128, seed=6)
+    c["table"][:3, 3] = c["table"][0, 1].clone()
+    c["table"][:3, 4] = c["table"][0, 1].clone()
+    c["table"][4, 2:5] = c["table"][3, 0].clone()
+    check(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams_at_once(dtype):
+    cases = [make([([700 + 3 * i for i in range(12)], 640 - 64 * j), ([90 + j], 0)], 8, 4, 128, dtype=dtype, seed=j) for j in range(2)]
+    want = [run(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(run(cases[j]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for x in got[j]:
+            assert torch.equal(x, want[j])
+
+
+@pytest.mark.gpu
 def test_the_most_rows():
     from kapel_b200 import kernels as K
 
