@@ -38,6 +38,7 @@ namespace cg = cooperative_groups;
 constexpr int SF_THREADS = 1024, SF_WARPS = SF_THREADS / 32;
 constexpr int SF_BINS = 2048, SF_LIST = 2048, SF_MAX_CLUSTER = 8;
 constexpr int SF_SMALL = 256;                            // lists up to here are ordered by counting
+constexpr int SF_FULL = 48;                              // entries of a bucket that are ordered among themselves
 constexpr int SF_ROWS = 64;                              // rows of 32 columns a warp has at most: a share of 2^16, a vocabulary of 2^19 over eight blocks
 constexpr float SF_SPAN = 24.f;                          // the bins reach e^-24 below the largest; the last holds all that is below
 constexpr double SF_FIXED = 17592186044416.0;            // 2^44
@@ -78,6 +79,7 @@ struct SfShared {
     SfFound found;
     SfCut cut;
     unsigned lo_key, hi_key;                             // the smallest and largest key of some bins
+    unsigned sort_lo, sort_hi;                           // ... and of a list
     int listed;
     int owner, owner2;
     int kept;
@@ -116,6 +118,15 @@ struct SfRow {
         const double x = fma((double)v - (double)largest, steps, 6755399441055744.0 - __hiloint2double(0x43380000 + (n >> 31), n));      // half a step, and what 32 bits round
         constexpr double A = SF_STEP, A2 = A * A / 2, A3 = A2 * A / 3, A4 = A3 * A / 4, A5 = A4 * A / 5;
         const double e = powers[n & 31] * fma(x, fma(x, fma(x, fma(x, fma(x, A5, A4), A3), A2), A), 1.0);
+        return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
+    }
+    // 2^(x / 32) for x from -2^15 to 0, to some 1e-11 of its value
+    __device__ __forceinline__ double power(double x) const {
+        const double sum = x + 6755399441055744.0;       // 1.5 2^52, as above
+        const int n = __double2loint(sum);
+        const double y = x - (sum - 6755399441055744.0);
+        constexpr double A = SF_STEP, A2 = A * A / 2, A3 = A2 * A / 3, A4 = A3 * A / 4;
+        const double e = powers[n & 31] * fma(y, fma(y, fma(y, fma(y, A4, A3), A2), A), 1.0);
         return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
     }
     // Calls f(column, value) for the block's columns whose value is `floor` or more, a thread every SF_THREADS-th.
@@ -173,10 +184,10 @@ struct SfBins {
             most = r.weight(sf_value(top));
             least = r.weight(sf_value(top - lo < span ? lo : top - span));
         } else {
-            const bool plain = step > 0.f && step < 1e30f;
-            const double wide = 1.0 / ((double)step * (1.0 - 1e-6)), narrow = 1.0 / ((double)step * (1.0 + 1e-6));
-            most = b == 0 || !plain ? 1.0 : exp(-(double)b * narrow * r.inv);
-            least = b == SF_BINS - 1 || !plain ? 0.0 : exp(-(double)(b + 1) * wide * r.inv);
+            const bool plain = step > 0.f && step < 1e30f;               // then an edge is a multiple of 24 / 2,047 whatever the temperature
+            constexpr double EDGE = (double)SF_SPAN / (SF_BINS - 1), WIDE = 3e-5;
+            most = b == 0 || !plain ? 1.0 : fmin(r.power(-EDGE / SF_STEP * b) * (1.0 + WIDE), 1.0);
+            least = b == SF_BINS - 1 || !plain ? 0.0 : r.power(-EDGE / SF_STEP * (b + 1)) * (1.0 - WIDE);
         }
     }
 };
@@ -212,34 +223,98 @@ template <typename V> __device__ __forceinline__ V sf_scan(V v, V* per_warp, V* 
     return warp ? before + v : v;
 }
 
-// Sorts list[0 .. n), largest first; n up to SF_LIST. A few entries go to where as many are larger; more by exchanges, those
-// within 64 neighbours by one warp each.
-__device__ void sf_sort(unsigned long long* list, int n) {
+// Sorts the list's first n entries (no two alike), largest first; n up to SF_LIST. A few go to where as many are larger. More go by their upper words
+// to SF_BINS buckets of equal width between the smallest and the largest, and within those to where as many are larger; where a bucket holds more
+// than SF_FULL (ties), all by exchanges, those within 64 neighbours by one warp each. 2,048 entries: 3 us by buckets, 15 by exchanges.
+__device__ void sf_sort(SfShared& s, int n) {
+    unsigned long long* list = s.list;
+    const int tid = threadIdx.x;
+    if (n > SF_SMALL) {
+        if (tid == 0) { s.sort_lo = 0xffffffffu; s.sort_hi = 0u; }
+        for (int i = tid; i < SF_BINS; i += SF_THREADS) s.counts[i] = 0u;
+    }
     __syncthreads();
     if (n <= SF_SMALL) {
         // four threads an entry, a quarter of the others each
-        const int i = threadIdx.x >> 2;
+        const int i = tid >> 2;
         const unsigned long long mine = i < n ? list[i] : 0ull;
         int rank = 0;
         if (i < n)
-            for (int j = threadIdx.x & 3; j < n; j += 4) rank += list[j] > mine ? 1 : 0;
+            for (int j = tid & 3; j < n; j += 4) rank += list[j] > mine ? 1 : 0;
         rank += __shfl_xor_sync(0xffffffffu, rank, 1);
         rank += __shfl_xor_sync(0xffffffffu, rank, 2);
         __syncthreads();
-        if (i < n && (threadIdx.x & 3) == 0) list[rank] = mine;          // entries differ: their indices do
+        if (i < n && (tid & 3) == 0) list[rank] = mine;          // entries differ: their indices do
+        __syncthreads();
+        return;
+    }
+    constexpr int EACH = SF_LIST / SF_THREADS;
+    unsigned long long mine[EACH];
+    unsigned lo = 0xffffffffu, hi = 0u;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const int i = tid + k * SF_THREADS;
+        mine[k] = i < n ? list[i] : 0ull;
+        if (i < n) { lo = min(lo, (unsigned)(mine[k] >> 32)); hi = max(hi, (unsigned)(mine[k] >> 32)); }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if ((tid & 31) == 0) { atomicMin(&s.sort_lo, lo); atomicMax(&s.sort_hi, hi); }
+    __syncthreads();
+    lo = s.sort_lo;
+    hi = s.sort_hi;
+    int shift = 0;
+    while (((hi - lo) >> shift) >= (unsigned)SF_BINS) ++shift;
+    unsigned bucket[EACH], slot[EACH];
+    bool full = false;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        if (tid + k * SF_THREADS >= n) continue;
+        bucket[k] = (hi - (unsigned)(mine[k] >> 32)) >> shift;
+        slot[k] = atomicAdd(&s.counts[bucket[k]], 1u);
+        full = full || slot[k] >= (unsigned)SF_FULL;
+    }
+    if (!__syncthreads_or(full)) {
+        constexpr int BINS = SF_BINS / SF_THREADS;
+        unsigned c[BINS], sum = 0, total;
+#pragma unroll
+        for (int k = 0; k < BINS; ++k) { c[k] = s.counts[tid * BINS + k]; sum += c[k]; }
+        unsigned before = sf_scan(sum, s.warp_count, &total) - sum;          // behind its barriers every thread has its counts
+#pragma unroll
+        for (int k = 0; k < BINS; ++k) { s.counts[tid * BINS + k] = before; before += c[k]; }
+        __syncthreads();
+        unsigned first[EACH], end[EACH];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            if (tid + k * SF_THREADS >= n) continue;
+            first[k] = s.counts[bucket[k]];
+            end[k] = bucket[k] + 1 < (unsigned)SF_BINS ? s.counts[bucket[k] + 1] : (unsigned)n;
+            list[first[k] + slot[k]] = mine[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            if (tid + k * SF_THREADS >= n) continue;
+            unsigned at = first[k];
+            for (unsigned i = first[k]; i < end[k]; ++i) at += list[i] > mine[k] ? 1u : 0u;
+            first[k] = at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+            if (tid + k * SF_THREADS < n) list[first[k]] = mine[k];
         __syncthreads();
         return;
     }
     int size = 512;
     while (size < n) size <<= 1;
-    for (int i = threadIdx.x; i < size; i += SF_THREADS)
+    for (int i = tid; i < size; i += SF_THREADS)
         if (i >= n) list[i] = 0ull;
     __syncthreads();
-    const int t = threadIdx.x;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            if (t < size / 2) {
-                const int i = 2 * (t & ~(j - 1)) + (t & (j - 1));
+            if (tid < size / 2) {
+                const int i = 2 * (tid & ~(j - 1)) + (tid & (j - 1));
                 const unsigned long long a = list[i], b = list[i + j];
                 if (((i & k) == 0) ? a < b : a > b) { list[i] = b; list[i + j] = a; }
             }
@@ -263,22 +338,20 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
     const int tid = threadIdx.x;
     if (cluster.block_rank() == 0 && tid == 0) { s.owner = SF_BINS; s.owner2 = SF_BINS; s.kept = -1; }
     cluster.sync();
-    if (cluster.block_rank() != 0) {
-        SfShared* home = cluster.map_shared_rank(&s, 0);
-        for (int i = tid; i < SF_BINS; i += SF_THREADS) {
-            const unsigned c = s.counts[i];
-            if (c != 0u) atomicAdd(&home->counts[i], c);
-        }
-    }
-    cluster.sync();
     if (cluster.block_rank() == 0) {
-        constexpr int EACH = SF_BINS / SF_THREADS;
+        constexpr int EACH = 2;
+        static_assert(EACH * SF_THREADS == SF_BINS, "two bins a thread");
         const bool by_weight = want == 0u;
-        unsigned c[EACH], count = 0, total_c;
+        unsigned c[EACH] = {0u, 0u}, count = 0, total_c;
+        uint2 theirs[SF_MAX_CLUSTER];                    // fetched, not added up here by the others' atomics, which took three times as long
+#pragma unroll
+        for (int k = 0; k < SF_MAX_CLUSTER; ++k)
+            theirs[k] = k < (int)cluster.num_blocks() ? reinterpret_cast<const uint2*>(cluster.map_shared_rank(&s, k)->counts)[tid] : make_uint2(0u, 0u);
+#pragma unroll
+        for (int k = 0; k < SF_MAX_CLUSTER; ++k) { c[0] += theirs[k].x; c[1] += theirs[k].y; }
         double least[EACH], most[EACH], lower = 0.0, upper = 0.0, unused;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            c[j] = s.counts[tid * EACH + j];
             count += c[j];
             least[j] = most[j] = 0.0;
             if (by_weight && c[j]) {
@@ -494,7 +567,7 @@ template <typename F> __device__ int sf_first(SfShared& s, int n, F cuts) {
 
 // The whole choice from the first block's list of the n largest.
 __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, double top_p, double min_p, double u, unsigned long long all) {
-    sf_sort(s.list, n);
+    sf_sort(s, n);
     int kept = n;
     if (top_k > 0 && top_k < n) {
         const unsigned kth = sf_key_of(s.list[top_k - 1]);
@@ -511,7 +584,7 @@ __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, 
     if (min_p > 0.0) kept = sf_first(s, kept, [&](unsigned long long x) { return r.weight(sf_value(sf_key_of(x))) < min_p; });
     // In the vocabulary's order: the index above the key, turned around so that the largest entry is the lowest index.
     for (int i = threadIdx.x; i < kept; i += SF_THREADS) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
-    sf_sort(s.list, kept);
+    sf_sort(s, kept);
     double e[SF_EACH], mine = 0.0, total;
 #pragma unroll
     for (int j = 0; j < SF_EACH; ++j) {
@@ -569,7 +642,7 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
             sf_gather(cluster, s, r, bins, cut, from, to);
             if (cluster.block_rank() == 0) {
                 const int n = (int)within;
-                sf_sort(s.list, n);
+                sf_sort(s, n);
                 int last;                                // the last entry that is left
                 if (by_weight) last = sf_kept_by_weight(s, r, n, weight_above, top_p, all) - 1;
                 else last = min(n - 1, max(0, (int)(want - f.above) - 1));
@@ -776,10 +849,10 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
     if (by_p) {
         sf_clear(s);
         unsigned long long all = 0, unused = 0;
+        const bool cuts = top_k > 0;
         r.each(sf_floor(cut), [&](int i, float v) {
-            const unsigned key = sf_key(v);
-            if (!sf_left(cut, key, r.first + i)) return;
-            atomicAdd(&s.counts[bins.of(v, key)], 1u);
+            if (cuts && !sf_left(cut, sf_key(v), r.first + i)) return;
+            atomicAdd(&s.counts[bins.of(v, 0u)], 1u);
             all += sf_fixed(r.weight(v));
         });
         sf_sum(cluster, s, all, unused);
