@@ -39,6 +39,7 @@ constexpr int SF_THREADS = 1024, SF_WARPS = SF_THREADS / 32;
 constexpr int SF_BINS = 2048, SF_LIST = 2048, SF_MAX_CLUSTER = 8;
 constexpr int SF_SMALL = 256;                            // lists up to here are ordered by counting
 constexpr int SF_FULL = 48;                              // entries of a bucket that are ordered among themselves
+constexpr int SF_DEEP = 8, SF_BATCH = SF_DEEP * SF_THREADS;      // loads a thread asks for at once
 constexpr int SF_ROWS = 64;                              // rows of 32 columns a warp has at most: a share of 2^16, a vocabulary of 2^19 over eight blocks
 constexpr float SF_SPAN = 24.f;                          // the bins reach e^-24 below the largest; the last holds all that is below
 constexpr double SF_FIXED = 17592186044416.0;            // 2^44
@@ -54,7 +55,7 @@ struct SfParams {
     const double* uniform;
     int rows, vocab;
     int share;                                           // columns a block of the cluster has (the last may have fewer)
-    int cached;                                          // of them in shared memory; the rest is read again from the row
+    int cached;                                          // of them in shared memory, all or whole batches; the rest is read again from the row
 };
 
 struct SfTop { float v; int nan; };
@@ -120,32 +121,21 @@ struct SfRow {
         const double e = powers[n & 31] * fma(x, fma(x, fma(x, fma(x, fma(x, A5, A4), A3), A2), A), 1.0);
         return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
     }
-    // 2^(x / 32) for x from -2^15 to 0, to some 1e-11 of its value
-    __device__ __forceinline__ double power(double x) const {
-        const double sum = x + 6755399441055744.0;       // 1.5 2^52, as above
-        const int n = __double2loint(sum);
-        const double y = x - (sum - 6755399441055744.0);
-        constexpr double A = SF_STEP, A2 = A * A / 2, A3 = A2 * A / 3, A4 = A3 * A / 4;
-        const double e = powers[n & 31] * fma(y, fma(y, fma(y, fma(y, A4, A3), A2), A), 1.0);
-        return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
-    }
     // Calls f(column, value) for the block's columns whose value is `floor` or more, a thread every SF_THREADS-th.
     template <typename F> __device__ __forceinline__ void each(float floor, F f) const {
-        constexpr int DEEP = 8;
-        if (cached == n) {
-            for (int base = threadIdx.x; base < n; base += DEEP * SF_THREADS) {
-                float v[DEEP];
+        for (int first = 0; first < n; first += SF_BATCH) {
+            const int base = first + threadIdx.x;
+            float v[SF_DEEP];
+            if (first < cached) {
 #pragma unroll
-                for (int k = 0; k < DEEP; ++k) v[k] = base + k * SF_THREADS < n ? cache[base + k * SF_THREADS] : -INFINITY;
+                for (int k = 0; k < SF_DEEP; ++k) v[k] = base + k * SF_THREADS < n ? cache[base + k * SF_THREADS] : -INFINITY;
+            } else {
 #pragma unroll
-                for (int k = 0; k < DEEP; ++k)
-                    if (v[k] >= floor) f(base + k * SF_THREADS, v[k]);
+                for (int k = 0; k < SF_DEEP; ++k) v[k] = base + k * SF_THREADS < n ? row[base + k * SF_THREADS] : -INFINITY;
             }
-        } else {
-            for (int i = threadIdx.x; i < n; i += SF_THREADS) {
-                const float v = at(i);
-                if (v >= floor) f(i, v);
-            }
+#pragma unroll
+            for (int k = 0; k < SF_DEEP; ++k)
+                if (v[k] >= floor) f(base + k * SF_THREADS, v[k]);
         }
     }
 };
@@ -156,41 +146,47 @@ __device__ __forceinline__ bool sf_left(const SfCut& cut, unsigned key, int inde
 }
 __device__ __forceinline__ float sf_floor(const SfCut& cut) { return cut.key == 0u ? SF_LOWEST : fmaxf(SF_LOWEST, sf_value(cut.key)); }
 
-// A level's bins: equal steps below the largest at first, then equal steps of the key between two keys.
+// A level's bins: equal steps of the value down from the largest in question, or of the key.
 struct SfBins {
     bool by_key;
-    float largest, step;                                 // bin = (largest - v) step
-    unsigned lo, hi;                                     // keys that count; bin = (hi - key) >> shift
+    float most, least, step;                             // bin = (most - v) step; the last holds all that is below too
+    unsigned lo, hi;                                     // the same as keys; bin = (hi - key) >> shift
     int shift;
-    __device__ __forceinline__ int of(float v, unsigned key) const {
-        if (by_key) return key < lo || key > hi ? -1 : (int)((hi - key) >> shift);
-        const float x = (largest - v) * step;
+    __device__ __forceinline__ int of(float v) const {
+        if (by_key) return (int)((hi - sf_key(v)) >> shift);
+        const float x = (most - v) * step;
         return x < (float)(SF_BINS - 1) ? (int)x : (x == x ? SF_BINS - 1 : 0);
     }
-    // No value below this is in the bins down to b.
-    __device__ __forceinline__ float floor(int b) const {
-        if (b >= SF_BINS - 1) return SF_LOWEST;
+    // No value above top(b), or below bottom(b), is in bin b (32-bit steps: an edge may lie a few roundings off).
+    __device__ __forceinline__ float top(int b) const {
+        if (by_key) return sf_value(hi - ((unsigned)b << shift));
+        const float reach = (float)b / step * 0.999999f;
+        return b > 0 && reach < FLT_MAX ? fminf(most, most - reach + fabsf(most) * 2.4e-7f) : most;
+    }
+    __device__ __forceinline__ float bottom(int b) const {
+        if (b >= SF_BINS - 1) return least;
         if (by_key) {
             const unsigned span = (((unsigned)b + 1u) << shift) - 1u;
-            return fmaxf(SF_LOWEST, sf_value(hi - lo < span ? lo : hi - span));
+            return sf_value(hi - lo < span ? lo : hi - span);
         }
-        const float reach = (float)(b + 1) / step;       // infinite where the steps are nothing
-        return fmaxf(SF_LOWEST, largest - reach * 1.00001f - fabsf(largest) * 1e-6f);
+        return fmaxf(least, most - (float)(b + 1) / step * 1.000001f - fabsf(most) * 2.4e-7f);       // (infinite where the steps are nothing)
     }
-    // Bounds of a token's weight in bin b (32-bit steps: an edge may lie a few roundings off).
-    __device__ __forceinline__ void bounds(const SfRow& r, int b, double& least, double& most) const {
-        if (by_key) {
-            const unsigned top = hi - ((unsigned)b << shift), span = (1u << shift) - 1u;
-            most = r.weight(sf_value(top));
-            least = r.weight(sf_value(top - lo < span ? lo : top - span));
-        } else {
-            const bool plain = step > 0.f && step < 1e30f;               // then an edge is a multiple of 24 / 2,047 whatever the temperature
-            constexpr double EDGE = (double)SF_SPAN / (SF_BINS - 1), WIDE = 3e-5;
-            most = b == 0 || !plain ? 1.0 : fmin(r.power(-EDGE / SF_STEP * b) * (1.0 + WIDE), 1.0);
-            least = b == SF_BINS - 1 || !plain ? 0.0 : r.power(-EDGE / SF_STEP * (b + 1)) * (1.0 - WIDE);
-        }
+    // Between two values that are in question: steps of the value (keys are sparse away from zero and crowded around it) unless those are so near one
+    // another that the steps come to a few roundings.
+    __device__ __forceinline__ static SfBins between(unsigned lo, unsigned hi, bool values) {
+        SfBins b;
+        b.lo = lo;
+        b.hi = hi;
+        b.most = sf_value(hi);
+        b.least = sf_value(lo);
+        b.step = (float)(SF_BINS - 1) / (b.most - b.least);
+        b.by_key = !(values && b.most - b.least > fmaxf(fabsf(b.most), fabsf(b.least)) / 64.f && b.step > 1e-30f && b.step < 1e30f);
+        b.shift = 0;
+        while (((hi - lo) >> b.shift) >= (unsigned)SF_BINS) ++b.shift;
+        return b;
     }
 };
+constexpr int SF_LEVELS = 8;                             // from here on by keys, whose number at least halves from level to level
 
 // e in fixed point: 2^52 added, the sum's last bits are the whole number.
 __device__ __forceinline__ unsigned long long sf_fixed(double e) {
@@ -332,9 +328,10 @@ __device__ __forceinline__ void sf_clear(SfShared& s) {
 
 // The counts of every block added up in the first, and there the bins in which the cut may be: by count (`want` > 0) the one in which it reaches
 // `want`; by weight from the first in which it may reach top_p of `all` to the first in which it does. `above` and `weight_above` lie above the
-// level's keys. Where nothing reaches it (fewer tokens, or rounding) the last bin that holds a token. Every block leaves with `found`.
+// level's keys; `whole`: all is in the level's bins, so what lies down to a bin is bounded by what lies below it too: the bounds are as near as a
+// bin is wide, of the smaller of the two. Where nothing reaches it (fewer tokens, or rounding) the last bin that holds a token. Every block leaves with `found`.
 __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, unsigned want, double top_p, unsigned above,
-                        unsigned long long weight_above, unsigned long long all) {
+                        unsigned long long weight_above, unsigned long long all, bool whole) {
     const int tid = threadIdx.x;
     if (cluster.block_rank() == 0 && tid == 0) { s.owner = SF_BINS; s.owner2 = SF_BINS; s.kept = -1; }
     cluster.sync();
@@ -349,13 +346,14 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
             theirs[k] = k < (int)cluster.num_blocks() ? reinterpret_cast<const uint2*>(cluster.map_shared_rank(&s, k)->counts)[tid] : make_uint2(0u, 0u);
 #pragma unroll
         for (int k = 0; k < SF_MAX_CLUSTER; ++k) { c[0] += theirs[k].x; c[1] += theirs[k].y; }
-        double least[EACH], most[EACH], lower = 0.0, upper = 0.0, unused;
+        double least[EACH], most[EACH], lower = 0.0, upper = 0.0, all_lower = 0.0, all_upper = 0.0;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             count += c[j];
             least[j] = most[j] = 0.0;
             if (by_weight && c[j]) {
-                bins.bounds(r, tid * EACH + j, least[j], most[j]);
+                most[j] = r.weight(bins.top(tid * EACH + j));
+                least[j] = r.weight(bins.bottom(tid * EACH + j));
                 least[j] = fmax(least[j] * c[j] * (1.0 - 1e-9) * SF_FIXED - 0.5 * c[j], 0.0);            // each rounded to a whole number
                 most[j] = most[j] * c[j] * (1.0 + 1e-9) * SF_FIXED + 0.5 * c[j];
             }
@@ -365,8 +363,8 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
         unsigned run_c = above + sf_scan(count, s.warp_count, &total_c) - count;
         double run_l = 0.0, run_u = 0.0;
         if (by_weight) {
-            run_l = (double)weight_above + sf_scan(lower, s.warp_sum, &unused) - lower;
-            run_u = (double)weight_above + sf_scan(upper, s.warp_sum2, &unused) - upper;
+            run_l = (double)weight_above + sf_scan(lower, s.warp_sum, &all_lower) - lower;
+            run_u = (double)weight_above + sf_scan(upper, s.warp_sum2, &all_upper) - upper;
         }
         const double target = top_p * (double)all;
         unsigned at[EACH];                               // tokens above each bin
@@ -379,8 +377,9 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
             if (c[j]) {
                 const int b = tid * EACH + j;
                 atomicMax(&s.kept, b);
-                if (by_weight ? run_u * (1.0 + 1e-12) >= target : run_c >= want) atomicMin(&s.owner, b);
-                if (by_weight ? run_l * (1.0 - 1e-12) >= target : run_c >= want) atomicMin(&s.owner2, b);
+                const double no_more = whole ? fmin(run_u, (double)all - (all_lower - run_l)) : run_u, no_less = whole ? fmax(run_l, (double)all - (all_upper - run_u)) : run_l;
+                if (by_weight ? no_more * (1.0 + 1e-12) >= target : run_c >= want) atomicMin(&s.owner, b);
+                if (by_weight ? no_less * (1.0 - 1e-12) >= target : run_c >= want) atomicMin(&s.owner2, b);
             }
         }
         __syncthreads();
@@ -422,20 +421,8 @@ __device__ void sf_sum(cg::cluster_group& cluster, SfShared& s, unsigned long lo
     for (unsigned k = 0; k < cluster.num_blocks(); ++k) { a += s.fixed_sums[k][0]; b += s.fixed_sums[k][1]; }
 }
 
-// What is left in the bins from `from` to `to` into the first block's list (`listed` of them there, of which SF_LIST are kept): every block lists its
-// own, then asks the first for room once.
-__device__ void sf_gather(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, const SfCut& cut, int from, int to) {
-    if (threadIdx.x == 0) s.listed = 0;
-    __syncthreads();
-    r.each(fmaxf(sf_floor(cut), bins.floor(to)), [&](int i, float v) {
-        const unsigned key = sf_key(v);
-        if (!sf_left(cut, key, r.first + i)) return;
-        const int b = bins.of(v, key);
-        if (b < from || b > to) return;
-        const int at = atomicAdd(&s.listed, 1);
-        if (at < SF_LIST) s.list[at] = ((unsigned long long)key << 32) | (unsigned)~(r.first + i);
-    });
-    cluster.sync();
+// Every block's list behind the first block's (`listed` of them there, of which SF_LIST are kept): each asks the first for room once. The lists are complete.
+__device__ void sf_collect(cg::cluster_group& cluster, SfShared& s) {
     if (cluster.block_rank() != 0) {
         SfShared* home = cluster.map_shared_rank(&s, 0);
         const int mine = s.listed;
@@ -446,6 +433,21 @@ __device__ void sf_gather(cg::cluster_group& cluster, SfShared& s, const SfRow& 
             if (at + i < SF_LIST) home->list[at + i] = s.list[i];
     }
     cluster.sync();
+}
+__device__ __forceinline__ void sf_list(SfShared& s, unsigned key, int index) {
+    const int at = atomicAdd(&s.listed, 1);
+    if (at < SF_LIST) s.list[at] = ((unsigned long long)key << 32) | (unsigned)~index;
+}
+// What is left in the bins down to `to` into the first block's list.
+__device__ void sf_gather(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, const SfCut& cut, int to) {
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    r.each(fmaxf(sf_floor(cut), bins.bottom(to)), [&](int i, float v) {
+        const unsigned key = sf_key(v);
+        if (sf_left(cut, key, r.first + i) && bins.of(v) <= to) sf_list(s, key, r.first + i);
+    });
+    cluster.sync();
+    sf_collect(cluster, s);
 }
 
 // The first index, over the whole row in order, whose running total of `weight_of(column, value)` (nothing below `floor`) exceeds the target that
@@ -609,79 +611,99 @@ __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, 
     return (int)~(unsigned)(s.list[at] >> 32);
 }
 
-// The exact cut inside the bins that a histogram found: every block leaves with it in `s.cut`. `weight_above` lies above the level's keys.
+// The exact cut inside the bins that a histogram found: every block leaves with it in `s.cut`. Every pass over the row adds up exactly what lies above the
+// keys that are still in question (of the last pass's, that is) and lists those, or where they are too many counts them in bins of their own.
 __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& r, SfBins bins, const SfCut cut, unsigned want, double top_p,
-                          unsigned long long weight_above, unsigned long long all) {
-    SfShared* home = cluster.map_shared_rank(&s, 0);
+                          unsigned long long all) {
     const bool by_weight = want == 0u;
-    for (;;) {
+    unsigned lo = max(cut.key, sf_key(SF_LOWEST)), hi = sf_key(r.largest);       // the keys in question; what lies above them:
+    unsigned long long weight_above = 0;
+    unsigned above = 0;
+    for (int level = 0;; ++level) {
         const SfFound f = s.found;
-        int from = f.from, to = f.to;
         const unsigned within = f.upto - f.above;
-        if (by_weight) {
-            // What lies above the bins in question, exactly; where those are many and full, down to their middle too, which halves them.
-            const bool halve = within > (unsigned)SF_LIST && to - from > SF_BINS / 4;
-            const int middle = from + (to - from) / 2;
-            unsigned long long above = 0, down = 0;
-            r.each(fmaxf(sf_floor(cut), bins.floor(halve ? middle : from - 1)), [&](int i, float v) {
-                const unsigned key = sf_key(v);
-                if (!sf_left(cut, key, r.first + i)) return;
-                const int b = bins.of(v, key);
-                if (b < 0 || b > (halve ? middle : from - 1)) return;
+        unsigned low = max(sf_key(bins.bottom(f.to)), lo), high = min(sf_key(bins.top(f.from)), hi);
+        const float was = sf_value(hi);
+        float least = sf_value(low), most = sf_value(high);
+        const bool list = within <= (unsigned)SF_LIST;
+        if (!list && by_weight && level > 0 && (bins.by_key ? high - low > (hi - lo) / 2 : most - least > 0.5f * (was - sf_value(lo)))) {
+            // Bounds that leave more than half of what was in question (weights far apart in a bin): half of it, exactly.
+            const unsigned middle = bins.by_key ? low + (high - low) / 2 : min(max(sf_key(0.5f * most + 0.5f * least), low), high - 1);
+            const float half = sf_value(middle);
+            unsigned long long a = 0, b = 0, na = 0, nb = 0;
+            r.each(least, [&](int, float v) {
+                if (v > was || v <= half) return;
                 const unsigned long long w = sf_fixed(r.weight(v));
-                if (b < from) above += w; else down += w;
+                if (v > most) { a += w; ++na; } else { b += w; ++nb; }
             });
-            sf_sum(cluster, s, above, down);
-            weight_above += above;
-            if (halve) {
-                if (sf_reached(weight_above + down, top_p, all)) to = middle;
-                else { from = middle + 1; weight_above += down; }
+            sf_sum(cluster, s, a, b);
+            cluster.sync();                              // the sums have been read
+            sf_sum(cluster, s, na, nb);
+            weight_above += a;
+            above += (unsigned)na;
+            if (sf_reached(weight_above + b, top_p, all)) {
+                low = middle + 1;
+                least = sf_value(low);
+            } else {
+                weight_above += b;
+                above += (unsigned)nb;
+                high = middle;
+                most = half;
             }
-        }
-        if (within <= (unsigned)SF_LIST) {
-            sf_gather(cluster, s, r, bins, cut, from, to);
-            if (cluster.block_rank() == 0) {
-                const int n = (int)within;
-                sf_sort(s, n);
-                int last;                                // the last entry that is left
-                if (by_weight) last = sf_kept_by_weight(s, r, n, weight_above, top_p, all) - 1;
-                else last = min(n - 1, max(0, (int)(want - f.above) - 1));
-                if (threadIdx.x == 0) {
-                    SfCut c;
-                    c.key = sf_key_of(s.list[last]);
-                    c.index = by_weight ? (int)~(unsigned)s.list[last] : 0x7fffffff;
-                    for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->cut = c;
-                }
-            }
+            hi = high;
             cluster.sync();
-            return;
         }
-        if (cluster.block_rank() == 0 && threadIdx.x == 0) { s.lo_key = 0xffffffffu; s.hi_key = 0u; }
-        cluster.sync();
-        unsigned lo = 0xffffffffu, hi = 0u;
-        r.each(fmaxf(sf_floor(cut), bins.floor(to)), [&](int i, float v) {
-            const unsigned key = sf_key(v);
-            if (!sf_left(cut, key, r.first + i)) return;
-            const int b = bins.of(v, key);
-            if (b < from || b > to) return;
-            lo = min(lo, key);
-            hi = max(hi, key);
+        const float top = sf_value(hi);
+        bins = SfBins::between(low, high, level < SF_LEVELS);
+        if (threadIdx.x == 0) s.listed = 0;
+        sf_clear(s);
+        unsigned long long weight = 0, number = 0;
+        r.each(least, [&](int i, float v) {
+            if (v > top) return;
+            if (v > most) {
+                if (by_weight) weight += sf_fixed(r.weight(v));
+                ++number;
+                return;
+            }
+            if (list) sf_list(s, sf_key(v), r.first + i);
+            else atomicAdd(&s.counts[bins.of(v)], 1u);
         });
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
-        if ((threadIdx.x & 31) == 0 && lo <= hi) { atomicMin(&home->lo_key, lo); atomicMax(&home->hi_key, hi); }
-        cluster.sync();
-        lo = home->lo_key;
-        hi = home->hi_key;
-        cluster.sync();
-        if (lo >= hi) {                                  // more equal tokens than the list holds
+        sf_sum(cluster, s, weight, number);
+        weight_above += weight;
+        above += (unsigned)number;
+        lo = low;
+        hi = high;
+        if (list) {
+            sf_collect(cluster, s);
+            const int n = cluster.map_shared_rank(&s, 0)->listed;        // more than the bins held where their edges are not exact
+            if (n <= SF_LIST) {
+                if (cluster.block_rank() == 0) {
+                    sf_sort(s, n);
+                    int last;                            // the last entry that is left
+                    if (by_weight) last = sf_kept_by_weight(s, r, n, weight_above, top_p, all) - 1;
+                    else last = min(n - 1, max(0, (int)(want - above) - 1));
+                    if (threadIdx.x == 0) {
+                        SfCut c;
+                        c.key = sf_key_of(s.list[last]);
+                        c.index = by_weight ? (int)~(unsigned)s.list[last] : 0x7fffffff;
+                        for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->cut = c;
+                    }
+                }
+                cluster.sync();
+                return;
+            }
+            sf_clear(s);
+            r.each(least, [&](int, float v) {
+                if (v <= most) atomicAdd(&s.counts[bins.of(v)], 1u);
+            });
+        } else if (low == high) {                        // more equal tokens than the list holds
             SfCut c;
-            c.key = lo;
+            c.key = low;
             c.index = 0x7fffffff;
             if (by_weight) {
                 // The first `keep` of them: the smallest number that reaches top_p, one at least.
-                const unsigned long long e = sf_fixed(r.weight(sf_value(lo)));
-                const int tied = (int)within;            // (of a halved level fewer may be there: the count below stops at the last)
+                const unsigned long long e = sf_fixed(r.weight(least));
+                const int tied = (int)within;            // (after a halving fewer may be there: the count below stops at the last)
                 int keep = tied;
                 if (e > 0) {
                     const double some = ceil((top_p * (double)all - (double)weight_above) / (double)e);
@@ -689,30 +711,17 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
                     while (keep > 1 && sf_reached(weight_above + (unsigned long long)(keep - 1) * e, top_p, all)) --keep;
                     while (keep < tied && !sf_reached(weight_above + (unsigned long long)keep * e, top_p, all)) ++keep;
                 }
-                const int at = sf_locate(cluster, s, r, fmaxf(SF_LOWEST, sf_value(lo)), [&](int i, float v) {
-                    return sf_key(v) == lo && sf_left(cut, lo, r.first + i) ? 1.0 : 0.0;
-                }, [&](double) { return (double)keep - 0.5; });
+                const int at = sf_locate(cluster, s, r, least, [&](int, float v) { return sf_key(v) == low ? 1.0 : 0.0; },
+                                         [&](double) { return (double)keep - 0.5; });
                 if (at >= 0)
-                    for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->cut = SfCut{lo, r.first + at};
+                    for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->cut = SfCut{low, r.first + at};
             } else if (threadIdx.x == 0) {
                 s.cut = c;
             }
             cluster.sync();
             return;
         }
-        bins.by_key = true;
-        bins.lo = lo;
-        bins.hi = hi;
-        bins.shift = 0;
-        while (((hi - lo) >> bins.shift) >= (unsigned)SF_BINS) ++bins.shift;
-        sf_clear(s);
-        r.each(fmaxf(SF_LOWEST, sf_value(lo)), [&](int i, float v) {
-            const unsigned key = sf_key(v);
-            if (!sf_left(cut, key, r.first + i)) return;
-            const int b = bins.of(v, key);
-            if (b >= 0) atomicAdd(&s.counts[b], 1u);
-        });
-        sf_find(cluster, s, r, bins, want, top_p, f.above, weight_above, all);
+        sf_find(cluster, s, r, bins, want, top_p, above, weight_above, all, false);
     }
 }
 
@@ -743,21 +752,21 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
     float most = -INFINITY;
     bool nan = false;
     {
-        const int head = min(r.n, (4 - ahead) & 3), fours = r.cached == r.n ? (r.n - head) / 4 : 0;
+        const int head = min(r.n, (4 - ahead) & 3), fours = (r.n - head) / 4;
         const float4* src = reinterpret_cast<const float4*>(r.row + head);
         float4* dst = reinterpret_cast<float4*>(cache + head);
-        constexpr int DEEP = 8;
-        for (int base = 0; base < fours; base += DEEP * SF_THREADS) {
-            float4 x[DEEP];
+        const int kept = r.cached == r.n ? fours : (r.cached - head + 3) / 4;          // the last may reach three columns beyond
+        for (int base = 0; base < fours; base += SF_BATCH) {
+            float4 x[SF_DEEP];
 #pragma unroll
-            for (int k = 0; k < DEEP; ++k) {
+            for (int k = 0; k < SF_DEEP; ++k) {
                 const int i = base + k * SF_THREADS + tid;
-                x[k] = i < fours ? __ldcs(src + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                x[k] = i < fours ? src[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             }
 #pragma unroll
-            for (int k = 0; k < DEEP; ++k) {
+            for (int k = 0; k < SF_DEEP; ++k) {
                 const int i = base + k * SF_THREADS + tid;
-                if (i < fours) dst[i] = x[k];
+                if (i < kept) dst[i] = x[k];
                 most = fmaxf(fmaxf(fmaxf(most, x[k].x), fmaxf(x[k].y, x[k].z)), x[k].w);
                 nan = nan || x[k].x != x[k].x || x[k].y != x[k].y || x[k].z != x[k].z || x[k].w != x[k].w;
             }
@@ -808,18 +817,19 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
     cut.key = 0u; cut.index = 0x7fffffff;
     SfBins bins;
     bins.by_key = false;
-    bins.largest = most;
+    bins.most = most;
+    bins.least = SF_LOWEST;
     bins.step = (float)((SF_BINS - 1) * r.inv / SF_SPAN);
-    bins.lo = 0u; bins.hi = 0xffffffffu; bins.shift = 0;
+    bins.lo = bins.hi = 0u; bins.shift = 0;
     const bool by_p = top_p < 1.0;
     if (top_k > 0) {
         if (top_k <= SF_LIST / 2) {
             sf_clear(s);
-            if (own > -INFINITY) atomicAdd(&s.counts[bins.of(own, sf_key(own))], 1u);
-            sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull);
+            if (own > -INFINITY) atomicAdd(&s.counts[bins.of(own)], 1u);
+            sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull, false);
             if (s.found.upto >= (unsigned)top_k) {
                 const int down = s.found.to;
-                sf_gather(cluster, s, r, bins, cut, 0, down);
+                sf_gather(cluster, s, r, bins, cut, down);
                 const int listed = cluster.map_shared_rank(&s, 0)->listed;
                 if (listed <= SF_LIST) {
                     cluster.sync();                      // the first block's count has been read
@@ -832,18 +842,18 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
             }
         }
         sf_clear(s);
-        r.each(SF_LOWEST, [&](int, float v) { atomicAdd(&s.counts[bins.of(v, 0u)], 1u); });
-        sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull);
+        r.each(SF_LOWEST, [&](int, float v) { atomicAdd(&s.counts[bins.of(v)], 1u); });
+        sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull, false);
         if (s.found.upto <= (unsigned)SF_LIST) {
             const int n = (int)(s.found.upto);
-            sf_gather(cluster, s, r, bins, cut, 0, s.found.to);
+            sf_gather(cluster, s, r, bins, cut, s.found.to);
             if (rank == 0) {
                 const int token = sf_draw_from_list(s, r, n, top_k, by_p ? top_p : 1.0, min_p, u, 0ull);
                 if (tid == 0) p.tokens[row] = token;
             }
             return;
         }
-        sf_refine(cluster, s, r, bins, cut, (unsigned)top_k, 0.0, 0ull, 0ull);
+        sf_refine(cluster, s, r, bins, cut, (unsigned)top_k, 0.0, 0ull);
         cut = s.cut;
     }
     if (by_p) {
@@ -852,21 +862,21 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
         const bool cuts = top_k > 0;
         r.each(sf_floor(cut), [&](int i, float v) {
             if (cuts && !sf_left(cut, sf_key(v), r.first + i)) return;
-            atomicAdd(&s.counts[bins.of(v, 0u)], 1u);
+            atomicAdd(&s.counts[bins.of(v)], 1u);
             all += sf_fixed(r.weight(v));
         });
         sf_sum(cluster, s, all, unused);
-        sf_find(cluster, s, r, bins, 0u, top_p, 0u, 0ull, all);
+        sf_find(cluster, s, r, bins, 0u, top_p, 0u, 0ull, all, true);
         if (s.found.upto <= (unsigned)SF_LIST) {
             const int n = (int)(s.found.upto);
-            sf_gather(cluster, s, r, bins, cut, 0, s.found.to);
+            sf_gather(cluster, s, r, bins, cut, s.found.to);
             if (rank == 0) {
                 const int token = sf_draw_from_list(s, r, n, 0, top_p, min_p, u, all);
                 if (tid == 0) p.tokens[row] = token;
             }
             return;
         }
-        sf_refine(cluster, s, r, bins, cut, 0u, top_p, 0ull, all);
+        sf_refine(cluster, s, r, bins, cut, 0u, top_p, all);
         cut = s.cut;
     }
     // Below this a weight is under min_p for sure: no exponential.
@@ -886,8 +896,22 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
 
 using namespace kb;
 
-// Blocks a row: a share of at most SF_SHARE columns each, up to a cluster of eight.
+// Blocks a row has at most: shares of SF_SHARE columns.
 constexpr int SF_SHARE = 8192;
+
+// Clusters of `blocks` blocks that run at once; asked for once a device (their blocks fill a multiprocessor whatever their share, and lie in one part of the
+// chip: of eight blocks far fewer than the multiprocessors would hold).
+static int active_clusters(int log_blocks, cudaLaunchConfig_t cfg, size_t smem) {
+    static int known[64][4] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 1;
+    int n = device < 64 ? __atomic_load_n(&known[device][log_blocks], __ATOMIC_RELAXED) : 0;
+    if (n > 0) return n;
+    cfg.dynamicSmemBytes = smem;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_filtered_kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    if (device < 64) __atomic_store_n(&known[device][log_blocks], n, __ATOMIC_RELAXED);
+    return n;
+}
 
 extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double* temperature, const int* top_k, const double* top_p,
                                   const double* min_p, const double* uniform, int rows, int vocab, void* stream) {
@@ -896,31 +920,41 @@ extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double
     KB_REQUIRE(vocab <= (1 << 19), "sample_filtered: a vocabulary of %d (up to %d: a row's weights are added in 64 bits)", vocab, 1 << 19);
     KB_REQUIRE(rows == 0 || (tokens && logits && temperature && top_k && top_p && min_p && uniform), "sample_filtered: a null pointer");
     if (rows == 0) return 0;
-    int blocks = 1;
-    while (blocks < SF_MAX_CLUSTER && (long long)blocks * SF_SHARE < vocab) blocks *= 2;
     SfParams p = {};
     p.tokens = tokens; p.logits = logits; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p; p.uniform = uniform;
     p.rows = rows; p.vocab = vocab;
-    p.share = (vocab + blocks - 1) / blocks;
     constexpr int MOST = 232448 - 1024;
-    static_assert(sizeof(SfShared) + 65536 <= MOST, "the histogram and the list leave no room for a share");
-    p.cached = (int)(((size_t)MOST - sizeof(SfShared) - 32) / 4);
-    if (p.cached > p.share) p.cached = p.share;
-    const size_t smem = (sizeof(SfShared) + 15) / 16 * 16 + 16 + (size_t)p.cached * 4;
+    constexpr int FIXED = (int)((sizeof(SfShared) + 15) / 16 * 16) + 32;
+    constexpr int CACHED = (MOST - FIXED) / 4 / SF_BATCH * SF_BATCH;
+    static_assert(CACHED > 0, "the histogram and the list leave no room for a share");
     static unsigned long long done = 0;
     if (int e = allow_shared_memory((const void*)sample_filtered_kernel, MOST, &done)) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * blocks));
-    cfg.blockDim = dim3(SF_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)blocks;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(SF_THREADS);
+    cfg.stream = (cudaStream_t)stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    int blocks = 1;
+    double least = 0.0;
+    for (int log_blocks = 0; log_blocks < 4; ++log_blocks) {
+        const int n = 1 << log_blocks, share = (vocab + n - 1) / n;
+        if (n > 1 && n / 2 * SF_SHARE >= vocab) break;       // half as many have small shares already
+        if (share > SF_ROWS * SF_THREADS) continue;
+        attr[0].val.clusterDim.x = (unsigned)n;
+        cfg.gridDim = dim3((unsigned)n);
+        const int at_once = rows == 1 ? 1 : active_clusters(log_blocks, cfg, MOST);
+        const double us = (double)((rows + at_once - 1) / at_once) * (16.0 + 0.45e-3 * share);
+        if (least == 0.0 || us < least) { least = us; blocks = n; }
+    }
+    p.share = (vocab + blocks - 1) / blocks;
+    p.cached = p.share <= (MOST - FIXED) / 4 ? p.share : CACHED;
+    attr[0].val.clusterDim.x = (unsigned)blocks;
+    cfg.gridDim = dim3((unsigned)(rows * blocks));
+    cfg.dynamicSmemBytes = (size_t)FIXED + (size_t)p.cached * 4;
     cudaLaunchKernelEx(&cfg, sample_filtered_kernel, p);
     return check_launch("sample_filtered");
 }

@@ -89,6 +89,42 @@ def test_ties(vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [50257, 256000])
+@pytest.mark.parametrize("rows", [1, 9, 20, 45, 150])
+def test_rows_by_themselves_and_many(rows, vocab):
+    """How many blocks a row has depends on the number of rows."""
+    rng = np.random.default_rng(rows)
+    logits = rng.normal(0.0, 2.0, (rows, vocab)) + rng.choice([0.0, 20.0, -1000.0], (rows, 1))
+    kinds = [(0.8, 0, 0.99, 0.0), (1.0, 5000, 1.0, 0.0), (1.5, 0, 0.9999, 0.0), (0.7, 0, 1.0, 0.001), (1.0, 30000, 0.97, 0.0), (2.0, 0, 0.5, 0.0), (0.3, 0, 1.0, 0.0), (0.0, 7, 0.5, 0.0)]
+    check(logits, [(*kinds[(i + rows) % len(kinds)], float(u)) for i, u in enumerate(rng.random(rows))])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [6, 60])
+def test_ties_in_large_rows(rows):
+    """81 values, some 3,000 tokens of each."""
+    rng = np.random.default_rng(rows + 2)
+    logits = (rng.integers(-40, 41, (rows, 256000)) / 8.0).astype(np.float32)
+    kinds = [(1.0, 0, 0.37, 0.0), (2.0, 0, 0.999, 0.0), (1.0, 3000, 0.61, 0.0), (30.0, 0, 0.9, 0.5), (1.0, 70000, 1.0, 0.0), (10.0, 0, 0.02, 0.0)]
+    settings = [(*kinds[i % 6], float(u)) for i, u in enumerate(rng.random(rows))]
+    got, want = device_tokens(logits, settings), [exact_token(row, *s) for row, s in zip(logits, settings)]
+    assert got == want, [(i, g, w, settings[i]) for i, (g, w) in enumerate(zip(got, want)) if g != w]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [20000, 256000])
+def test_values_far_apart(vocab):
+    """Of both signs, from 1e-40 to 1e4 in size: neither equal steps of the value nor of its bits part them evenly."""
+    rng = np.random.default_rng(21)
+    logits = (rng.choice([-1.0, 1.0], (24, vocab)) * 10.0 ** rng.uniform(-40.0, 4.0, (24, vocab))).astype(np.float32)
+    logits[12:] = -np.abs(logits[12:])                       # the largest is next to nothing, and half of all lie within 1e-18 of it
+    kinds = [(2000.0, 0, 0.9, 0.0), (1.0, 0, 0.9999999, 0.0), (1e4, 0, 0.3, 0.0), (100.0, vocab // 2, 0.8, 0.0), (1e30, 0, 0.7, 0.0), (1e-20, 0, 0.6, 0.0)]
+    settings = [(*kinds[i % 6], float(u)) for i, u in enumerate(rng.random(24))]
+    got, want = device_tokens(logits, settings), [exact_token(row, *s) for row, s in zip(logits, settings)]
+    assert got == want, [(i, g, w, settings[i]) for i, (g, w) in enumerate(zip(got, want)) if g != w]
+
+
+@pytest.mark.gpu
 def test_ends_of_the_uniform_number_and_of_the_settings():
     rng = np.random.default_rng(9)
     logits = rng.normal(0.0, 2.0, (40, 9001))
