@@ -6,17 +6,19 @@
 // whose running total over what is left exceeds u times the whole. All three filters cut the same order (x down, index up), so what is
 // left is always "above a cut (key, index)".
 //
-// A row is one cluster's: its blocks read the row once and keep their shares in shared memory; everything after works on chip.
+// A row is one cluster's: its blocks read the row once and keep their shares in shared memory (of a share beyond 49,152 columns the rest is read again,
+// from the second-level cache); everything after works on chip.
 //   1. The largest logit, whether a NaN is there.
 //   2. For a top_k up to LIST / 2: as many of the threads' own largest logits lie above the cut's lower bound that a histogram of those few
 //      finds; what lies above it is gathered in the cluster's first block, sorted, cut and drawn from there. (Sorted logits may leave more
 //      than LIST above it: then as below.)
 //   3. Else a histogram of counts over 2,048 bins of equal steps of x below the largest. top_k: the bin in which the k-th lies. top_p: a
-//      bin's weight lies between its count times the weights at its ends, so the histogram bounds where the cut is to a few bins; what is
-//      above those is added up exactly (in fixed point, 44 bits behind the point: whole numbers, whose order changes nothing; a row's
-//      sum, 2^19 tokens, fits 64 bits). The bins in question, or all down to them where they hold no more than LIST tokens, are gathered and
-//      sorted for the exact cut; bins too full for that are divided again between their smallest and largest key. (Weights
-//      added up by atomics instead took 1.1 ms a row of 256,000: shared memory has none of 64 bits.)
+//      bin's weight lies between its count times the weights at its ends, so the histogram bounds where the cut is to a few bins, from above
+//      and, all weights' sum being known, from below. The bins in question, or all down to them, are gathered and sorted for the exact cut
+//      where they hold no more than LIST tokens, else counted again in 2,048 bins of their own; the same pass adds up what lies above them exactly (in
+//      fixed point, 44 bits behind the point: whole numbers, whose order changes nothing; a row's sum, 2^19 tokens, fits 64 bits). (Weights added up by
+//      atomics instead took 1.1 ms a row of 256,000: shared memory has none of 64 bits. Without the bound from below a nucleus of 0.99 took
+//      three levels and 160 us where it takes one and 50.)
 //   4. The draw goes over the whole share of every block: totals of warps, of the 32 rows of the warp's that the target falls in,
 //      then along that row.
 // e^x is in 64 bits, and so are the draw's sums, as on the host: a seed gives the tokens it gave there, but for borders that lie within a
@@ -25,9 +27,9 @@
 // clock. Two entries of T share a bank, so a warp's loads take two turns at most.
 //
 // What bounds it, over 256,000 tokens: one row alone takes 15 us under top_k 50, of which the row's load is 3 and the rest some eight cluster
-// barriers and what lies between them. 64 rows: 67 us under top_k 50 (1.0 TB/s), 110 without filters, 130 under a nucleus of 0.95 (the exponentials of
-// all tokens and the histogram's atomics), 215 under 0.99, whose cut lies among so many tokens of nearly one weight that the bins are divided
-// again. A multiprocessor holds one block, so 16 to 18 rows are under way at a time, and none while the last of them end.
+// barriers and what lies between them; 26 under a nucleus of 0.95, of which 10 are the pass that adds up all weights and counts them (64-bit
+// operations, conversions and atomics of shared memory together: two tokens' weights side by side were no faster). 64 rows: 43 us under top_k 50
+// (1.5 TB/s), 73 without filters, 87 under a nucleus of 0.95 or 0.99.
 #include <cooperative_groups.h>
 #include <cfloat>
 #include "common.cuh"
@@ -938,6 +940,10 @@ extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double
     cfg.stream = (cudaStream_t)stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    // Blocks a row: as many as make the rows' time least, which is the rounds of clusters times some 16 us and 0.45 ns a column of a share (what a
+    // nucleus takes). 15 clusters of eight run at once, 33 of four, 74 of two, 148 of one. As measured under a nucleus of 0.95 (us): 256,000 columns,
+    // of 12 rows 27 by eight blocks a row and 38 by four, of 16 rows 49 and 38, of 64 rows 116 and 76; 50,257 columns, of 12 rows 18, 20, 24 and 33 by
+    // eight, four, two and one, of 40 rows 46, 35, 25 and 34, of 256 rows 249, 141, 94 and 66.
     int blocks = 1;
     double least = 0.0;
     for (int log_blocks = 0; log_blocks < 4; ++log_blocks) {
