@@ -193,6 +193,15 @@ def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
             raise KernelError(f"{what}: a tensor on {t.device} while device {here} is the current one")
 
 
+def _as_wanted(dtype, *tensors: torch.Tensor) -> bool:
+    """Whether all are on the current device, contiguous and of this type: what the checks by name would find one by one, at a quarter of their time."""
+    here = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != here or not t.is_contiguous():
+            return False
+    return True
+
+
 def _f(x: float) -> ctypes.c_float:
     return ctypes.c_float(float(x))
 
@@ -1062,24 +1071,28 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
     count; 0 shares nothing. Up to SHARED_PREFIX_ROWS rows. Window, soft cap and `sinks` as for `paged_attention_mma`; a row that
     sees nothing gives zeros. Every page with a position that a row sees has to be in its table; what lies in it behind the row's count, or before its
     window, may be anything, but that with a window shared values which only some rows of a group still see have to be finite in bfloat16."""
-    _need(q, "shared attention q")
-    if q.dim() != 3:
-        raise KernelError(f"shared attention: q {tuple(q.shape)} is not [rows, heads, head size]")
+    if not (_as_wanted(q.dtype, q, k_table, v_table) and _as_wanted(torch.int32, block_table, row_count, share_id, share_len) and q.dim() == 3 and
+            row_count.shape == share_id.shape == share_len.shape == q.shape[:1]):
+        _need(q, "shared attention q")
+        if q.dim() != 3:
+            raise KernelError(f"shared attention: q {tuple(q.shape)} is not [rows, heads, head size]")
+        _need(k_table, "shared attention k table", q.dtype)
+        _need(v_table, "shared attention v table", q.dtype)
+        _need(block_table, "shared attention block table", torch.int32)
+        for t, what in ((row_count, "row_count"), (share_id, "share_id"), (share_len, "share_len")):
+            _need(t, f"shared attention {what}", torch.int32, (q.shape[0],))
+        _on_current_device("shared attention", q, k_table, v_table, block_table, row_count, share_id, share_len)
     rows, hq, d = q.shape
     dt = _dt(q, "shared attention q")
-    _need(k_table, "shared attention k table", q.dtype)
-    _need(v_table, "shared attention v table", q.dtype)
-    if k_table.dim() != 4 or k_table.shape[2] != page_size or k_table.shape[3] != d or v_table.dim() != 4 or v_table.shape[:3] != k_table.shape[:3]:
-        raise KernelError(f"shared attention: tables {tuple(k_table.shape)} / {tuple(v_table.shape)} are not [pages, kv_heads, {page_size}, {d}]")
-    n_pages, hkv, dv = k_table.shape[0], k_table.shape[1], v_table.shape[3]
-    _need(block_table, "shared attention block table", torch.int32)
-    if block_table.dim() != 2 or block_table.shape[0] < rows:
-        raise KernelError(f"shared attention: a block table of {tuple(block_table.shape)} for {rows} requests")
-    for t, what in ((row_count, "row_count"), (share_id, "share_id"), (share_len, "share_len")):
-        _need(t, f"shared attention {what}", torch.int32, (rows,))
+    keys, values, table = tuple(k_table.shape), tuple(v_table.shape), tuple(block_table.shape)
+    if len(keys) != 4 or keys[2] != page_size or keys[3] != d or len(values) != 4 or values[:3] != keys[:3]:
+        raise KernelError(f"shared attention: tables {keys} / {values} are not [pages, kv_heads, {page_size}, {d}]")
+    n_pages, hkv, dv = keys[0], keys[1], values[3]
+    if len(table) != 2 or table[0] < rows:
+        raise KernelError(f"shared attention: a block table of {table} for {rows} requests")
     if sinks is not None:
         _need(sinks, "shared attention sinks", torch.float32, (hq,))
-    _on_current_device("shared attention", q, k_table, v_table, block_table, row_count, share_id, share_len, sinks)
+        _on_current_device("shared attention", sinks)
     if window is not None and window < 0:
         raise KernelError(f"shared attention: a window of {window}")
     out = _fresh((rows, hq, dv), q.dtype, q.device)
@@ -1090,7 +1103,7 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
         need = _SHARED_SCRATCH[sizes] = int(lib.kb_shared_attention_scratch_floats(rows, hq, hkv, d, dv))
     scratch = _fresh((need,), torch.float32, q.device) if need else None
     _check(lib.kb_shared_attention(out.data_ptr(), q.data_ptr(), k_table.data_ptr(), v_table.data_ptr(), dt, block_table.data_ptr(), row_count.data_ptr(),
-                                   share_id.data_ptr(), share_len.data_ptr(), rows, hq, hkv, d, dv, int(page_size), block_table.shape[1], n_pages,
+                                   share_id.data_ptr(), share_len.data_ptr(), rows, hq, hkv, d, dv, int(page_size), table[1], n_pages,
                                    int(window or 0), float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
                                    None if scratch is None else scratch.data_ptr(), need, _stream()))
     return out
@@ -2123,14 +2136,16 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     whose running total exceeds `uniform`, in [0, 1), times what is left. `temperature`, `top_p`, `min_p` and `uniform` are float64 [rows], `top_k`
     int32 [rows], all on the logits' device, which has to be the current one. Nothing left (a top_p of 0 or less, a min_p above 1) gives
     token 0; logits with a NaN or an infinity among them their first largest."""
-    _need(logits, "sample_filtered logits", torch.float32)
-    if logits.dim() != 2:
-        raise KernelError(f"sample_filtered: logits {tuple(logits.shape)} are not [rows, vocab]")
+    if not (_as_wanted(torch.float64, temperature, top_p, min_p, uniform) and _as_wanted(torch.float32, logits) and _as_wanted(torch.int32, top_k) and logits.dim() == 2 and
+            temperature.shape == top_k.shape == top_p.shape == min_p.shape == uniform.shape == logits.shape[:1]):
+        _need(logits, "sample_filtered logits", torch.float32)
+        if logits.dim() != 2:
+            raise KernelError(f"sample_filtered: logits {tuple(logits.shape)} are not [rows, vocab]")
+        for t, what in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (uniform, "uniform")):
+            _need(t, f"sample_filtered {what}", torch.float64, (logits.shape[0],))
+        _need(top_k, "sample_filtered top_k", torch.int32, (logits.shape[0],))
+        _on_current_device("sample_filtered", logits, temperature, top_k, top_p, min_p, uniform)
     rows, vocab = logits.shape
-    for t, what in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (uniform, "uniform")):
-        _need(t, f"sample_filtered {what}", torch.float64, (rows,))
-    _need(top_k, "sample_filtered top_k", torch.int32, (rows,))
-    _on_current_device("sample_filtered", logits, temperature, top_k, top_p, min_p, uniform)
     out = _fresh((rows,), torch.int32, logits.device)
     _check(library().kb_sample_filtered(out.data_ptr(), logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
                                         uniform.data_ptr(), rows, vocab, _stream()))
