@@ -10,7 +10,7 @@
 // from the second-level cache); everything after works on chip.
 //   1. The largest logit, whether a NaN is there.
 //   2. For a top_k up to LIST / 2: as many of the threads' own largest logits lie above the cut's lower bound that a histogram of those few
-//      finds; what lies above it is gathered in the cluster's first block, sorted, cut and drawn from there. (Sorted logits may leave more
+//      finds (its bins reach to the least of them: where they ended at e^-24, one row in a hundred, with a token far above the rest, took 60 us for 15); what lies above it is gathered in the cluster's first block, sorted, cut and drawn from there. (Sorted logits may leave more
 //      than LIST above it: then as below.)
 //   3. Else a histogram of counts over 2,048 bins of equal steps of x below the largest. top_k: the bin in which the k-th lies. top_p: a
 //      bin's weight lies between its count times the weights at its ends, so the histogram bounds where the cut is to a few bins, from above
@@ -60,7 +60,7 @@ struct SfParams {
     int cached;                                          // of them in shared memory, all or whole batches; the rest is read again from the row
 };
 
-struct SfTop { float v; int nan; };
+struct SfTop { float v; int nan; unsigned low; };       // a block's largest logit, and the smallest key of its threads' largest
 struct SfCut { unsigned key; int index; };               // what is left: key above, or equal and the index no larger
 struct SfFound {                                         // what the first block tells the others about a histogram
     int from, to;                                        // the bins the cut may be in
@@ -79,6 +79,7 @@ struct SfShared {
     unsigned long long warp_fixed[SF_WARPS], warp_fixed2[SF_WARPS];
     unsigned warp_count[SF_WARPS];
     float warp_max[SF_WARPS];
+    unsigned warp_low[SF_WARPS];
     SfFound found;
     SfCut cut;
     unsigned lo_key, hi_key;                             // the smallest and largest key of some bins
@@ -785,17 +786,20 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
     const float own = most;                              // this thread's largest
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if ((tid & 31) == 0) s.warp_max[tid >> 5] = most;
+    unsigned low = __reduce_min_sync(0xffffffffu, own > -INFINITY ? sf_key(own) : 0xffffffffu);
+    if ((tid & 31) == 0) { s.warp_max[tid >> 5] = most; s.warp_low[tid >> 5] = low; }
     nan = __syncthreads_or(nan);
     most = s.warp_max[tid & 31];
+    low = __reduce_min_sync(0xffffffffu, s.warp_low[tid & 31]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     cluster.barrier_wait();
-    if (tid < blocks) cluster.map_shared_rank(&s, tid)->tops[rank] = SfTop{most, nan ? 1 : 0};
+    if (tid < blocks) cluster.map_shared_rank(&s, tid)->tops[rank] = SfTop{most, nan ? 1 : 0, low};
     cluster.sync();
     for (int b = 0; b < blocks; ++b) {
         most = fmaxf(most, s.tops[b].v);
         nan = nan || s.tops[b].nan != 0;
+        low = min(low, s.tops[b].low);
     }
     // Certain choices: greedy; a temperature that is no number leaves token 0, as a top_p that keeps nothing does; with a NaN among the
     // logits, an infinite one, or none above -inf the probabilities are none and the first largest stands.
@@ -825,6 +829,10 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
     bins.lo = bins.hi = 0u; bins.shift = 0;
     const bool by_p = top_p < 1.0;
     if (top_k > 0) {
+        // The k-th may lie further below the largest than any weight that counts: here the bins reach down to the least of the threads' largest, or 200
+        // below (some may have nothing but masked tokens).
+        const float weights = bins.step;
+        bins.step = (float)(SF_BINS - 1) / (most - fmaxf(sf_value(low), most - fmaxf(200.f, SF_SPAN / (float)fmax(r.inv, 1e-30))));
         if (top_k <= SF_LIST / 2) {
             sf_clear(s);
             if (own > -INFINITY) atomicAdd(&s.counts[bins.of(own)], 1u);
@@ -857,6 +865,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
         }
         sf_refine(cluster, s, r, bins, cut, (unsigned)top_k, 0.0, 0ull);
         cut = s.cut;
+        bins.step = weights;
     }
     if (by_p) {
         sf_clear(s);

@@ -125,6 +125,19 @@ def test_values_far_apart(vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [500, 30000, 256000])
+def test_a_token_far_above_the_rest(vocab):
+    """The k-th largest lies where no weight counts any more, among masked tokens or not; the nucleus is one token, or a temperature brings the rest back."""
+    rng = np.random.default_rng(vocab)
+    logits = rng.normal(0.0, 2.0, (36, vocab)).astype(np.float32)
+    logits[:, vocab // 3] = np.repeat([30.0, 300.0, 1e30], 12)
+    logits[6:12][rng.random((6, vocab)) < 0.97] = np.finfo(np.float32).min
+    logits[18:24][rng.random((6, vocab)) < 0.97] = -np.inf
+    kinds = [(0.5, 64, 0.9, 0.0), (0.5, 300, 1.0, 0.0), (50.0, 64, 0.95, 0.0), (50.0, 5000, 0.8, 0.0), (0.3, 1000, 0.999999, 0.01), (400.0, 20, 1.0, 0.0)]
+    check(logits, [(*kinds[i % 6], float(u)) for i, u in enumerate(rng.random(36))])
+
+
+@pytest.mark.gpu
 def test_ends_of_the_uniform_number_and_of_the_settings():
     rng = np.random.default_rng(9)
     logits = rng.normal(0.0, 2.0, (40, 9001))
