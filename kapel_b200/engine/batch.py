@@ -58,7 +58,7 @@ def decode_split(pairs: int, longest: int, sms: int, window: Optional[int] = Non
 
 
 # When a step of single tokens goes by `kernels.shared_prefix_attention`. In bfloat16: from so many bytes of a layer's keys and values on that need not be
-# read again. Its three kernels take 19 us where the decode kernel takes 7 at the least; as measured (us, shared and row by row, each request with
+# read again. Its three kernels take 19 us where the decode kernel takes 7 at the least (its two, where little is held at all, 9); as measured (us, shared and row by row, each request with
 # 100 positions of its own): 8 heads over 4 of 256, 8 requests sharing 4,096 positions (117 MB) 29 and 29, 16 sharing 1,024 (63 MB) 22 and 18,
 # 32 sharing 1,024 (130 MB) 22 and 29, 64 sharing 4,096 (1.1 GB) 33 and 189; 16 over 8 of 256, 16 sharing 1,024 (126 MB) 22 and 28; 32 over 16 of 128,
 # 8 sharing 1,024 (59 MB) 26 and 19, 64 sharing 256 (132 MB) 32 and 38.
