@@ -369,7 +369,7 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
             run_l = (double)weight_above + sf_scan(lower, s.warp_sum, &all_lower) - lower;
             run_u = (double)weight_above + sf_scan(upper, s.warp_sum2, &all_upper) - upper;
         }
-        const double target = top_p * (double)all;
+        const double target = top_p * (double)all, slack = 1e-12 * (double)all;         // (what 64-bit sums of up to 2,048 terms may be off by)
         unsigned at[EACH];                               // tokens above each bin
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
@@ -381,8 +381,8 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
                 const int b = tid * EACH + j;
                 atomicMax(&s.kept, b);
                 const double no_more = whole ? fmin(run_u, (double)all - (all_lower - run_l)) : run_u, no_less = whole ? fmax(run_l, (double)all - (all_upper - run_u)) : run_l;
-                if (by_weight ? no_more * (1.0 + 1e-12) >= target : run_c >= want) atomicMin(&s.owner, b);
-                if (by_weight ? no_less * (1.0 - 1e-12) >= target : run_c >= want) atomicMin(&s.owner2, b);
+                if (by_weight ? no_more + slack >= target : run_c >= want) atomicMin(&s.owner, b);
+                if (by_weight ? no_less - slack >= target : run_c >= want) atomicMin(&s.owner2, b);
             }
         }
         __syncthreads();
@@ -622,7 +622,7 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
     unsigned lo = max(cut.key, sf_key(SF_LOWEST)), hi = sf_key(r.largest);       // the keys in question; what lies above them:
     unsigned long long weight_above = 0;
     unsigned above = 0;
-    for (int level = 0;; ++level) {
+    for (int level = 0; level < SF_LEVELS + 40; ++level) {       // (the last SF_LEVELS + 32nd has one key in question)
         const SfFound f = s.found;
         const unsigned within = f.upto - f.above;
         unsigned low = max(sf_key(bins.bottom(f.to)), lo), high = min(sf_key(bins.top(f.from)), hi);
@@ -726,6 +726,8 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
         }
         sf_find(cluster, s, r, bins, want, top_p, above, weight_above, all, false);
     }
+    if (threadIdx.x == 0) s.cut = SfCut{lo, 0x7fffffff};
+    cluster.sync();
 }
 
 __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const SfParams p) {
