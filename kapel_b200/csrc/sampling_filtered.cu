@@ -82,8 +82,7 @@ struct SfShared {
     unsigned warp_low[SF_WARPS];
     SfFound found;
     SfCut cut;
-    unsigned lo_key, hi_key;                             // the smallest and largest key of some bins
-    unsigned sort_lo, sort_hi;                           // ... and of a list
+    unsigned sort_lo, sort_hi;                           // the smallest and largest upper word of a list
     int listed;
     int owner, owner2;
     int kept;
@@ -954,7 +953,8 @@ extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double
     // Blocks a row: as many as make the rows' time least, which is the rounds of clusters times some 16 us and 0.45 ns a column of a share (what a
     // nucleus takes). 15 clusters of eight run at once, 33 of four, 74 of two, 148 of one. As measured under a nucleus of 0.95 (us): 256,000 columns,
     // of 12 rows 27 by eight blocks a row and 38 by four, of 16 rows 49 and 38, of 64 rows 116 and 76; 50,257 columns, of 12 rows 18, 20, 24 and 33 by
-    // eight, four, two and one, of 40 rows 46, 35, 25 and 34, of 256 rows 249, 141, 94 and 66.
+    // eight, four, two and one, of 40 rows 46, 35, 25 and 34, of 256 rows 249, 141, 94 and 66. (Blocks of 512 threads, two a multiprocessor, eight a row of
+    // 256,000: 46 of 32 rows where four of 1,024 take 39, 85 of 64 where those take 76.)
     int blocks = 1;
     double least = 0.0;
     for (int log_blocks = 0; log_blocks < 4; ++log_blocks) {
