@@ -46,6 +46,7 @@ constexpr int SF_ROWS = 64;                              // rows of 32 columns a
 constexpr float SF_SPAN = 24.f;                          // the bins reach e^-24 below the largest; the last holds all that is below
 constexpr double SF_FIXED = 17592186044416.0;            // 2^44
 constexpr double SF_STEP = 0.6931471805599453 / 32.0;    // ln 2 / 32
+constexpr int SF_SMALLEST = -1076;                       // a weight below 2^-1075 is none
 
 struct SfParams {
     int* tokens;
@@ -103,25 +104,28 @@ struct SfRow {
     const double* powers;
     int n, cached, first;                                // columns of the share, how many are in `cache`, the share's first column
     double inv, steps;                                   // 1 / temperature, and in steps of ln 2 / 32
-    float largest, steps32, lowest;                      // below `lowest` a weight is under e^-690: none
+    float largest, half, steps32;                        // the largest, half of it; twice the steps, in 32 bits
     __device__ __forceinline__ float at(int i) const { return i < cached ? cache[i] : row[i]; }
     __device__ __forceinline__ void scale(float top, double temperature, const double* table) {
         largest = top;
-        inv = isinf(temperature) ? 0.0 : fmin(1.0 / temperature, 1e300);
-        steps = inv / SF_STEP;
-        steps32 = (float)fmin(steps, 1e38);
-        lowest = (float)fmax((double)top - 690.0 / inv, (double)-FLT_MAX);
+        inv = fmin(1.0 / temperature, 1e36);             // (of colder rows only what ties with the largest counts, as of one at 1e-36)
+        steps = inv / SF_STEP;                           // below 2^126
+        half = 0.5f * top;
+        steps32 = (float)(2.0 * steps);
         powers = table;
     }
-    // e^((v - largest) / temperature), which is at most 1
+    // e^((v - largest) / temperature), which is at most 1. The logits are subtracted before they are divided (the host rounds each quotient first). What
+    // is small is told by the exponent itself: one that 64-bit floats have no power of two for must not reach their exponent's bits.
     __device__ __forceinline__ double weight(float v) const {
-        if (v < lowest) return 0.0;
         const float magic32 = 12582912.f;                // 1.5 2^23: a sum's last bits are the nearest integer
-        const int n = __float_as_int(fmaf(v - largest, steps32, magic32)) - __float_as_int(magic32);
+        const float at = fmaf(fmaf(0.5f, v, -half), steps32, magic32);           // (by halves: a difference may pass the largest float)
+        if (at < magic32 + 32.f * SF_SMALLEST) return 0.0;
+        const int n = __float_as_int(at) - __float_as_int(magic32), k = n >> 5;
         const double x = fma((double)v - (double)largest, steps, 6755399441055744.0 - __hiloint2double(0x43380000 + (n >> 31), n));      // half a step, and what 32 bits round
         constexpr double A = SF_STEP, A2 = A * A / 2, A3 = A2 * A / 3, A4 = A3 * A / 4, A5 = A4 * A / 5;
         const double e = powers[n & 31] * fma(x, fma(x, fma(x, fma(x, fma(x, A5, A4), A3), A2), A), 1.0);
-        return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
+        if (k < -1000) return __hiloint2double(__double2hiint(e) + ((k + 128) << 20), __double2loint(e)) * 2.938735877055719e-39;     // 2^-128: rounded where it is subnormal
+        return __hiloint2double(__double2hiint(e) + (k << 20), __double2loint(e));
     }
     // Calls f(column, value) for the block's columns whose value is `floor` or more, a thread every SF_THREADS-th.
     template <typename F> __device__ __forceinline__ void each(float floor, F f) const {
