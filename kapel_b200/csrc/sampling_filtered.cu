@@ -16,14 +16,16 @@
 //      bin's weight lies between its count times the weights at its ends, so the histogram bounds where the cut is to a few bins, from above
 //      and, all weights' sum being known, from below. The bins in question, or all down to them, are gathered and sorted for the exact cut
 //      where they hold no more than LIST tokens, else counted again in 2,048 bins of their own; the same pass adds up what lies above them exactly (in
-//      fixed point, 44 bits behind the point: whole numbers, whose order changes nothing; a row's sum, 2^19 tokens, fits 64 bits). (Weights added up by
+//      fixed point, 52 bits behind the point: whole numbers, whose order changes nothing; a thread's sums and a warp's fit 64 bits, a row's, of up to
+//      2^19 tokens, has 72). (Weights added up by
 //      atomics instead took 1.1 ms a row of 256,000: shared memory has none of 64 bits. Without the bound from below a nucleus of 0.99 took
 //      three levels and 160 us where it takes one and 50.)
 //   4. The draw goes over the whole share of every block: totals of warps, of the 32 rows of the warp's that the target falls in,
 //      then along that row.
-// e^x is in 64 bits, and so are the draw's sums, as on the host: a seed gives the tokens it gave there, but for borders that lie within a
-// few units of the 13th digit. It is made of 2^(n / 32) = 2^k T[n mod 32], n an integer within a roundoff of the nearest to 32 x / ln 2 (found in 32 bits), and a
-// polynomial of degree 5 for what is left (the series' next term is below 3e-15): nine 64-bit operations, of which a multiprocessor does some 37 a
+// e^x is in 64 bits, and so are the draw's sums, as on the host: a seed gives the tokens it gives there, but for borders within the roundings of either side. Those of
+// the draw lie in the 13th digit. In the nucleus' sums a token is off by up to 2^-53 of the likeliest, where the host rounds every running total to as
+// much of the whole: some 1e-13 of 256,000 tokens as roundings go, 3e-11 where all weights lie just below half a unit. e^x is
+// made of 2^(n / 32) = 2^k T[n mod 32], n an integer within a roundoff of the nearest to 32 x / ln 2 (found in 32 bits), and a polynomial of degree 5 for what is left (the series' next term is below 3e-15): nine 64-bit operations, of which a multiprocessor does some 37 a
 // clock. Two entries of T share a bank, so a warp's loads take two turns at most.
 //
 // What bounds it, over 256,000 tokens: one row alone takes 15 us under top_k 50, of which the row's load is 3 and the rest some eight cluster
@@ -44,7 +46,7 @@ constexpr int SF_FULL = 48;                              // entries of a bucket 
 constexpr int SF_DEEP = 8, SF_BATCH = SF_DEEP * SF_THREADS;      // loads a thread asks for at once
 constexpr int SF_ROWS = 64;                              // rows of 32 columns a warp has at most: a share of 2^16, a vocabulary of 2^19 over eight blocks
 constexpr float SF_SPAN = 24.f;                          // the bins reach e^-24 below the largest; the last holds all that is below
-constexpr double SF_FIXED = 17592186044416.0;            // 2^44
+constexpr double SF_FIXED = 4503599627370496.0;          // 2^52
 constexpr double SF_STEP = 0.6931471805599453 / 32.0;    // ln 2 / 32
 constexpr int SF_SMALLEST = -1076;                       // a weight below 2^-1075 is none
 
@@ -61,6 +63,12 @@ struct SfParams {
     int cached;                                          // of them in shared memory, all or whole batches; the rest is read again from the row
 };
 
+// Sums of weights that decide a cut, in units of 2^-52: up to 2^19 of them. Those of a warp's share (2^11 columns) and of a list fit 64 bits.
+typedef unsigned __int128 SfTotal;
+__device__ __forceinline__ double sf_double(SfTotal x) {
+    return fma((double)(unsigned long long)(x >> 64), 18446744073709551616.0, (double)(unsigned long long)x);
+}
+
 struct SfTop { float v; int nan; unsigned low; };       // a block's largest logit, and the smallest key of its threads' largest
 struct SfCut { unsigned key; int index; };               // what is left: key above, or equal and the index no larger
 struct SfFound {                                         // what the first block tells the others about a histogram
@@ -74,7 +82,7 @@ struct SfShared {
     unsigned long long list[SF_LIST];                    // first block: key << 32 | ~index, the largest first once sorted
     SfTop tops[SF_MAX_CLUSTER];
     double sums[SF_MAX_CLUSTER];
-    unsigned long long fixed_sums[SF_MAX_CLUSTER][2];
+    unsigned long long fixed_sums[SF_MAX_CLUSTER][4];
     double warp_sum[SF_WARPS], warp_sum2[SF_WARPS];
     double row_sum[SF_ROWS];
     unsigned long long warp_fixed[SF_WARPS], warp_fixed2[SF_WARPS];
@@ -194,13 +202,13 @@ struct SfBins {
 };
 constexpr int SF_LEVELS = 8;                             // from here on by keys, whose number at least halves from level to level
 
-// e in fixed point: 2^52 added, the sum's last bits are the whole number.
+// e in fixed point, rounded to a unit: 2^52 added, the sum's bits are the whole number above those of 2^52 (those of 2^53 too, where e is 1).
 __device__ __forceinline__ unsigned long long sf_fixed(double e) {
-    return (unsigned long long)__double_as_longlong(fma(e, SF_FIXED, 4503599627370496.0)) & 0xfffffffffffffull;
+    return (unsigned long long)__double_as_longlong(fma(e, SF_FIXED, 4503599627370496.0)) - 0x4330000000000000ull;
 }
 // run >= top_p all, the product not rounded before it is compared: equal weights reach a round share of the whole exactly.
-__device__ __forceinline__ bool sf_reached(unsigned long long run, double top_p, unsigned long long all) {
-    return fma(top_p, (double)all, -(double)run) <= 0.0;
+__device__ __forceinline__ bool sf_reached(SfTotal run, double top_p, SfTotal all) {
+    return fma(top_p, sf_double(all), -sf_double(run)) <= 0.0;
 }
 
 // Inclusive running totals over the block's first `warps` warps (the others have nothing), in thread order.
@@ -337,7 +345,7 @@ __device__ __forceinline__ void sf_clear(SfShared& s) {
 // level's keys; `whole`: all is in the level's bins, so what lies down to a bin is bounded by what lies below it too: the bounds are as near as a
 // bin is wide, of the smaller of the two. Where nothing reaches it (fewer tokens, or rounding) the last bin that holds a token. Every block leaves with `found`.
 __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r, const SfBins& bins, unsigned want, double top_p, unsigned above,
-                        unsigned long long weight_above, unsigned long long all, bool whole) {
+                        SfTotal weight_above, SfTotal all, bool whole) {
     const int tid = threadIdx.x;
     if (cluster.block_rank() == 0 && tid == 0) { s.owner = SF_BINS; s.owner2 = SF_BINS; s.kept = -1; }
     cluster.sync();
@@ -369,10 +377,10 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
         unsigned run_c = above + sf_scan(count, s.warp_count, &total_c) - count;
         double run_l = 0.0, run_u = 0.0;
         if (by_weight) {
-            run_l = (double)weight_above + sf_scan(lower, s.warp_sum, &all_lower) - lower;
-            run_u = (double)weight_above + sf_scan(upper, s.warp_sum2, &all_upper) - upper;
+            run_l = sf_double(weight_above) + sf_scan(lower, s.warp_sum, &all_lower) - lower;
+            run_u = sf_double(weight_above) + sf_scan(upper, s.warp_sum2, &all_upper) - upper;
         }
-        const double target = top_p * (double)all, slack = 1e-12 * (double)all;         // (what 64-bit sums of up to 2,048 terms may be off by)
+        const double sum = sf_double(all), target = top_p * sum, slack = 1e-12 * sum;          // (what 64-bit sums of up to 2,048 terms may be off by)
         unsigned at[EACH];                               // tokens above each bin
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
@@ -383,7 +391,7 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
             if (c[j]) {
                 const int b = tid * EACH + j;
                 atomicMax(&s.kept, b);
-                const double no_more = whole ? fmin(run_u, (double)all - (all_lower - run_l)) : run_u, no_less = whole ? fmax(run_l, (double)all - (all_upper - run_u)) : run_l;
+                const double no_more = whole ? fmin(run_u, sum - (all_lower - run_l)) : run_u, no_less = whole ? fmax(run_l, sum - (all_upper - run_u)) : run_l;
                 if (by_weight ? no_more + slack >= target : run_c >= want) atomicMin(&s.owner, b);
                 if (by_weight ? no_less - slack >= target : run_c >= want) atomicMin(&s.owner2, b);
             }
@@ -404,27 +412,32 @@ __device__ void sf_find(cg::cluster_group& cluster, SfShared& s, const SfRow& r,
     cluster.sync();
 }
 
-// Two sums over the whole row of what each thread brings, in fixed point.
-__device__ void sf_sum(cg::cluster_group& cluster, SfShared& s, unsigned long long& a, unsigned long long& b) {
+// Two sums over the whole row of what each thread brings, up to 2^58.
+__device__ void sf_sum(cg::cluster_group& cluster, SfShared& s, unsigned long long a, unsigned long long b, SfTotal& all_a, SfTotal& all_b) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
     if (lane == 0) { s.warp_fixed[warp] = a; s.warp_fixed2[warp] = b; }
     __syncthreads();
-    if (warp == 0) {
-        a = s.warp_fixed[lane];
-        b = s.warp_fixed2[lane];
+    if (warp == 0) {                                     // the warps' sums of up to 63 bits, upper and lower halves by themselves
+        unsigned long long half[4] = {s.warp_fixed[lane] & 0xffffffffull, s.warp_fixed[lane] >> 32, s.warp_fixed2[lane] & 0xffffffffull, s.warp_fixed2[lane] >> 32};
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) half[k] += __shfl_xor_sync(0xffffffffu, half[k], o);
         if (lane < (int)cluster.num_blocks()) {
             unsigned long long* there = cluster.map_shared_rank(&s, lane)->fixed_sums[cluster.block_rank()];
-            there[0] = a;
-            there[1] = b;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) there[k] = half[k];
         }
     }
     cluster.sync();
-    a = b = 0;
-    for (unsigned k = 0; k < cluster.num_blocks(); ++k) { a += s.fixed_sums[k][0]; b += s.fixed_sums[k][1]; }
+    unsigned long long half[4] = {0ull, 0ull, 0ull, 0ull};
+    for (unsigned k = 0; k < cluster.num_blocks(); ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) half[j] += s.fixed_sums[k][j];
+    all_a = ((SfTotal)half[1] << 32) + half[0];
+    all_b = ((SfTotal)half[3] << 32) + half[2];
 }
 
 // Every block's list behind the first block's (`listed` of them there, of which SF_LIST are kept): each asks the first for room once. The lists are complete.
@@ -539,7 +552,7 @@ __device__ __forceinline__ unsigned sf_key_of(unsigned long long entry) { return
 
 // Of the sorted list's first n entries, how many are left where the weight before each must be below top_p of `all` (`above` lies before the
 // first).
-__device__ int sf_kept_by_weight(SfShared& s, const SfRow& r, int n, unsigned long long above, double top_p, unsigned long long all) {
+__device__ int sf_kept_by_weight(SfShared& s, const SfRow& r, int n, SfTotal above, double top_p, SfTotal all) {
     unsigned long long w[SF_EACH], mine = 0, listed;
 #pragma unroll
     for (int j = 0; j < SF_EACH; ++j) {
@@ -548,7 +561,7 @@ __device__ int sf_kept_by_weight(SfShared& s, const SfRow& r, int n, unsigned lo
         mine += w[j];
     }
     if (threadIdx.x == 0) s.kept = n;
-    unsigned long long run = above + sf_scan(mine, s.warp_fixed, &listed) - mine;
+    SfTotal run = above + (sf_scan(mine, s.warp_fixed, &listed) - mine);
 #pragma unroll
     for (int j = 0; j < SF_EACH; ++j) {
         const int i = threadIdx.x * SF_EACH + j;
@@ -574,7 +587,7 @@ template <typename F> __device__ int sf_first(SfShared& s, int n, F cuts) {
 }
 
 // The whole choice from the first block's list of the n largest.
-__device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, double top_p, double min_p, double u, unsigned long long all) {
+__device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, double top_p, double min_p, double u, SfTotal all) {
     sf_sort(s, n);
     int kept = n;
     if (top_k > 0 && top_k < n) {
@@ -583,11 +596,12 @@ __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, 
     }
     if (top_p < 1.0) {
         if (top_k > 0) {                                 // the whole is what top_k left
-            unsigned long long mine = 0;
+            unsigned long long mine = 0, listed;
             for (int i = threadIdx.x; i < kept; i += SF_THREADS) mine += sf_fixed(r.weight(sf_value(sf_key_of(s.list[i]))));
-            sf_scan(mine, s.warp_fixed, &all);
+            sf_scan(mine, s.warp_fixed, &listed);
+            all = listed;
         }
-        kept = sf_kept_by_weight(s, r, kept, 0ull, top_p, all);
+        kept = sf_kept_by_weight(s, r, kept, 0, top_p, all);
     }
     if (min_p > 0.0) kept = sf_first(s, kept, [&](unsigned long long x) { return r.weight(sf_value(sf_key_of(x))) < min_p; });
     // In the vocabulary's order: the index above the key, turned around so that the largest entry is the lowest index.
@@ -620,10 +634,10 @@ __device__ int sf_draw_from_list(SfShared& s, const SfRow& r, int n, int top_k, 
 // The exact cut inside the bins that a histogram found: every block leaves with it in `s.cut`. Every pass over the row adds up exactly what lies above the
 // keys that are still in question (of the last pass's, that is) and lists those, or where they are too many counts them in bins of their own.
 __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& r, SfBins bins, const SfCut cut, unsigned want, double top_p,
-                          unsigned long long all) {
+                          SfTotal all) {
     const bool by_weight = want == 0u;
     unsigned lo = max(cut.key, sf_key(SF_LOWEST)), hi = sf_key(r.largest);       // the keys in question; what lies above them:
-    unsigned long long weight_above = 0;
+    SfTotal weight_above = 0;
     unsigned above = 0;
     for (int level = 0; level < SF_LEVELS + 40; ++level) {       // (the last SF_LEVELS + 32nd has one key in question)
         const SfFound f = s.found;
@@ -642,17 +656,18 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
                 const unsigned long long w = sf_fixed(r.weight(v));
                 if (v > most) { a += w; ++na; } else { b += w; ++nb; }
             });
-            sf_sum(cluster, s, a, b);
+            SfTotal wa, wb, ca, cb;
+            sf_sum(cluster, s, a, b, wa, wb);
             cluster.sync();                              // the sums have been read
-            sf_sum(cluster, s, na, nb);
-            weight_above += a;
-            above += (unsigned)na;
-            if (sf_reached(weight_above + b, top_p, all)) {
+            sf_sum(cluster, s, na, nb, ca, cb);
+            weight_above += wa;
+            above += (unsigned)ca;
+            if (sf_reached(weight_above + wb, top_p, all)) {
                 low = middle + 1;
                 least = sf_value(low);
             } else {
-                weight_above += b;
-                above += (unsigned)nb;
+                weight_above += wb;
+                above += (unsigned)cb;
                 high = middle;
                 most = half;
             }
@@ -674,9 +689,10 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
             if (list) sf_list(s, sf_key(v), r.first + i);
             else atomicAdd(&s.counts[bins.of(v)], 1u);
         });
-        sf_sum(cluster, s, weight, number);
-        weight_above += weight;
-        above += (unsigned)number;
+        SfTotal passed, count;
+        sf_sum(cluster, s, weight, number, passed, count);
+        weight_above += passed;
+        above += (unsigned)count;
         lo = low;
         hi = high;
         if (list) {
@@ -712,10 +728,10 @@ __device__ void sf_refine(cg::cluster_group& cluster, SfShared& s, const SfRow& 
                 const int tied = (int)within;            // (after a halving fewer may be there: the count below stops at the last)
                 int keep = tied;
                 if (e > 0) {
-                    const double some = ceil((top_p * (double)all - (double)weight_above) / (double)e);
-                    keep = (int)fmin(fmax(some, 1.0), (double)tied);
-                    while (keep > 1 && sf_reached(weight_above + (unsigned long long)(keep - 1) * e, top_p, all)) --keep;
-                    while (keep < tied && !sf_reached(weight_above + (unsigned long long)keep * e, top_p, all)) ++keep;
+                    for (int from = 1; from < keep;) {           // by halves
+                        const int some = from + (keep - from) / 2;
+                        if (sf_reached(weight_above + (SfTotal)some * e, top_p, all)) keep = some; else from = some + 1;
+                    }
                 }
                 const int at = sf_locate(cluster, s, r, least, [&](int, float v) { return sf_key(v) == low ? 1.0 : 0.0; },
                                          [&](double) { return (double)keep - 0.5; });
@@ -841,7 +857,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
         if (top_k <= SF_LIST / 2) {
             sf_clear(s);
             if (own > -INFINITY) atomicAdd(&s.counts[bins.of(own)], 1u);
-            sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull, false);
+            sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0, 0, false);
             if (s.found.upto >= (unsigned)top_k) {
                 const int down = s.found.to;
                 sf_gather(cluster, s, r, bins, cut, down);
@@ -849,7 +865,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
                 if (listed <= SF_LIST) {
                     cluster.sync();                      // the first block's count has been read
                     if (rank == 0) {
-                        const int token = sf_draw_from_list(s, r, listed, top_k, by_p ? top_p : 1.0, min_p, u, 0ull);
+                        const int token = sf_draw_from_list(s, r, listed, top_k, by_p ? top_p : 1.0, min_p, u, 0);
                         if (tid == 0) p.tokens[row] = token;
                     }
                     return;
@@ -858,31 +874,32 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
         }
         sf_clear(s);
         r.each(SF_LOWEST, [&](int, float v) { atomicAdd(&s.counts[bins.of(v)], 1u); });
-        sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0ull, 0ull, false);
+        sf_find(cluster, s, r, bins, (unsigned)top_k, 0.0, 0u, 0, 0, false);
         if (s.found.upto <= (unsigned)SF_LIST) {
             const int n = (int)(s.found.upto);
             sf_gather(cluster, s, r, bins, cut, s.found.to);
             if (rank == 0) {
-                const int token = sf_draw_from_list(s, r, n, top_k, by_p ? top_p : 1.0, min_p, u, 0ull);
+                const int token = sf_draw_from_list(s, r, n, top_k, by_p ? top_p : 1.0, min_p, u, 0);
                 if (tid == 0) p.tokens[row] = token;
             }
             return;
         }
-        sf_refine(cluster, s, r, bins, cut, (unsigned)top_k, 0.0, 0ull);
+        sf_refine(cluster, s, r, bins, cut, (unsigned)top_k, 0.0, 0);
         cut = s.cut;
         bins.step = weights;
     }
     if (by_p) {
         sf_clear(s);
-        unsigned long long all = 0, unused = 0;
+        unsigned long long mine = 0;
+        SfTotal all, unused;
         const bool cuts = top_k > 0;
         r.each(sf_floor(cut), [&](int i, float v) {
             if (cuts && !sf_left(cut, sf_key(v), r.first + i)) return;
             atomicAdd(&s.counts[bins.of(v)], 1u);
-            all += sf_fixed(r.weight(v));
+            mine += sf_fixed(r.weight(v));
         });
-        sf_sum(cluster, s, all, unused);
-        sf_find(cluster, s, r, bins, 0u, top_p, 0u, 0ull, all, true);
+        sf_sum(cluster, s, mine, 0ull, all, unused);
+        sf_find(cluster, s, r, bins, 0u, top_p, 0u, 0, all, true);
         if (s.found.upto <= (unsigned)SF_LIST) {
             const int n = (int)(s.found.upto);
             sf_gather(cluster, s, r, bins, cut, s.found.to);
