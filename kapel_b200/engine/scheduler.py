@@ -172,8 +172,13 @@ class Scheduler:
         entry = self.entries.pop(rid, None)
         if entry is None:
             return
-        others = self.answers.pop(rid, None)
-        self._wait_together(others or [])                   # the next answer takes the prompt over
+        others = self.answers.pop(rid, None)                # the next answer takes the prompt over,
+        if others and not entry.running:                    # in its place among those that wait
+            self.waiting[self.waiting.index(rid)] = others[0]
+            if others[1:]:
+                self.answers[others[0]] = others[1:]
+            return
+        self._wait_together(others or [])
         for first, rest in list(self.answers.items()):
             if rid in rest:
                 rest.remove(rid)
