@@ -521,7 +521,7 @@ class Scheduler:
     def _choose_on_device(self, logits, producing: List[int], rows: List[int]):
         """The chosen tokens as an int32 device tensor, a token a row of `logits` (rows outside `rows`
         belong to nobody and get the largest logit), enqueued and not waited for; None where the
-        choice needs the host (penalties) or the logits are not on a device."""
+        choice needs the host (penalties, filters under an extreme temperature) or the logits are not on a device."""
         if not producing or not getattr(logits, "is_cuda", False):
             return None
         entries = [self.entries[rid] for rid in producing]
@@ -557,7 +557,7 @@ class Scheduler:
         top_k = table[4].view(np.int32)
         for i, e in zip(rows, entries):
             s = e.request.sampling
-            temperature = max(0.0, s.temperature)           # a row of its own that is greedy stays greedy
+            temperature = 0.0 if s.is_greedy() else s.temperature
             u = e.sampler.uniform() if temperature > 0 else 0.0
             table[:4, i] = temperature, s.top_p, s.min_p, u
             top_k[i] = min(max(0, int(s.top_k or 0)), 2 ** 31 - 1)

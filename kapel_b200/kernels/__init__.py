@@ -2132,7 +2132,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
                     uniform: torch.Tensor) -> torch.Tensor:
     """One token a row of float32 logits [rows, vocab], by the host sampler's rules (`sampling.Sampler`) and in 64 bits as there: the
     first largest where the row's temperature is 0 or less; else logits / temperature, top_k (0 or less: none; what ties with the
-    k-th stays), top_p (1 or more: none; the lower index first among equals), min_p (0 or less: none), and the first index
+    k-th stays), top_p (1 or more: none; the larger logit first, the lower index among equals), min_p (0 or less: none), and the first index
     whose running total exceeds `uniform`, in [0, 1), times what is left. `temperature`, `top_p`, `min_p` and `uniform` are float64 [rows], `top_k`
     int32 [rows], all on the logits' device, which has to be the current one. Nothing left (a top_p of 0 or less, a min_p above 1) gives
     token 0; logits with a NaN or an infinity among them their first largest."""

@@ -28,6 +28,7 @@ from ..hostlib import host_library
 
 _M = (1 << 64) - 1
 _CPUS = os.cpu_count() or 1
+HOTTEST_ON_DEVICE = 1000.0
 
 
 @dataclass
@@ -77,10 +78,11 @@ class Sampling:
         """Only the logits, a temperature and a uniform number decide."""
         return not self.has_penalties() and (self.is_greedy() or not self.has_filters())
 
-
     def filtered_on_device(self) -> bool:
-        """The logits, the filters' settings and a uniform number decide: `kernels.sample_filtered` follows the host's rules."""
-        return not self.has_penalties()
+        """The logits, the filters' settings and a uniform number decide: `kernels.sample_filtered` follows the host's rules up to this temperature.
+        The hotter the row, the more logits differ and have the same probability in 64 bits (or, at an infinite temperature, the same quotient): those the host
+        takes by their index, and keeps at top_k's border, the kernel by the logits themselves."""
+        return not self.has_penalties() and not self.temperature > HOTTEST_ON_DEVICE
 
 
 class Rng:
