@@ -558,7 +558,8 @@ class Scheduler:
         for i, e in zip(rows, entries):
             s = e.request.sampling
             temperature = 0.0 if s.is_greedy() else s.temperature
-            u = e.sampler.uniform() if temperature > 0 else 0.0
+            certain = not temperature > 0 or s.top_p <= 0 or s.min_p > 1        # whatever the logits: no number is taken, as on the host
+            u = 0.0 if certain else e.sampler.uniform()
             table[:4, i] = temperature, s.top_p, s.min_p, u
             top_k[i] = min(max(0, int(s.top_k or 0)), 2 ** 31 - 1)
         host = torch.from_numpy(table).pin_memory()

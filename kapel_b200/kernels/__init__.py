@@ -2135,7 +2135,8 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     k-th stays), top_p (1 or more: none; the larger logit first, the lower index among equals), min_p (0 or less: none), and the first index
     whose running total exceeds `uniform`, in [0, 1), times what is left. `temperature`, `top_p`, `min_p` and `uniform` are float64 [rows], `top_k`
     int32 [rows], all on the logits' device, which has to be the current one. Nothing left (a top_p of 0 or less, a min_p above 1) gives
-    token 0; logits with a NaN or an infinity among them their first largest."""
+    token 0; logits with a NaN or an infinity among them their first largest. (The host's generator takes no number for a choice
+    that is certain so: whoever draws `uniform` from it ahead of the logits has taken one.)"""
     if not (_as_wanted(torch.float64, temperature, top_p, min_p, uniform) and _as_wanted(torch.float32, logits) and _as_wanted(torch.int32, top_k) and logits.dim() == 2 and
             temperature.shape == top_k.shape == top_p.shape == min_p.shape == uniform.shape == logits.shape[:1]):
         _need(logits, "sample_filtered logits", torch.float32)

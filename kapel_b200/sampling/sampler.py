@@ -9,7 +9,10 @@ uniform number in [0, 1) (sampling.rs:241-260). Arithmetic on the host is 64-bit
 A request whose choice needs only the logits (greedy without penalties, or a plain
 temperature) can be served where the logits are, by `kernels.sample`, one with filters by
 `kernels.sample_filtered`; the uniform number still comes from this generator, so the same seed
-gives the same tokens. Penalties, which look at the tokens so far, stay here.
+gives the same tokens. (With one exception: a choice that the logits make certain, where one is infinite
+or no number or none is above -inf, takes no number here but has taken one there, before the logits were
+known; later tokens of such a request depend on where that step was served.) Penalties, which look at the
+tokens so far, stay here.
 
 The arithmetic runs in the host library (`csrc/host/sampler_core.cpp`): a choice over 256,000
 logits with top_k takes about a millisecond there, where sorting them with numpy took ten to
