@@ -383,10 +383,11 @@ extern "C" long long kb_shared_attention_scratch_floats(int rows, int hq, int hk
     return (x.tile_places + x.row_places) * SH_PIECE(dv) + SH_CUT_INTS;
 }
 
-// 1 where the kernels take these sizes.
+// 1 where the kernels take these sizes, 2 where they take them on the tensor cores.
 extern "C" int kb_shared_attention_takes(int dtype, int hq, int hkv, int d, int dv, int page_size) {
-    return (dtype == KB_DT_F32 || dtype == KB_DT_BF16) && hkv > 0 && hq > 0 && hq % hkv == 0 && hq / hkv <= SR_PAIRS && d > 0 && d <= SR_DIM && dv > 0 &&
-           dv <= SR_DIM && page_size > 0;
+    if ((dtype != KB_DT_F32 && dtype != KB_DT_BF16) || hkv <= 0 || hq <= 0 || hq % hkv || hq / hkv > SR_PAIRS || d <= 0 || d > SR_DIM || dv <= 0 || dv > SR_DIM || page_size <= 0)
+        return 0;
+    return shared_on_tensor_cores(dtype, hq, hkv, d, dv, page_size) ? 2 : 1;
 }
 
 extern "C" int kb_shared_attention(void* out, const void* q, const void* k_table, const void* v_table, int dtype, const int* block_table,

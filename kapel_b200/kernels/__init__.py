@@ -1062,6 +1062,17 @@ def shared_prefix_takes(dtype, hq: int, hkv: int, d: int, dv: int, page_size: in
     return dtype in _CODES and bool(library().kb_shared_attention_takes(_CODES[dtype], int(hq), int(hkv), int(d), int(dv), int(page_size)))
 
 
+def shared_prefix_pays(dtype, hq: int, hkv: int, d: int, dv: int, page_size: int) -> bool:
+    """Whether `shared_prefix_attention` may be faster than each row by itself at these sizes. In bfloat16 it is on the tensor cores, and where the kernels for
+    single rows are not on them either; where only those are it never was. As measured (us, shared and row by row): 12 heads over 4 of 96,
+    8 requests sharing 12,288 positions 84 and 32, 128 sharing 1,024 157 and 66; 16 over 2 of 112, 64 sharing 2,048 120 and 43; 40 over 8 of 48, the same 268 and
+    56. Keys of 128 and values of 64, 8 over 2, 64 sharing 2,048 72 and 85; 32 over 1 of 64, 64 sharing 2,048 164 and 175."""
+    if dtype not in _CODES:
+        return False
+    takes = library().kb_shared_attention_takes(_CODES[dtype], int(hq), int(hkv), int(d), int(dv), int(page_size))
+    return takes == 2 or (takes == 1 and not (d == dv and attention_mma_takes(dtype, d, hq // hkv)))
+
+
 def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_id, share_len, page_size: int, window: Optional[int],
                             scale: float, softcap: Optional[float], sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of a decode step's single tokens [rows, hq, d] (row r is request r, its pages in row r of `block_table`, its own

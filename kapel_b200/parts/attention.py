@@ -216,11 +216,17 @@ class Attention(Part):
         return CacheNeeds(paged=PagedKV(s.num_kv_heads, s.head_dim, s.window, s.keep_first if s.window else 0,
                                         self.v_dim if self.v_dim != s.head_dim else None))
 
-    def shared_pages(self, q, batch, group, k_table, v_table):
-        """Attention of a step of single tokens some of which share pages, reading those once; None where nothing is shared or that kernel does
-        not take the layer."""
+    def share_of(self, batch):
+        """(ids, positions) of the rows of a step of single tokens that share pages; None where nothing is shared or this layer gains nothing by reading it once."""
         s, share = self.spec, getattr(batch, "share", None)
-        if share is None or (s.window and s.keep_first) or not K.shared_prefix_takes(q.dtype, s.num_heads, s.num_kv_heads, s.head_dim, self.v_dim, self.ctx.page_size):
+        if share is None or (s.window and s.keep_first) or not K.shared_prefix_pays(self.ctx.dtype, s.num_heads, s.num_kv_heads, s.head_dim, self.v_dim, self.ctx.page_size):
+            return None
+        return share
+
+    def shared_pages(self, q, batch, group, k_table, v_table):
+        """Attention of such a step, reading shared pages once, or None."""
+        s, share = self.spec, self.share_of(batch)
+        if share is None:
             return None
         return K.shared_prefix_attention(q.view(-1, s.num_heads, s.head_dim), k_table, v_table, group.block_table, batch.row_count, share[0], share[1], self.ctx.page_size, s.window,
                                          s.scale, s.softcap, sinks=getattr(self, "sinks", None))
@@ -388,7 +394,7 @@ class Attention(Part):
         k_table, v_table = cache.tables()
         group = batch.groups[cache.group]
         heads_per_kv = s.num_heads // s.num_kv_heads
-        if getattr(batch, "share", None) is None and K.attention_decode_fused_takes(qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim,
+        if self.share_of(batch) is None and K.attention_decode_fused_takes(qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim,
                                           self.ctx.page_size, self.ctx.dtype):
             decode, tiles, split, slots, relative = batch.attention_tiles(
                 heads_per_kv, s.num_kv_heads, s.window, s.head_dim,
