@@ -110,6 +110,7 @@ class Plan:
     committed: bool = False
     native: object = None        # the manager's own: the entries as the host library takes them
     share: object = None         # (ids, positions) by row where single tokens share pages (`CacheManager.shared_runs`), else None
+    windows: Tuple[Optional[int], ...] = ()      # of the groups
     line_bytes: int = 0          # bytes of a position's keys and values in the group that holds most of them, and of one component
     item_bytes: int = 2
     added: List[Hashable] = field(default_factory=list)   # the step function's: sequences it added for this step
@@ -206,6 +207,7 @@ class CacheManager:
         self._family: Dict[Hashable, Tuple[int, int]] = {}       # sequence -> (family, positions its members share, whole pages)
         self._families = 0
         self.line_bytes, self.item_bytes = 0, 2
+        self._windows = tuple(g.window for g in self.groups)
         self._names = 0                                          # counts the sequences that have come or gone
         if allocate is not None:
             self.allocate_tables(allocate, dtype)
@@ -430,7 +432,7 @@ class CacheManager:
         plan.native = (self._names, sc, n)
         if n_rows == n:
             plan.share = self.shared_runs([s for s, _ in entries])
-            plan.line_bytes, plan.item_bytes = self.line_bytes, self.item_bytes
+            plan.windows, plan.line_bytes, plan.item_bytes = self._windows, self.line_bytes, self.item_bytes
         return plan
 
     def _entries_arrays(self, entries):

@@ -57,11 +57,15 @@ def decode_split(pairs: int, longest: int, sms: int, window: Optional[int] = Non
     return split, max(1, -(-(span if relative else longest) // split))
 
 
-# When a step of single tokens goes by `kernels.shared_prefix_attention`. In bfloat16: from so many bytes of a layer's keys and values on that need not be
-# read again. Its three kernels take 19 us where the decode kernel takes 7 at the least (its two, where little is held at all, 9); as measured (us, shared and row by row, each request with
-# 100 positions of its own): 8 heads over 4 of 256, 8 requests sharing 4,096 positions (117 MB) 29 and 29, 16 sharing 1,024 (63 MB) 22 and 18,
-# 32 sharing 1,024 (130 MB) 22 and 29, 64 sharing 4,096 (1.1 GB) 33 and 189; 16 over 8 of 256, 16 sharing 1,024 (126 MB) 22 and 28; 32 over 16 of 128,
-# 8 sharing 1,024 (59 MB) 26 and 19, 64 sharing 256 (132 MB) 32 and 38.
+# When the layers of a group go by `kernels.shared_prefix_attention` in a step of single tokens. In bfloat16: from so many bytes of a layer's keys and values on
+# that need not be read again, and where they are at least twice what is read once: a tile of two requests reads no faster than the decode
+# kernel reads both. As measured (us, shared and row by row by `paged_attention_mma`, a layer's pages not in the second-level cache, each request with 100 positions
+# of its own; bytes saved): 8 heads over 4 of 256, 8 requests sharing 2,048 positions (59 MB) 18 and 18, 4,096 (117) 31 and 29, 8,192 (235) 33 and
+# 51, 16 sharing 1,024 (63) 19 and 18, 2,048 (126) 25 and 29, 64 sharing 4,096 (1,057) 34 and 190; 16 over 8 of 256, 4 sharing 4,096 (101) 31 and 29, 8,192
+# (201) 47 and 51, 16 sharing 1,024 (126) 22 and 28; 32 over 16 of 128, 16 sharing 1,024 (126) 25 and 22, 3 sharing 8,192 (134) 41 and 48, 64 sharing 512 (264)
+# 34 and 55. Two requests: 16,384 positions (134) 59 and 37, 50 and 46 of 16 over 8 of 256, 32,768 (268) 94 and 67, 72 and 86. Where a window leaves 4,096 of
+# 16,384: 8 requests, 16 over 8 of 256 (229) 33 and 52, 4 (98) 32 and 29, 2 (33) 30 and 18. (The fused decode kernel, which goes row by row in most designs,
+# also has the rotation and the cache's new line in it.)
 SHARED_BYTES = 110_000_000
 # In 32-bit, where the kernel takes longer than the row-wise one over what requests have of their own: from so many positions a request (on average),
 # for each request of the step, on. 8 over 4 of 256: 2 requests sharing 64 positions 20 and 30, 16 sharing 256 36 and 46, 64 sharing 256 64 and 55; 32 over 16
@@ -69,17 +73,32 @@ SHARED_BYTES = 110_000_000
 SHARED_POSITIONS_32 = 16
 
 
-def sharing_of(plan):
-    """`plan.share` where reading shared pages once pays, else None."""
+def sharing_groups(plan):
+    """For each group of layers whether reading shared pages once pays there, or None where it pays nowhere."""
     share = getattr(plan, "share", None)
     if share is None or plan.rows > SHARED_PREFIX_ROWS:
         return None
     ids, lengths = share
     begins = np.ones(len(ids), bool)
-    begins[1:] = (ids[1:] != ids[:-1]) | (lengths[1:] == 0)
-    saved = int(lengths[~begins].sum())
-    pays = saved >= SHARED_POSITIONS_32 * plan.rows ** 2 if plan.item_bytes == 4 else saved * plan.line_bytes >= SHARED_BYTES
-    return share if saved and pays else None
+    begins[1:] = (ids[1:] != ids[:-1]) | (lengths[1:] != lengths[:-1]) | (lengths[1:] == 0)
+    starts = np.flatnonzero(begins)
+    seen = {}
+    for window in set(plan.windows):
+        first = np.maximum(plan.row_count - window, 0) if window else np.zeros_like(lengths)
+        sees = np.maximum(lengths - first, 0).astype(np.int64)
+        once = int(np.maximum.reduceat(sees, starts).sum())            # positions that some row of a run sees of what it shares
+        saved = int(sees.sum()) - once
+        if plan.item_bytes == 4:
+            pays = saved >= SHARED_POSITIONS_32 * plan.rows ** 2
+        else:
+            pays = saved * plan.line_bytes >= SHARED_BYTES and saved >= 2 * once
+        seen[window] = saved > 0 and pays
+    return tuple(seen[w] for w in plan.windows) if any(seen.values()) else None
+
+
+def sharing_of(plan):
+    """`plan.share` where reading shared pages once pays in some group of layers, else None."""
+    return plan.share if sharing_groups(plan) is not None else None
 
 
 # Latent attention: a request's rows from which its keys and values are made for every head: that costs about 6 ns a position (16 heads of
@@ -259,7 +278,8 @@ class StepBatch:
         for i, shape in enumerate(table_shapes):
             self.groups.append(GroupBatch(views[6 + 2 * i], views[7 + 2 * i].view(shape)))
         at = 6 + 2 * len(table_shapes)
-        self.share = (views[at], views[at + 1]) if len(views) > at else None        # (ids, positions) of rows that share pages
+        self.share = (views[at], views[at + 1]) if len(views) > at else None        # (ids, positions) of rows that share pages, in the groups of layers
+        self.share_groups = sharing_groups(self.plan)                                # ... for which it pays
 
     def attention_tiles(self, heads_per_kv: int, kv_heads: int, window: Optional[int] = None, head_dim: int = 256,
                         prompt_kernel: str = "mma", keep_first: int = 0):

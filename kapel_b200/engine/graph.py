@@ -19,7 +19,7 @@ from typing import Dict, List, Optional, Tuple
 import numpy as np
 import torch
 
-from .batch import GroupBatch, StepBatch, decode_split, pooled_slices, sharing_of, sm_count
+from .batch import GroupBatch, StepBatch, decode_split, pooled_slices, sharing_groups, sm_count
 
 ROW_BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
 WIDTH_STEP = 64          # block-table widths are rounded up to a multiple of this many pages
@@ -28,15 +28,16 @@ WIDTH_STEP = 64          # block-table widths are rounded up to a multiple of th
 class StaticBatch:
     """A batch of fixed size whose inputs live in one device buffer that replays rewrite."""
 
-    share = None             # (ids, positions) of rows that share pages, on the device, in a recording that reads those once
+    share = None             # (ids, positions) of rows that share pages, on the device, in a recording that reads those once,
+    share_groups = None      # ... in these groups of layers
 
-    def __init__(self, rows: int, width: int, n_groups: int, device, chunk: int, page_size: int, shared: bool = False):
-        """`shared`: the pass's rows say which of them share pages (`share`), and attention reads what they share once."""
+    def __init__(self, rows: int, width: int, n_groups: int, device, chunk: int, page_size: int, shared: Optional[tuple] = None):
+        """`shared`: the pass's rows say which of them share pages (`share`), and attention reads what they share once in the groups of layers for which it is true."""
         self.rows = self.entries = rows
         self.width = width
         self.chunk = chunk
         self.memo: Dict[object, object] = {}
-        sizes = [rows] * 6 + [rows, rows * width] * n_groups + [rows, rows] * int(shared)
+        sizes = [rows] * 6 + [rows, rows * width] * n_groups + [rows, rows] * int(shared is not None)
         self.total = sum(sizes)
         # Two pinned staging buffers taken in turn: the next pass can be written while the copy of
         # the last one may still be in flight. Each has an event recorded behind its copy; the host
@@ -54,7 +55,8 @@ class StaticBatch:
             at += n
         self.ids, self.positions, self.row_entry, self.row_count, self.want_rows, self.slots = views[:6]
         self.groups = [GroupBatch(views[6 + 2 * g], views[7 + 2 * g].view(rows, width)) for g in range(n_groups)]
-        self.share = (views[-2], views[-1]) if shared else None
+        if shared is not None:
+            self.share, self.share_groups = (views[-2], views[-1]), shared
         self._sizes = sizes
         self.fixed_slots = max(1, -(-(width * page_size) // chunk))
         # the tensor-core attention kernel's tiles: every row a tile of one token
@@ -194,10 +196,11 @@ class DecodeGraphs:
         return None
 
     def key_of(self, plan) -> Optional[tuple]:
-        """The bucket of a decode-only plan: (rows, block-table width), and a third word where it reads shared pages once."""
+        """The bucket of a decode-only plan: (rows, block-table width), and where it reads shared pages once in which groups of layers."""
         width = max(g.block_table.shape[1] for g in plan.groups) if plan.groups else 1
         key = self.bucket(plan.rows, width)
-        return (*key, "shared") if key is not None and sharing_of(plan) is not None else key
+        groups = sharing_groups(plan) if key is not None else None
+        return key if groups is None else (*key, groups)
 
     def prepare(self, plan):
         """Stages a decode-only plan whose token ids are not known yet: (plan, bucket, staging
@@ -236,7 +239,7 @@ class DecodeGraphs:
 
         graph = None
         try:
-            static = StaticBatch(key[0], key[1], len(plan.groups), eng.device, eng.chunk, eng.cache.page_size, shared=len(key) > 2)
+            static = StaticBatch(key[0], key[1], len(plan.groups), eng.device, eng.chunk, eng.cache.page_size, shared=key[2] if len(key) > 2 else None)
             static.fill(plan, ids)
             # Once eagerly on a side stream (kernels set their attributes, the allocator warms up), then the capture.
             side = torch.cuda.Stream()
@@ -369,7 +372,7 @@ class PromptGraphs:
         before = tuple(int(plan.row_count[int(s)]) - 1 for s in plan.q_start)
         # which rows are wanted is data (the gather's indices) when a row count was rounded; else part of the shape
         wanted = (len(want_rows),) if rounded else tuple(int(w) for w in want_rows)
-        return q_len, before, rounded, wanted, tuple(tuple(g.block_table.shape) for g in plan.groups), sharing_of(plan) is not None
+        return q_len, before, rounded, wanted, tuple(tuple(g.block_table.shape) for g in plan.groups), sharing_groups(plan)
 
     def run(self, plan, ids, want_rows) -> Optional[torch.Tensor]:
         """Logits of the pass through a recording of its shape, or None: the caller runs it eagerly.

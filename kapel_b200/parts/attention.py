@@ -216,18 +216,19 @@ class Attention(Part):
         return CacheNeeds(paged=PagedKV(s.num_kv_heads, s.head_dim, s.window, s.keep_first if s.window else 0,
                                         self.v_dim if self.v_dim != s.head_dim else None))
 
-    def share_of(self, batch):
+    def share_of(self, batch, cache):
         """(ids, positions) of the rows of a step of single tokens that share pages; None where nothing is shared or this layer gains nothing by reading it once."""
         s, share = self.spec, getattr(batch, "share", None)
-        if share is None or (s.window and s.keep_first) or not K.shared_prefix_pays(self.ctx.dtype, s.num_heads, s.num_kv_heads, s.head_dim, self.v_dim, self.ctx.page_size):
+        if share is None or not batch.share_groups[cache.group] or (s.window and s.keep_first) or not K.shared_prefix_pays(self.ctx.dtype, s.num_heads, s.num_kv_heads, s.head_dim, self.v_dim, self.ctx.page_size):
             return None
         return share
 
-    def shared_pages(self, q, batch, group, k_table, v_table):
+    def shared_pages(self, q, batch, cache):
         """Attention of such a step, reading shared pages once, or None."""
-        s, share = self.spec, self.share_of(batch)
+        s, share = self.spec, self.share_of(batch, cache)
         if share is None:
             return None
+        (k_table, v_table), group = cache.tables(), batch.groups[cache.group]
         return K.shared_prefix_attention(q.view(-1, s.num_heads, s.head_dim), k_table, v_table, group.block_table, batch.row_count, share[0], share[1], self.ctx.page_size, s.window,
                                          s.scale, s.softcap, sinks=getattr(self, "sinks", None))
 
@@ -316,7 +317,7 @@ class Attention(Part):
                                    s.num_heads, s.num_kv_heads, s.head_dim, dv, cache.owns, self.ctx.dtype)
         heads_per_kv = s.num_heads // s.num_kv_heads
         keep = s.keep_first if s.window else 0
-        y = self.shared_pages(q, batch, group, k_table, v_table)
+        y = self.shared_pages(q, batch, cache)
         if y is None and dv == s.head_dim and K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
             # with kept first keys only prompt portions go to the tensor-core kernel; a pass of single tokens stays with
             # the row-wise kernel below
@@ -360,7 +361,7 @@ class Attention(Part):
                                     self.position.tables(batch) if rotary else None, rotary, group.lines, k_table, v_table,
                                     s.num_heads, s.num_kv_heads, s.head_dim, dv, cache.owns, self.ctx.dtype)
         heads_per_kv = s.num_heads // s.num_kv_heads
-        y = self.shared_pages(q, batch, group, k_table, v_table)
+        y = self.shared_pages(q, batch, cache)
         if y is not None:
             pass
         elif dv == s.head_dim and s.head_dim % 16 == 0 and K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
@@ -394,7 +395,7 @@ class Attention(Part):
         k_table, v_table = cache.tables()
         group = batch.groups[cache.group]
         heads_per_kv = s.num_heads // s.num_kv_heads
-        if self.share_of(batch) is None and K.attention_decode_fused_takes(qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim,
+        if self.share_of(batch, cache) is None and K.attention_decode_fused_takes(qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim,
                                           self.ctx.page_size, self.ctx.dtype):
             decode, tiles, split, slots, relative = batch.attention_tiles(
                 heads_per_kv, s.num_kv_heads, s.window, s.head_dim,
@@ -410,7 +411,7 @@ class Attention(Part):
             s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim, write_kv=cache.owns,
             out_dtype=self.ctx.dtype,
         )
-        y = self.shared_pages(q, batch, group, k_table, v_table)
+        y = self.shared_pages(q, batch, cache)
         if y is not None:
             pass
         elif K.attention_mma_takes(q.dtype, s.head_dim, heads_per_kv):
