@@ -171,19 +171,30 @@ __device__ inline void shared_cut_rows(const SharedParams& p, int* upto, int* lo
     __syncthreads();
 }
 
-// The units of all tiles of one kv head as a rule that both kernels can follow has them: a tile's opening row stands for the tile. By one warp.
-__device__ __forceinline__ int shared_tile_units(const SharedParams& p, const int* length, const int* id, int rows_a_tile, int keys) {
+// The units of all tiles of one kv head, the number that shared_cut_tiles comes to, for the kernel over rows, which needs no more of that cut: both kernels
+// divide the multiprocessors by it. `length` and `id` by row; klo and khi [SH_ROWS] are scratch. By one warp.
+__device__ __forceinline__ int shared_tile_units(const SharedParams& p, const int* length, const int* id, int* klo, int* khi, int rows_a_tile, int keys) {
     const int lane = threadIdx.x & 31;
-    int run = 0, units = 0;
+    int run = 0, tiles = 0;
 #pragma unroll 1
     for (int base = 0; base < p.rows; base += 32) {
         const int r = base + lane, n = r < p.rows ? length[r] : 0;
         const bool starts = r < p.rows && (r == 0 || n == 0 || length[r - 1] != n || id[r - 1] != id[r]);
-        const unsigned who = __ballot_sync(0xffffffffu, starts), mine = who & (0xffffffffu >> (31 - lane));
+        const unsigned upto_here = 0xffffffffu >> (31 - lane), who = __ballot_sync(0xffffffffu, starts), mine = who & upto_here;
         const int begins = mine ? base + 31 - __clz(mine) : run;
-        if (n > 0 && (r - begins) % rows_a_tile == 0) units += max(0, n - shared_first(p, p.row_count[r]) + keys - 1) / keys;
+        const bool opens = n > 0 && (r - begins) % rows_a_tile == 0;
+        const unsigned opened = __ballot_sync(0xffffffffu, opens);
+        const int tile = tiles + __popc(opened & upto_here) - 1;
+        if (opens) { klo[tile] = 0x7fffffff; khi[tile] = n; }
+        __syncwarp();
+        if (n > 0) atomicMin(klo + tile, shared_first(p, p.row_count[r]));
+        tiles += __popc(opened);
         if (who) run = base + 31 - __clz(who);
     }
+    __syncwarp();
+    int units = 0;
+    for (int i = lane; i < tiles; i += 32)
+        if (klo[i] < khi[i]) units += (khi[i] - klo[i] / keys * keys + keys - 1) / keys;
     return __reduce_add_sync(0xffffffffu, units);
 }
 

@@ -23,7 +23,7 @@ template <int D> struct OwnCfg {
     static constexpr int BOXES = D / 64;
     static constexpr int STAGE = 2 * BOXES * 2048;                       // bytes: keys, then values
     static constexpr int PIPES = WARPS * STAGES * STAGE;
-    static constexpr int SMEM = 1024 + PIPES + WARPS * STAGES * 8 + (5 * SH_ROWS + 4) * 4;
+    static constexpr int SMEM = 1024 + PIPES + WARPS * STAGES * 8 + (7 * SH_ROWS + 4) * 4;
     static_assert(SMEM <= 232448, "more shared memory than a block can have");
 };
 
@@ -40,7 +40,9 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
     int* row_hi = row_lo + SH_ROWS;
     int* length = row_hi + SH_ROWS;                          // what rows share, and with whom
     int* id = length + SH_ROWS;
-    int* tile_units = id + SH_ROWS;
+    int* tile_lo = id + SH_ROWS;                            // the positions that tiles see
+    int* tile_hi = tile_lo + SH_ROWS;
+    int* tile_units = tile_hi + SH_ROWS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* pipe = smem + warp * C::STAGES * C::STAGE;
     uint64_t* bars = all_bars + warp * C::STAGES;
@@ -59,7 +61,10 @@ shared_own_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_
     }
     shared_cut_rows(p, upto, row_lo, row_hi, 16);            // ends with a barrier
     if (p.tile_cost > 0.f) {                                 // the tiles' kernel runs beside this one and has its share of the multiprocessors
-        if (warp == 0) *tile_units = shared_tile_units(p, length, id, 128 / group, D == 256 ? 64 : 128);
+        if (warp == 0) {
+            const int units = shared_tile_units(p, length, id, tile_lo, tile_hi, 128 / group, D == 256 ? 64 : 128);
+            if (lane == 0) *tile_units = units;
+        }
         __syncthreads();
         const int theirs = shared_tile_blocks(p, *tile_units, upto[p.rows], gridDim.x);
         if (theirs < blocks) blocks -= theirs;
