@@ -359,7 +359,8 @@ static bool shared_on_tensor_cores(int dtype, int hq, int hkv, int d, int dv, in
     return dtype == KB_DT_BF16 && d == dv && (d == 64 || d == 128 || d == 256) && page_size % 16 == 0 && hq / hkv <= 16;
 }
 
-// Where all rows' block tables together hold no more keys and values than this, every row reads what it sees by itself: the shared part comes out of
+// Where all rows' block tables together have room for no more keys and values than this (the tables' width, not what lies in them: a recorded launch's choice stays
+// while lengths change), every row reads what it sees by itself: the shared part comes out of
 // the second-level cache for all but the first, and the kernel over tiles, some 10 us before its first product, is not launched. As measured
 // (us, with tiles and without): 8 heads over 4 of 256, 2 rows sharing 64 positions (1 MB) 19 and 9, 16 sharing 1,024 (75 MB) 22 and 19, 8 sharing
 // 4,096 (138 MB) 30 and 26, 32 sharing 1,024 (153 MB) 22 and 26, 16 sharing 4,096 (277 MB) 29 and 38; 32 over 16 of 128, 8 sharing 1,024 (74 MB) 27 and
@@ -373,7 +374,8 @@ static SharedScratch shared_scratch(int rows, int hq, int hkv, int d) {         
 }
 // What a unit of a tile costs a multiprocessor, counted in units of 16 positions of a row; more than its bytes say, since a block over tiles takes
 // some 15 us to begin and to leave its pieces. As measured at 8, 12, 16, 24: 64 answers to 2,048 tokens, 16 heads over 8 of 256, 61, 58, 53, 54 us; 8
-// to 6,144, 8 over 4 of 256, 31, 27, 31, 36; two prompts and 34 requests, 32 over 16 of 128, 84, 76, 70, 68.
+// to 6,144, 8 over 4 of 256, 31, 27, 31, 36; two prompts and 34 requests, 32 over 16 of 128, 84, 76, 70, 68. (These three only, and before both kernels
+// counted the same units: the last takes 53 since.)
 static float shared_tile_cost(int d) { return d == 256 ? 14.f : 20.f; }
 
 // Floats of scratch memory: the tiles' pieces, the rows' pieces, then the cut.

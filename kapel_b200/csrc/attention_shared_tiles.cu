@@ -19,7 +19,8 @@
 //
 // What bounds it: 128 requests behind 16,384 positions, 32 heads over 16 of 128 (two tiles a kv head): 69 us, 500 Tflop/s. A unit of 128 positions takes
 // 3,200 clocks where its exponentials take 1,024 and its products as many: the sixteen warps wait for the same scores, load them, agree on m
-// and write their weights at the same time. Before the first scores a block takes some 7 us (the cut, the queries), which is most of what a tile
+// and write their weights at the same time. In tiles of few pairs it is the softmax of the quarter that is not full: its places without a pair see no position, so its
+// warps take every unit for one that not all of their pairs see, score by score (two exponentials and a reciprocal each under a soft cap). Before the first scores a block takes some 7 us (the cut, the queries), which is most of what a tile
 // of few units costs.
 #include "attention_shared_bf16.cuh"
 #include "tensor_map.cuh"
@@ -281,7 +282,7 @@ shared_tiles_kernel(const SharedParams p, const __grid_constant__ CUtensorMap ma
                     uint32_t x[PART];
                     sh_ld(lanes + (uint32_t)(C::COL_S + b * KEYS + share * PART), x);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    const bool edge = j0 < lo_max || j0 + PART > hi_min;         // some pair does not see all of it: the same for the whole warp
+                    const bool edge = j0 < lo_max || j0 + PART > hi_min;         // some pair does not see all of it (a place without one sees nothing): the same for the whole warp
                     float top = -INFINITY, far = 0.f;
                     if (edge) {
 #pragma unroll

@@ -28,10 +28,12 @@
 // made of 2^(n / 32) = 2^k T[n mod 32], n an integer within a roundoff of the nearest to 32 x / ln 2 (found in 32 bits), and a polynomial of degree 5 for what is left (the series' next term is below 3e-15): nine 64-bit operations, of which a multiprocessor does some 37 a
 // clock. Two entries of T share a bank, so a warp's loads take two turns at most.
 //
-// What bounds it, over 256,000 tokens: one row alone takes 15 us under top_k 50, of which the row's load is 3 and the rest some eight cluster
-// barriers and what lies between them; 26 under a nucleus of 0.95, of which 10 are the pass that adds up all weights and counts them (64-bit
-// operations, conversions and atomics of shared memory together: two tokens' weights side by side were no faster). 64 rows: 43 us under top_k 50
-// (1.5 TB/s), 73 without filters, 87 under a nucleus of 0.95 or 0.99.
+// What bounds it, over 256,000 tokens (recorded; logits of deviation 1.5 with 300 likely tokens above them, under a temperature of 0.8): one row alone
+// takes 15 us under top_k 50, of which the row's load is 3 and the rest some eight cluster barriers and what lies between them; 20 without filters; 27 under a nucleus of
+// 0.95, of which 10 are the pass that adds up all weights and counts them (two tokens' weights side by side were no faster). 64 rows: 34 us
+// under top_k 50 (1.9 TB/s), 63 without filters, 78 under a nucleus of 0.95 or 0.99: two rounds of clusters, one block a multiprocessor, with
+// nothing beside a row's chain of load, barriers, passes and sort; their 64-bit operations alone would take some 15. Where the nucleus is a third of all tokens (a normal distribution of
+// deviation 2) its border lies among more than the list holds and takes two passes more: one row 57 us, 64 rows 177.
 #include <cooperative_groups.h>
 #include <cfloat>
 #include "common.cuh"
@@ -929,7 +931,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1) sample_filtered_kernel(const Sf
 
 using namespace kb;
 
-// Blocks a row has at most: shares of SF_SHARE columns.
+// No more blocks are tried for a row once half as many would have no more than this many columns each.
 constexpr int SF_SHARE = 8192;
 
 // Clusters of `blocks` blocks that run at once; asked for once a device (their blocks fill a multiprocessor whatever their share, and lie in one part of the
@@ -972,7 +974,7 @@ extern "C" int kb_sample_filtered(int* tokens, const float* logits, const double
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     // Blocks a row: as many as make the rows' time least, which is the rounds of clusters times some 16 us and 0.45 ns a column of a share (what a
-    // nucleus takes). 15 clusters of eight run at once, 33 of four, 74 of two, 148 of one. As measured under a nucleus of 0.95 (us): 256,000 columns,
+    // nucleus takes). 15 clusters of eight run at once, 33 of four, 74 of two, 148 of one. As measured under a nucleus of 0.95 (us; the logits of the figures above): 256,000 columns,
     // of 12 rows 27 by eight blocks a row and 38 by four, of 16 rows 49 and 38, of 64 rows 116 and 76; 50,257 columns, of 12 rows 18, 20, 24 and 33 by
     // eight, four, two and one, of 40 rows 46, 35, 25 and 34, of 256 rows 249, 141, 94 and 66. (Blocks of 512 threads, two a multiprocessor, eight a row of
     // 256,000: 46 of 32 rows where four of 1,024 take 39, 85 of 64 where those take 76.)

@@ -1078,7 +1078,8 @@ def shared_prefix_attention(q, k_table, v_table, block_table, row_count, share_i
     """Attention of a decode step's single tokens [rows, hq, d] (row r is request r, its pages in row r of `block_table`, its own
     position the last of the `row_count[r]` it has seen) where requests share the pages of a prompt: rows that follow one another with the
     same `share_id` and `share_len` (int32 [rows]) have the same pages for their first share_len positions, and what they share is read
-    once for all of them, out of the block table of the one that sees furthest back. share_len is taken down to whole pages and to the row's
+    once for all of them, out of the block table of the one that sees furthest back (in bfloat16, where all block tables have room for no more than 144 MB,
+    by every row itself). share_len is taken down to whole pages and to the row's
     count; 0 shares nothing. Up to SHARED_PREFIX_ROWS rows. Window, soft cap and `sinks` as for `paged_attention_mma`; a row that
     sees nothing gives zeros. Every page with a position that a row sees has to be in its table; what lies in it behind the row's count, or before its
     window, may be anything, but that with a window shared values which only some rows of a group still see have to be finite in bfloat16."""
